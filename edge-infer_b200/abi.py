@@ -52,6 +52,15 @@ class View3(C.Structure):
     _fields_ = [("data", C.c_void_p), ("shape", C.c_size_t * 3), ("stride", C.c_size_t * 3)]
 
 
+class View4(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("shape", C.c_size_t * 4), ("stride", C.c_size_t * 4)]
+
+
+class RopeScaling(C.Structure):
+    _fields_ = [("kind", C.c_int32), ("factor", C.c_double), ("original_positions", C.c_double), ("fast", C.c_double),
+                ("slow", C.c_double), ("length", C.c_double)]
+
+
 class Array(C.Structure):
     _fields_ = [("data", C.c_void_p), ("size", C.c_size_t)]
 
@@ -137,6 +146,15 @@ PROTOTYPES = {
     "ei_attention_prefill_bf16": (_S, [C.POINTER(Context), View3, View3, View3, View3, _Z, _P, _Z]),
     "ei_attention_verify_bf16": (_S, [C.POINTER(Context), View3, View3, View3, View3, _P, _P, _Z]),
     "ei_attention_prefill_static_bf16": (_S, [C.POINTER(Context), View3, View3, View3, View3, _Z]),
+    "ei_build_rope_table_scaled": (_S, [_P, _Z, _Z, C.c_double, C.POINTER(RopeScaling)]),
+    "ei_qk_norm_rope_bf16": (_S, [C.POINTER(Context), View3, View3, View2, _P, _Z, View1, View1, C.c_float, C.c_int32, View3,
+                                  View3]),
+    "ei_attention_window_bf16": (_S, [C.POINTER(Context), View3, View4, View4, View3, _P, _Z, _Z, _Z]),
+    "ei_attention_shared_prefix_scratch_bytes": (_Z, [_Z, _Z, _Z, _Z]),
+    "ei_attention_shared_prefix_bf16": (_S, [C.POINTER(Context), View3, View3, View3, View4, View4, View3, _P, _Z, _P, _Z]),
+    "ei_attention_accumulate_scratch_bytes": (_Z, [_Z, _Z, _Z, _Z, _Z]),
+    "ei_attention_accumulate_bf16": (_S, [C.POINTER(Context), View3, View4, View4, View3, _P, _Z, View3, View3, _P, _Z]),
+    "ei_evict_kv_bf16": (_S, [C.POINTER(Context), View4, View4, View3, _P, _Z, _Z, _Z, View4, View4, View3, View3, _P]),
     "ei_sample_scratch_bytes": (_Z, [_Z, _Z]),
     "ei_sample_greedy_bf16": (_S, [C.POINTER(Context), View2, View1, _P, _Z]),
     "ei_verify_accept": (_S, [C.POINTER(Context), _P, _P, _Z, _P, _P, _P]),
@@ -224,6 +242,10 @@ def view2(t) -> View2:
 
 def view3(t) -> View3:
     return View3(t.data_ptr(), tuple(t.shape), tuple(t.stride()))
+
+
+def view4(t) -> View4:
+    return View4(t.data_ptr(), tuple(t.shape), tuple(t.stride()))
 
 
 def array(t) -> Array:

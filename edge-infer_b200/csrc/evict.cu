@@ -1,0 +1,169 @@
+// A cache cut to a budget: per sequence and KV head the first `sinks` tokens, the last `recent` and, of the others, those with
+// the largest accumulated weight, moved in order of position into another cache.
+//
+// Selection is exact: the place-th largest score is found bit by bit (two bits of the order-preserving integer key a step,
+// three counts each), scores above it stay, of those equal to it the ones with the lowest positions. Bound: the scores once,
+// the kept rows in and out; the selection's 16 steps are a chain of block-wide counts, some microseconds however few tokens,
+// so that the blocks which share a head's rows each repeat it (from their own copy of the keys in shared memory) instead of
+// waiting for one another, and then move a part of the rows each.
+#include "context_kernels.cuh"
+
+#include <algorithm>
+
+namespace ei {
+namespace {
+
+constexpr int kDim = 128;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kMoves = 4;          // tokens a warp has under way
+constexpr int kCachedKeys = 40960;  // keys that a block holds itself (160 KB); further ones are made from the scores again
+
+struct EvictShared {
+  int counts[2][kWarps][4];
+  int above[kWarps], ties[kWarps];
+};
+
+// Larger scores have larger keys; -0 is 0, and what is not a number comes last.
+__device__ __forceinline__ uint32_t key_of(float score) {
+  if (score != score) return 0u;
+  const uint32_t bits = __float_as_uint(score + 0.0f);
+  return bits ^ ((bits >> 31) ? 0xffffffffu : 0x80000000u);
+}
+
+// Block (part of the kept rows, KV head, sequence).
+__global__ void __launch_bounds__(kThreads) evict_kernel(const EvictParams p, int cached, int part_rows) {
+  extern __shared__ uint32_t evict_smem[];
+  EvictShared* const sh = reinterpret_cast<EvictShared*>(evict_smem);
+  int* const rows = reinterpret_cast<int*>(sh + 1);                    // [part_rows] tokens of this block's part
+  uint32_t* const keys = reinterpret_cast<uint32_t*>(rows + part_rows);  // [cached]
+  const int kv_head = blockIdx.y, sequence = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int length = p.lengths ? p.lengths[sequence] : p.length;
+  if (length < 0 || length > p.capacity) length = 0;
+  const int stay = min(length, p.budget);  // tokens of the result
+  const int part_first = blockIdx.x * part_rows, part_last = min(part_first + part_rows, p.budget);
+  const float* scores = p.scores + sequence * p.scores_sequence + kv_head * p.scores_head;
+  if (blockIdx.x == 0 && kv_head == 0 && threadIdx.x == 0) p.lengths_out[sequence] = stay;
+
+  if (length <= p.budget) {
+    for (int i = part_first + int(threadIdx.x); i < min(part_last, stay); i += kThreads) rows[i - part_first] = i;
+  } else {
+    // The tokens that compete: [sinks, length - recent).
+    const int from = p.sinks, to = length - p.recent;
+    for (int t = from + int(threadIdx.x); t < min(to, from + cached); t += kThreads) keys[t - from] = key_of(scores[t]);
+    __syncthreads();
+    auto key_at = [&](int t) { return t - from < cached ? keys[t - from] : key_of(scores[t]); };
+    const int place = p.budget - p.sinks - p.recent;  // of them stay
+    uint32_t threshold = 0;                            // the place-th largest key
+    if (place > 0) {
+      for (int shift = 30, step = 0; shift >= 0; shift -= 2, ++step) {
+        const uint32_t unit = 1u << shift;
+        int one = 0, two = 0, three = 0;  // keys at or above threshold + 1, 2, 3 units
+        for (int t = from + int(threadIdx.x); t < to; t += kThreads) {
+          const uint32_t key = key_at(t);
+          one += key >= threshold + unit;
+          two += key >= threshold + 2 * unit;
+          three += key >= threshold + 3 * unit;
+        }
+        one = __reduce_add_sync(0xffffffffu, one);
+        two = __reduce_add_sync(0xffffffffu, two);
+        three = __reduce_add_sync(0xffffffffu, three);
+        int(&mine)[4] = sh->counts[step & 1][warp];
+        if (lane == 0) mine[0] = one, mine[1] = two, mine[2] = three;
+        __syncthreads();
+        one = two = three = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          one += sh->counts[step & 1][w][0];
+          two += sh->counts[step & 1][w][1];
+          three += sh->counts[step & 1][w][2];
+        }
+        threshold += three >= place ? 3 * unit : two >= place ? 2 * unit : one >= place ? unit : 0u;
+      }
+    }
+    // Positions: a warp takes a stretch of tokens; how many before it stay comes from the other warps' counts.
+    const int span = ((to - from + kWarps - 1) / kWarps + 31) / 32 * 32;
+    const int first = min(from + warp * span, to), last = min(first + span, to);
+    int above = 0, ties = 0;
+    for (int t0 = first; t0 < last; t0 += 32) {
+      const int t = t0 + lane;
+      const uint32_t key = t < last ? key_at(t) : 0u;
+      above += __popc(__ballot_sync(0xffffffffu, t < last && key > threshold));
+      ties += __popc(__ballot_sync(0xffffffffu, t < last && key == threshold));
+    }
+    if (lane == 0) sh->above[warp] = above, sh->ties[warp] = ties;
+    __syncthreads();
+    int above_before = 0, ties_before = 0, above_all = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) above_before += sh->above[w], ties_before += sh->ties[w];
+      above_all += sh->above[w];
+    }
+    const int ties_stay = place > 0 ? place - above_all : 0;
+    auto put = [&](int index, int token) {
+      if (index >= part_first && index < part_last) rows[index - part_first] = token;
+    };
+    if (place > 0) {
+      for (int t0 = first; t0 < last; t0 += 32) {
+        const int t = t0 + lane;
+        const uint32_t key = t < last ? key_at(t) : 0u;
+        const uint32_t over = __ballot_sync(0xffffffffu, t < last && key > threshold);
+        const uint32_t equal = __ballot_sync(0xffffffffu, t < last && key == threshold);
+        const uint32_t below = (1u << lane) - 1;
+        const int tie = ties_before + __popc(equal & below);  // ties before this token
+        if ((over >> lane & 1) || ((equal >> lane & 1) && tie < ties_stay))
+          put(p.sinks + above_before + __popc(over & below) + min(tie, ties_stay), t);
+        above_before += __popc(over);
+        ties_before += __popc(equal);
+      }
+    }
+    for (int i = threadIdx.x; i < p.sinks; i += kThreads) put(i, i);
+    for (int i = threadIdx.x; i < p.recent; i += kThreads) put(p.budget - p.recent + i, length - p.recent + i);
+  }
+  __syncthreads();
+
+  const int moved = max(0, min(part_last, stay) - part_first);
+  for (int i = threadIdx.x; i < part_last - part_first; i += kThreads) {
+    const size_t at = size_t(part_first + i);
+    p.kept[sequence * p.kept_sequence + kv_head * p.kept_head + at] = i < moved ? rows[i] : -1;
+    if (i < moved) p.scores_out[sequence * p.scores_out_sequence + kv_head * p.scores_out_head + at] = scores[rows[i]];
+  }
+  // A warp moves a token's K (lanes 0-15) and V (16-31).
+  const CacheStrides& cache = lane < 16 ? p.k : p.v;
+  const bf16* source = cache.data + sequence * cache.sequence + kv_head * cache.head + (lane & 15) * 8;
+  bf16* target = lane < 16 ? p.k_out + sequence * p.k_out_sequence + kv_head * p.k_out_head
+                           : p.v_out + sequence * p.v_out_sequence + kv_head * p.v_out_head;
+  target += (lane & 15) * 8;
+  const size_t step = lane < 16 ? p.k_out_token : p.v_out_token;
+  for (int i0 = warp * kMoves; i0 < moved; i0 += kWarps * kMoves) {
+    uint4 held[kMoves];
+#pragma unroll
+    for (int u = 0; u < kMoves; ++u)
+      if (i0 + u < moved) held[u] = ldg_stream(source + size_t(rows[i0 + u]) * cache.token);
+#pragma unroll
+    for (int u = 0; u < kMoves; ++u)
+      if (i0 + u < moved) *reinterpret_cast<uint4*>(target + size_t(part_first + i0 + u) * step) = held[u];
+  }
+}
+
+}  // namespace
+
+void launch_evict(const EvictParams& p, int multiprocessors, cudaStream_t stream) {
+  const int units = p.sequences * p.kv_heads;
+  const int cached = std::max(0, std::min(p.capacity - p.sinks - p.recent, kCachedKeys));
+  // Parts of a head's rows: enough blocks for every SM, of 32 rows at least and 8192 at most (their list is in shared memory).
+  int parts = std::max(1, std::min((2 * multiprocessors + units - 1) / units, p.budget / 32));
+  parts = std::max(parts, (p.budget + 8191) / 8192);
+  const int part_rows = (p.budget + parts - 1) / parts;
+  const size_t shared = sizeof(EvictShared) + size_t(part_rows) * 4 + size_t(cached) * 4;
+  static thread_local int configured_device = -1;
+  int device = 0;
+  EI_CUDA(cudaGetDevice(&device));
+  if (configured_device != device) {
+    EI_CUDA(cudaFuncSetAttribute(evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 int(sizeof(EvictShared) + (8192 + kCachedKeys) * 4)));
+    configured_device = device;
+  }
+  launch(evict_kernel, dim3(unsigned((p.budget + part_rows - 1) / part_rows), unsigned(p.kv_heads), unsigned(p.sequences)), dim3(kThreads),
+         shared, stream, false, p, cached, part_rows);
+}
+
+}  // namespace ei

@@ -1,0 +1,520 @@
+// Attention of few query rows over a batch of caches: a sliding window with first tokens that stay visible, the own part of
+// sequences that share a prefix, and attention that also reports the weight every cached token received.
+//
+//   o_i = sum_t w_it v_t,  w_it = exp(q_i k_t / sqrt(128) - m_i) / l_i  over the tokens t that row i sees.
+//
+// A unit is 32 stacked query rows (row x query head of one KV head) of one sequence; 16 where no unit has more. The path is
+// bound by the bytes of K and V, so each is fetched once per unit and every warp streams on its own: a warp walks every
+// fourth tile of 32 tokens of its block with a private ring of three 8 KB buffers filled by TMA (K and V in turn: a tile's V
+// and the next tile's K travel while the scores are made) on its own mbarriers, so that the loop has no barrier of the block
+// and no empty barriers. Two blocks of 96 KB fit on an SM: eight warps, some 128 KB under way. Scores and products are
+// mma.sync (16 rows are all that a decode step has; a tcgen05 tile would be 128), weights are rounded to BF16 for the second
+// product only and their sum is of the rounded ones, so that the weights used add up to one exactly.
+// The blocks of a unit form a cluster (up to 16): they join (sums, maximum, sum) through distributed shared memory, each
+// finishing a part of the rows, so that there is no scratch, no second launch and a fixed order of every addition.
+//
+// Only tokens that some row of the unit sees are read: tiles start at the window's first token, sinks are a stretch of their
+// own. What a box brings beyond a stretch (other tokens, rows never written) is masked in the scores and cleared in V.
+#include "step_attention.cuh"
+
+#include "step_choice.hpp"
+
+#include <algorithm>
+#include <stdexcept>
+
+namespace ei {
+namespace {
+
+constexpr int kDim = 128;
+constexpr int kThreads = kStepWarps * 32;
+constexpr int kBuffer = kStepTile * kDim * 2;
+constexpr int kBuffers = 3;
+
+struct StepShared {
+  uint64_t full[kStepWarps][kBuffers];
+  float maxima[kStepWarps][kStepRows], sums[kStepWarps][kStepRows];
+  // Of the block, read by the others of the cluster.
+  float maximum[kStepRows], sum[kStepRows];
+  float factor[kStepMaxSplits][kStepRows];  // weight of each block's result in the joined one
+  float top[kStepRows], inverse[kStepRows];
+};
+constexpr size_t step_shared(int row_tiles) {
+  return size_t(kStepWarps) * kBuffers * kBuffer + (row_tiles > 1 ? size_t(kStepRows) * kDim * 2 : 0) + sizeof(StepShared) + 1024;
+}
+
+__device__ __forceinline__ int tile_offset(int token, int chunk) {
+  return (chunk >> 3) * (kStepTile * 128) + token * 128 + (((chunk & 7) ^ (token & 7)) << 4);
+}
+__device__ __forceinline__ int query_offset(int row, int chunk) {
+  return (chunk >> 3) * (kStepRows * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t remote_address(const void* own, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_address(own)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float remote_float(const void* own, uint32_t rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote_address(own, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 remote_float4(const void* own, uint32_t rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(remote_address(own, rank))
+               : "memory");
+  return v;
+}
+
+template <int kRowTiles, bool kWeights>
+__global__ void __launch_bounds__(kThreads, 2) step_attention_kernel(const __grid_constant__ StepAttentionParams p) {
+  extern __shared__ unsigned char step_smem_raw[];
+  unsigned char* const smem = step_smem_raw + ((1024u - (smem_address(step_smem_raw) & 1023u)) & 1023u);
+  unsigned char* const queries = smem + kStepWarps * kBuffers * kBuffer;
+  StepShared* const sh = reinterpret_cast<StepShared*>(queries + (kRowTiles > 1 ? kStepRows * kDim * 2 : 0));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const uint32_t rank = cluster_rank(), splits = cluster_size();
+  const int kv_head = blockIdx.x / splits, sequence = blockIdx.y;
+  const int group = p.heads / p.kv_heads, stacked = p.rows * group;
+  const int first_stacked = (p.first_group + int(blockIdx.z)) * kStepRows;
+  const int have = min(kStepRows, stacked - first_stacked);  // rows of this unit
+
+  int length = p.lengths ? p.lengths[sequence] : p.length;
+  if (length < 0 || length > p.capacity) length = 0;
+  // Position of the unit's first and last row; a negative one is no row of the sequence.
+  const int base = length - p.rows;
+  const int first_position = p.together ? length - 1 : base + first_stacked / group;
+  const int last_position = p.together ? length - 1 : base + (first_stacked + have - 1) / group;
+  const int end = kWeights ? length : last_position + 1;
+  const int low = max(0, min(first_position - p.window + 1, end));
+  const int sink_end = min(p.sinks, low);
+  const int sink_tiles = (sink_end + kStepTile - 1) / kStepTile;
+  const int tiles = sink_tiles + (max(0, end - low) + kStepTile - 1) / kStepTile;
+  const int first_tile = int((long long)tiles * rank / splits), last_tile = int((long long)tiles * (rank + 1) / splits);
+
+  unsigned char* const ring = smem + warp * kBuffers * kBuffer;
+  uint64_t* const full = sh->full[warp];
+  auto start_of = [&](int tile) { return tile < sink_tiles ? tile * kStepTile : low + (tile - sink_tiles) * kStepTile; };
+  // Item 2n is K and 2n + 1 V of this warp's n-th tile; item i lies in buffer i % 3.
+  auto request = [&](int item) {
+    const int tile = first_tile + warp + (item >> 1) * kStepWarps;
+    if (tile >= last_tile) return;
+    uint64_t* bar = &full[item % kBuffers];
+    mbarrier_expect_tx(bar, kBuffer);
+    tma_load_5d(ring + (item % kBuffers) * kBuffer, (item & 1) ? &p.v_map : &p.k_map, 0, start_of(tile), 0, kv_head, sequence, bar);
+  };
+  if (lane == 0) {
+    for (int b = 0; b < kBuffers; ++b) mbarrier_init(&full[b], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    for (int i = 0; i < kBuffers; ++i) request(i);
+  }
+  __syncwarp();
+  if (p.partial) grid_launch_dependents();  // this kernel follows nothing early; what joins its results waits for them
+
+  // Row i of the unit: stacked row first_stacked + i = query row * group + head of the group.
+  const long long row0 = (long long)sequence * p.rows;
+  auto row_of = [&](int i) { return (first_stacked + i) / group; };
+  auto query_at = [&](int i) {
+    const int r = row_of(i), h = first_stacked + i - r * group;
+    return p.q + (row0 + r) * p.q_stride + size_t(kv_head * group + h) * kDim;
+  };
+  uint32_t qa[kRowTiles == 1 ? 8 : 1][4];
+  if (kRowTiles == 1) {
+    const bf16* lo = query_at(g < have ? g : 0);
+    const bf16* hi = query_at(g + 8 < have ? g + 8 : 0);
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) {
+      qa[kRowTiles == 1 ? kk : 0][0] = g < have ? *reinterpret_cast<const uint32_t*>(lo + kk * 16 + 2 * c) : 0u;
+      qa[kRowTiles == 1 ? kk : 0][1] = g + 8 < have ? *reinterpret_cast<const uint32_t*>(hi + kk * 16 + 2 * c) : 0u;
+      qa[kRowTiles == 1 ? kk : 0][2] = g < have ? *reinterpret_cast<const uint32_t*>(lo + kk * 16 + 8 + 2 * c) : 0u;
+      qa[kRowTiles == 1 ? kk : 0][3] = g + 8 < have ? *reinterpret_cast<const uint32_t*>(hi + kk * 16 + 8 + 2 * c) : 0u;
+    }
+  } else {
+    for (int i = threadIdx.x; i < kStepRows * 16; i += kThreads) {
+      const int row = i >> 4, chunk = i & 15;
+      const uint4 v = row < have ? reinterpret_cast<const uint4*>(query_at(row))[chunk] : make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(queries + query_offset(row, chunk)) = v;
+    }
+    __syncthreads();
+  }
+
+  // Rows' positions: what a row sees is t <= limit and (t >= floor or t < sinks).
+  int limit[kRowTiles][2];
+#pragma unroll
+  for (int rt = 0; rt < kRowTiles; ++rt)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int i = rt * 16 + half * 8 + g;
+      limit[rt][half] = i < have ? (p.together ? length - 1 : base + row_of(i)) : -1;
+    }
+  const float exponent_scale = rsqrtf(float(kDim)) * kLog2e;
+  float* const raw = kWeights ? p.raw + (size_t(sequence) * p.kv_heads + kv_head) * p.raw_rows * p.raw_stride : nullptr;
+
+  float o[kRowTiles][16][4];
+  float m[kRowTiles][2], l[kRowTiles][2];
+#pragma unroll
+  for (int rt = 0; rt < kRowTiles; ++rt) {
+#pragma unroll
+    for (int d = 0; d < 16; ++d) o[rt][d][0] = o[rt][d][1] = o[rt][d][2] = o[rt][d][3] = 0.0f;
+    m[rt][0] = m[rt][1] = -INFINITY;
+    l[rt][0] = l[rt][1] = 0.0f;
+  }
+
+  bool ok = true;
+  int item = 0, buffer = 0;
+  uint32_t parity = 0;
+  for (int tile = first_tile + warp; tile < last_tile; tile += kStepWarps) {
+    ok = __all_sync(0xffffffffu, mbarrier_wait(&full[buffer], parity));
+    if (!ok) break;
+    const unsigned char* ks = ring + buffer * kBuffer;
+    const int first = start_of(tile);
+    const int stop = tile < sink_tiles ? sink_end : end;  // of the tile's stretch
+
+    float s[kRowTiles][4][4];
+#pragma unroll
+    for (int rt = 0; rt < kRowTiles; ++rt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[rt][j][0] = s[rt][j][1] = s[rt][j][2] = s[rt][j][3] = 0.0f;
+#pragma unroll
+    for (int pair = 0; pair < 4; ++pair) {
+      uint32_t a[kRowTiles][2][4];
+#pragma unroll
+      for (int rt = 0; rt < kRowTiles; ++rt)
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          if (kRowTiles == 1) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) a[rt][kk][x] = qa[kRowTiles == 1 ? 2 * pair + kk : 0][x];
+          } else {
+            ldmatrix_x4(a[rt][kk][0], a[rt][kk][1], a[rt][kk][2], a[rt][kk][3],
+                        queries + query_offset(rt * 16 + (lane & 15), 2 * (2 * pair + kk) + (lane >> 4)));
+          }
+        }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t b0, b1, b2, b3;
+        ldmatrix_x4(b0, b1, b2, b3, ks + tile_offset(j * 8 + (lane & 7), 4 * pair + (lane >> 3)));
+#pragma unroll
+        for (int rt = 0; rt < kRowTiles; ++rt) {
+          mma_bf16_16816(s[rt][j], a[rt][0][0], a[rt][0][1], a[rt][0][2], a[rt][0][3], b0, b1);
+          mma_bf16_16816(s[rt][j], a[rt][1][0], a[rt][1][1], a[rt][1][2], a[rt][1][3], b2, b3);
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) request(item + kBuffers);  // K has been read: its buffer takes the next tile's V
+    __syncwarp();
+
+    if (first + kStepTile > min(first_position + 1, stop) || (tile >= sink_tiles && first <= last_position - p.window)) {
+#pragma unroll
+      for (int rt = 0; rt < kRowTiles; ++rt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int t = first + j * 8 + 2 * c + (x & 1), at = limit[rt][x >> 1];
+            if (t >= stop || t > at || (t <= at - p.window && t >= p.sinks)) s[rt][j][x] = -INFINITY;
+          }
+    }
+    if (kWeights) {
+      // Scores as powers of two, for the weights when the row's maximum and sum are known.
+#pragma unroll
+      for (int rt = 0; rt < kRowTiles; ++rt)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int i = rt * 16 + half * 8 + g;
+          if (i < have) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<float2*>(raw + size_t(i) * p.raw_stride + size_t(tile) * kStepTile + j * 8 + 2 * c) =
+                  make_float2(s[rt][j][2 * half] * exponent_scale, s[rt][j][2 * half + 1] * exponent_scale);
+          }
+        }
+    }
+
+    uint32_t pa[kRowTiles][4][2];
+#pragma unroll
+    for (int rt = 0; rt < kRowTiles; ++rt) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float top = m[rt][half];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = fmaxf(top, fmaxf(s[rt][j][2 * half], s[rt][j][2 * half + 1]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // A row with nothing visible yet keeps -inf; 0 as the exponent's base then makes every weight 0.
+        const float reference = top == -INFINITY ? 0.0f : top, shift = reference * exponent_scale;
+        if (__any_sync(0xffffffffu, top != m[rt][half])) {
+          const float rescale = power_of_two((m[rt][half] - reference) * exponent_scale);  // exactly 1 where it stayed
+          l[rt][half] *= rescale;
+#pragma unroll
+          for (int d = 0; d < 16; ++d) {
+            o[rt][d][2 * half] *= rescale;
+            o[rt][d][2 * half + 1] *= rescale;
+          }
+          m[rt][half] = top;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float w0 = power_of_two(fmaf(s[rt][j][2 * half], exponent_scale, -shift));
+          const float w1 = power_of_two(fmaf(s[rt][j][2 * half + 1], exponent_scale, -shift));
+          const uint32_t both = pack_bf16(w0, w1);
+          l[rt][half] += kWeights ? w0 + w1 : bf16_lo(both) + bf16_hi(both);
+          pa[rt][j][half] = both;
+        }
+      }
+    }
+
+    ++item;
+    if (++buffer == kBuffers) buffer = 0, parity ^= 1;
+    ok = __all_sync(0xffffffffu, mbarrier_wait(&full[buffer], parity));
+    if (!ok) break;
+    unsigned char* vs = ring + buffer * kBuffer;
+    if (stop - first < kStepTile) {
+      // Nothing beyond the stretch may pass through a zero weight.
+      const int live = stop - first;
+      for (int i = lane; i < (kStepTile - live) * 16; i += 32)
+        *reinterpret_cast<uint4*>(vs + tile_offset(live + (i >> 4), i & 15)) = make_uint4(0, 0, 0, 0);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the buffer is a copy's again after this tile
+      __syncwarp();
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int d = 0; d < 16; d += 2) {
+        const int matrix = lane >> 3;
+        uint32_t b0, b1, b2, b3;
+        ldmatrix_x4_trans(b0, b1, b2, b3, vs + tile_offset(t * 16 + (matrix & 1) * 8 + (lane & 7), d + (matrix >> 1)));
+#pragma unroll
+        for (int rt = 0; rt < kRowTiles; ++rt) {
+          mma_bf16_16816(o[rt][d], pa[rt][2 * t][0], pa[rt][2 * t][1], pa[rt][2 * t + 1][0], pa[rt][2 * t + 1][1], b0, b1);
+          mma_bf16_16816(o[rt][d + 1], pa[rt][2 * t][0], pa[rt][2 * t][1], pa[rt][2 * t + 1][0], pa[rt][2 * t + 1][1], b2, b3);
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) request(item + kBuffers);
+    __syncwarp();
+    ++item;
+    if (++buffer == kBuffers) buffer = 0, parity ^= 1;
+  }
+  if (!ok) {
+    // A copy did not arrive within the bound. Those requested are waited for (bounded) before their buffers are used for
+    // anything else, and the unit's rows come out as NaN.
+    if (lane == 0) {
+      for (int i = item; i < item + kBuffers; ++i) {
+        if (first_tile + warp + (i >> 1) * kStepWarps < last_tile) mbarrier_wait(&full[i % kBuffers], (i / kBuffers) & 1);
+      }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int rt = 0; rt < kRowTiles; ++rt) l[rt][0] = l[rt][1] = __int_as_float(0x7fffffff), m[rt][0] = m[rt][1] = 0.0f;
+  }
+  grid_dependency_wait();  // what is joined below may be the preceding kernel's
+
+  // The warps' results: maxima first, then each warp's sums relative to the block's maximum.
+#pragma unroll
+  for (int rt = 0; rt < kRowTiles; ++rt)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      l[rt][half] += __shfl_xor_sync(0xffffffffu, l[rt][half], 1);
+      l[rt][half] += __shfl_xor_sync(0xffffffffu, l[rt][half], 2);
+      m[rt][half] *= exponent_scale;
+      if (c == 0) {
+        sh->maxima[warp][rt * 16 + half * 8 + g] = m[rt][half];
+        sh->sums[warp][rt * 16 + half * 8 + g] = l[rt][half];
+      }
+    }
+  __syncthreads();
+  constexpr int kUnitRows = kRowTiles * 16;
+  if (threadIdx.x < kUnitRows) {
+    const int i = threadIdx.x;
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kStepWarps; ++w) top = fmaxf(top, sh->maxima[w][i]);
+#pragma unroll
+    for (int w = 0; w < kStepWarps; ++w) {
+      const float part = sh->sums[w][i];
+      if (part != 0.0f) sum += part * power_of_two(sh->maxima[w][i] - top);  // a warp without a visible token has none
+    }
+    sh->maximum[i] = top;
+    sh->sum[i] = sum;
+  }
+  float* const area = reinterpret_cast<float*>(ring);  // [rows][128]
+#pragma unroll
+  for (int rt = 0; rt < kRowTiles; ++rt)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int i = rt * 16 + half * 8 + g;
+      const float top = fmaxf(fmaxf(sh->maxima[0][i], sh->maxima[1][i]), fmaxf(sh->maxima[2][i], sh->maxima[3][i]));
+      const float factor = m[rt][half] == -INFINITY ? 0.0f : power_of_two(m[rt][half] - top);
+#pragma unroll
+      for (int d = 0; d < 16; ++d)
+        *reinterpret_cast<float2*>(area + i * kDim + ((d * 8 + 2 * c) ^ ((i & 3) << 3))) =
+            make_float2(o[rt][d][2 * half] * factor, o[rt][d][2 * half + 1] * factor);
+    }
+  __syncthreads();
+  float* const block_area = reinterpret_cast<float*>(smem);
+  for (int i = threadIdx.x; i < kUnitRows * (kDim / 4); i += kThreads) {
+    float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < kStepWarps; ++w) {
+      const float4 v = reinterpret_cast<const float4*>(smem + w * kBuffers * kBuffer)[i];
+      total.x += v.x, total.y += v.y, total.z += v.z, total.w += v.w;
+    }
+    reinterpret_cast<float4*>(block_area)[i] = total;
+  }
+  if (splits > 1) cluster_sync();
+  else __syncthreads();
+
+  // Joined over the cluster and with what other kernels left.
+  if (threadIdx.x < kUnitRows) {
+    const int i = threadIdx.x;
+    const bool real = i < have && (p.together || base + row_of(i) >= 0);
+    float top = -INFINITY, sum = 0.0f;
+    for (uint32_t r = 0; r < splits; ++r) top = fmaxf(top, remote_float(&sh->maximum[i], r));
+    const size_t slots = size_t(p.sequences) * p.rows * p.heads;
+    size_t slot = 0;
+    if (i < have) {
+      const int r = row_of(i);
+      slot = size_t(row0 + r) * p.heads + kv_head * group + (first_stacked + i - r * group);
+    }
+    for (int j = 0; j < p.joined_count && real; ++j) top = fmaxf(top, p.joined[(j * slots + slot) * kStepPartial + 128]);
+    for (uint32_t r = 0; r < splits; ++r) {
+      const float part = remote_float(&sh->sum[i], r);
+      const float factor = part == 0.0f ? 0.0f : power_of_two(remote_float(&sh->maximum[i], r) - top);
+      sh->factor[r][i] = factor;
+      if (part != 0.0f) sum += part * factor;
+    }
+    for (int j = 0; j < p.joined_count && real; ++j) {
+      const float* from = p.joined + (j * slots + slot) * kStepPartial;
+      if (from[129] != 0.0f) sum += from[129] * power_of_two(from[128] - top);
+    }
+    sh->top[i] = top;
+    sh->inverse[i] = !real || sum == 0.0f ? 0.0f : p.partial ? sum : 1.0f / sum;
+  }
+  __syncthreads();
+  {
+    const int quads = have * (kDim / 4);
+    const int from = int((long long)quads * rank / splits), to = int((long long)quads * (rank + 1) / splits);
+    const size_t slots = size_t(p.sequences) * p.rows * p.heads;
+    for (int e = from + int(threadIdx.x); e < to; e += kThreads) {
+      const int i = e / (kDim / 4), quad = e % (kDim / 4);
+      const float* own = block_area + i * kDim + ((quad * 4) ^ ((i & 3) << 3));
+      float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (uint32_t r = 0; r < splits; ++r) {
+        const float factor = sh->factor[r][i];
+        if (factor == 0.0f) continue;
+        const float4 v = remote_float4(own, r);
+        total.x = fmaf(v.x, factor, total.x), total.y = fmaf(v.y, factor, total.y);
+        total.z = fmaf(v.z, factor, total.z), total.w = fmaf(v.w, factor, total.w);
+      }
+      const int r = row_of(i), h = kv_head * group + first_stacked + i - r * group;
+      const size_t slot = size_t(row0 + r) * p.heads + h;
+      for (int j = 0; j < p.joined_count; ++j) {
+        const float* other = p.joined + (j * slots + slot) * kStepPartial;
+        if (other[129] == 0.0f) continue;
+        const float factor = power_of_two(other[128] - sh->top[i]);
+        const float4 v = *reinterpret_cast<const float4*>(other + quad * 4);
+        total.x = fmaf(v.x, factor, total.x), total.y = fmaf(v.y, factor, total.y);
+        total.z = fmaf(v.z, factor, total.z), total.w = fmaf(v.w, factor, total.w);
+      }
+      const float inverse = sh->inverse[i];
+      if (p.partial) {
+        float* to_slot = p.partial + slot * kStepPartial;
+        *reinterpret_cast<float4*>(to_slot + quad * 4) = total;
+        if (quad == 0) to_slot[128] = sh->top[i], to_slot[129] = inverse;
+      } else {
+        uint2 packed = make_uint2(0u, 0u);
+        if (inverse != 0.0f) {  // also a NaN
+          packed.x = pack_bf16(total.x * inverse, total.y * inverse);
+          packed.y = pack_bf16(total.z * inverse, total.w * inverse);
+        }
+        *reinterpret_cast<uint2*>(p.out + (row0 + r) * p.out_stride + size_t(h) * kDim + quad * 4) = packed;
+      }
+    }
+  }
+  if (kWeights) {
+    // This block's tokens: the sum over the rows, in their order.
+    const float* scores = p.scores ? p.scores + sequence * p.scores_sequence + kv_head * p.scores_head : nullptr;
+    float* scores_out = p.scores_out + sequence * p.out_sequence + kv_head * p.out_head;
+    const int stop = min(last_tile * kStepTile, end);
+    for (int t = first_tile * kStepTile + int(threadIdx.x); t < stop; t += kThreads) {
+      float sum = 0.0f;
+      for (int i = 0; i < have; ++i) {
+        const float inverse = sh->inverse[i];
+        if (inverse != 0.0f) sum = fmaf(power_of_two(raw[size_t(i) * p.raw_stride + t] - sh->top[i]), inverse, sum);
+      }
+      scores_out[t] = (scores ? scores[t] : 0.0f) + sum;
+    }
+  }
+  if (splits > 1) cluster_sync();  // no block leaves while another reads its shared memory
+}
+
+auto step_kernel(bool two, bool weights) {
+  return two ? (weights ? step_attention_kernel<2, true> : step_attention_kernel<2, false>)
+             : (weights ? step_attention_kernel<1, true> : step_attention_kernel<1, false>);
+}
+
+void configure_step_kernels() {
+  static thread_local int configured_device = -1;
+  int device = 0;
+  EI_CUDA(cudaGetDevice(&device));
+  if (configured_device == device) return;
+  for (const bool two : {false, true})
+    for (const bool weights : {false, true}) {
+      EI_CUDA(cudaFuncSetAttribute(step_kernel(two, weights), cudaFuncAttributeMaxDynamicSharedMemorySize, int(step_shared(two ? 2 : 1))));
+      EI_CUDA(cudaFuncSetAttribute(step_kernel(two, weights), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    }
+  configured_device = device;
+}
+
+}  // namespace
+
+void encode_cache_map(CUtensorMap* map, const CacheStrides& cache, size_t capacity, size_t kv_heads, size_t sequences, int box_tokens) {
+  const cuuint64_t dims[5] = {64, cuuint64_t(capacity), 2, cuuint64_t(kv_heads), cuuint64_t(sequences)};
+  // An axis of extent 1 is not stepped along; its stride only has to be one that the encoder takes.
+  const cuuint64_t strides[4] = {cuuint64_t(capacity > 1 ? cache.token : kDim) * 2, 128, cuuint64_t(kv_heads > 1 ? cache.head : kDim) * 2,
+                                 cuuint64_t(sequences > 1 ? cache.sequence : kDim) * 2};
+  const cuuint32_t box[5] = {64, cuuint32_t(box_tokens), 2, 1, 1};
+  encode_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, cache.data, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, "K / V cache");
+}
+
+void launch_step_attention(const StepAttentionParams& p, size_t tokens, cudaStream_t stream, bool pdl) {
+  configure_step_kernels();
+  const int group = p.heads / p.kv_heads;
+  const bool two = size_t(p.rows) * group > 16;
+  const size_t units = size_t(p.kv_heads) * p.sequences * p.groups;
+  const int splits = step_splits(units, tokens, device_multiprocessors());
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(unsigned(p.kv_heads * splits), unsigned(p.sequences), unsigned(p.groups));
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = step_shared(two ? 2 : 1);
+  config.stream = stream;
+  cudaLaunchAttribute attributes[2]{};
+  attributes[0].id = cudaLaunchAttributeClusterDimension;
+  attributes[0].val.clusterDim.x = unsigned(splits);
+  attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
+  attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attributes;
+  config.numAttrs = pdl ? 2 : 1;
+  check_cuda(cudaLaunchKernelEx(&config, step_kernel(two, p.raw != nullptr), p), "cudaLaunchKernelEx");
+}
+
+}  // namespace ei

@@ -125,6 +125,115 @@ def attention_verify(ctx, q, k_capacity, v_capacity, output, device_offset, scra
                                               C.c_void_p(device_offset.data_ptr()), ptr, size))
 
 
+# ---- long contexts: rotation with norms, window, shared prefix, accumulated weights, eviction ------------------------
+ROPE_SCALINGS = {"plain": 0, "linear": 1, "yarn": 2, "bands": 3}
+
+
+def _expect(ctx, dtype: str, **tensors) -> None:
+    """Device, type and rank of what a C call only sees as pointers; `name=(tensor, rank)`."""
+    for name, (t, rank) in tensors.items():
+        if t.device.type != "cuda" or t.device.index != ctx.device:
+            raise ValueError(f"{name} is on {t.device}, the execution context on cuda:{ctx.device}")
+        if str(t.dtype) != dtype or t.dim() != rank:
+            raise ValueError(f"{name} must be a {dtype} tensor with {rank} axes, not {t.dtype} with {t.dim()}")
+
+
+def _lengths(ctx, lengths, sequences: int):
+    if lengths is None:
+        return None
+    _expect(ctx, "torch.int32", lengths=(lengths, 1))
+    if lengths.shape[0] != sequences or not lengths.is_contiguous():
+        raise ValueError("lengths must hold one packed value per sequence")
+    return lengths.data_ptr()
+
+
+def build_rope_table_scaled(max_positions: int, rotary_dim: int, theta: float, kind: str = "plain", factor: float = 1.0,
+                            original_positions: float = 0.0, fast: float = 32.0, slow: float = 1.0, length: float = 0.0):
+    """Rotation table for contexts longer than a model was trained on; kinds: plain, linear, yarn, bands."""
+    import numpy as np
+    if kind not in ROPE_SCALINGS:
+        raise ValueError(f"unknown RoPE scaling {kind!r}")
+    table = np.empty((max_positions, rotary_dim), dtype=np.float32)
+    scaling = abi.RopeScaling(ROPE_SCALINGS[kind], factor, original_positions, fast, slow, length)
+    abi.check(_lib().ei_build_rope_table_scaled(table.ctypes.data_as(C.c_void_p), max_positions, rotary_dim, theta,
+                                                C.byref(scaling)))
+    return table
+
+
+def qk_norm_rope(ctx, q, k, table, q_out, k_out, *, positions=None, offset: int = 0, q_weight=None, k_weight=None,
+                 epsilon: float = 1e-6, interleaved: bool = False) -> None:
+    """Norm of every query and key head (where a weight is given) and rotation of its first table.shape[1] values, in one
+    pass with one rounding. positions: int32 [rows] on the device, else offset + row. Outputs may be the inputs."""
+    _expect(ctx, "torch.bfloat16", q=(q, 3), k=(k, 3), q_out=(q_out, 3), k_out=(k_out, 3))
+    _expect(ctx, "torch.float32", table=(table, 2))
+    for weight in (q_weight, k_weight):
+        if weight is not None:
+            _expect(ctx, "torch.bfloat16", weight=(weight, 1))
+    if positions is not None:
+        _expect(ctx, "torch.int32", positions=(positions, 1))
+        if positions.shape[0] != q.shape[0] or not positions.is_contiguous():
+            raise ValueError("positions must hold one packed value per row")
+    abi.check(_lib().ei_qk_norm_rope_bf16(
+        C.byref(ctx), abi.view3(q), abi.view3(k), abi.view2(table), None if positions is None else positions.data_ptr(), offset,
+        abi.view1(q_weight), abi.view1(k_weight), epsilon, int(interleaved), abi.view3(q_out), abi.view3(k_out)))
+
+
+def attention_window(ctx, q, k, v, output, window: int, sinks: int = 0, *, lengths=None, length: int = 0) -> None:
+    """Causal attention of [sequences * rows, heads, 128] queries over caches [sequences, capacity, kv_heads, 128]: a row at
+    position p sees the tokens t <= p with t > p - window or t < sinks. lengths: int32 [sequences] on the device, the rows'
+    own tokens included, else `length` for all."""
+    _expect(ctx, "torch.bfloat16", q=(q, 3), k=(k, 4), v=(v, 4), output=(output, 3))
+    abi.check(_lib().ei_attention_window_bf16(C.byref(ctx), abi.view3(q), abi.view4(k), abi.view4(v), abi.view3(output),
+                                              _lengths(ctx, lengths, k.shape[0]), length, window, sinks))
+
+
+def attention_shared_prefix_scratch_bytes(q_rows: int, query_heads: int, kv_heads: int, prefix_length: int) -> int:
+    return _lib().ei_attention_shared_prefix_scratch_bytes(q_rows, query_heads, kv_heads, prefix_length)
+
+
+def attention_shared_prefix(ctx, q, prefix_k, prefix_v, k, v, output, scratch, *, lengths=None, length: int = 0) -> None:
+    """Causal attention of sequences that share their first tokens, prefix_k / prefix_v [prefix, kv_heads, 128], read once for
+    all of them; lengths and positions count each sequence's own tokens in k / v."""
+    _expect(ctx, "torch.bfloat16", q=(q, 3), prefix_k=(prefix_k, 3), prefix_v=(prefix_v, 3), k=(k, 4), v=(v, 4), output=(output, 3))
+    if scratch is not None:
+        _expect(ctx, str(scratch.dtype), scratch=(scratch, scratch.dim()))
+    ptr, size = _scratch(scratch)
+    abi.check(_lib().ei_attention_shared_prefix_bf16(
+        C.byref(ctx), abi.view3(q), abi.view3(prefix_k), abi.view3(prefix_v), abi.view4(k), abi.view4(v), abi.view3(output),
+        _lengths(ctx, lengths, k.shape[0]), length, ptr, size))
+
+
+def attention_accumulate_scratch_bytes(sequences: int, rows: int, query_heads: int, kv_heads: int, capacity: int) -> int:
+    return _lib().ei_attention_accumulate_scratch_bytes(sequences, rows, query_heads, kv_heads, capacity)
+
+
+def attention_accumulate(ctx, q, k, v, output, scores, scores_out, scratch, *, lengths=None, length: int = 0) -> None:
+    """Causal attention that also adds every token's softmax weights, over rows and a KV head's query heads, to scores
+    (FP32 [sequences, kv_heads, capacity]; None counts as zeros) and leaves them in scores_out (which may be scores)."""
+    _expect(ctx, "torch.bfloat16", q=(q, 3), k=(k, 4), v=(v, 4), output=(output, 3))
+    _expect(ctx, "torch.float32", scores_out=(scores_out, 3))
+    if scores is not None:
+        _expect(ctx, "torch.float32", scores=(scores, 3))
+    if scratch is not None:
+        _expect(ctx, str(scratch.dtype), scratch=(scratch, scratch.dim()))
+    ptr, size = _scratch(scratch)
+    abi.check(_lib().ei_attention_accumulate_bf16(
+        C.byref(ctx), abi.view3(q), abi.view4(k), abi.view4(v), abi.view3(output), _lengths(ctx, lengths, k.shape[0]), length,
+        abi.View3() if scores is None else abi.view3(scores), abi.view3(scores_out), ptr, size))
+
+
+def evict_kv(ctx, k, v, scores, k_out, v_out, scores_out, kept, lengths_out, sinks: int = 0, recent: int = 0, *, lengths=None,
+             length: int = 0) -> None:
+    """Cuts caches to the k_out.shape[1] tokens that are first, latest or heaviest, each KV head its own, in order of
+    position; kept (int32) receives their positions, -1 behind them, lengths_out (int32) the new lengths."""
+    _expect(ctx, "torch.bfloat16", k=(k, 4), v=(v, 4), k_out=(k_out, 4), v_out=(v_out, 4))
+    _expect(ctx, "torch.float32", scores=(scores, 3), scores_out=(scores_out, 3))
+    _expect(ctx, "torch.int32", kept=(kept, 3))
+    abi.check(_lib().ei_evict_kv_bf16(
+        C.byref(ctx), abi.view4(k), abi.view4(v), abi.view3(scores), _lengths(ctx, lengths, k.shape[0]), length, sinks, recent,
+        abi.view4(k_out), abi.view4(v_out), abi.view3(scores_out), abi.view3(kept), _lengths(ctx, lengths_out, k.shape[0])))
+
+
 def sample_scratch_bytes(rows: int, vocabulary: int) -> int:
     return _lib().ei_sample_scratch_bytes(rows, vocabulary)
 

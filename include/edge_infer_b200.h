@@ -44,6 +44,8 @@ typedef struct ei_view1 { void* data; size_t shape[1]; size_t stride[1]; } ei_vi
 typedef struct ei_view2 { void* data; size_t shape[2]; size_t stride[2]; } ei_view2;
 typedef struct ei_view3 { void* data; size_t shape[3]; size_t stride[3]; } ei_view3;
 typedef struct ei_array { void* data; size_t size; } ei_array;
+/* The same with four axes (no counterpart in the reference): a batch of caches. */
+typedef struct ei_view4 { void* data; size_t shape[4]; size_t stride[4]; } ei_view4;
 
 /* ref: operators/include/operators/cuda/execution.hpp:18-26 (ExecutionContext). `handle` is kept for
  * layout familiarity and ignored: no entry point calls cuBLAS. */
@@ -163,6 +165,67 @@ ei_status ei_attention_verify_bf16(const ei_context* ctx, ei_view3 q, ei_view3 k
 #define EI_ATTENTION_STATIC_SCRATCH_BYTES (10u * 1024u * 1024u)
 ei_status ei_attention_prefill_static_bf16(const ei_context* ctx, ei_view3 q, ei_view3 k, ei_view3 v,
                                            ei_view3 out, size_t offset);
+
+/* ---- long contexts ---------------------------------------------------------------------------
+ * No counterparts in the reference. Operators over a batch of caches k, v [sequences, capacity, kv_heads, 128] of any
+ * strides that are multiples of 16 bytes; queries and outputs are [sequences * rows, heads, 128] with the heads of a row
+ * adjacent, `rows` rows for each sequence, heads a multiple of kv_heads. `lengths` [sequences] (device; read when the kernel
+ * runs, so a captured graph follows it) says how many tokens of each cache live, the rows' own keys and values among them;
+ * null: `length` for every sequence. Row r of a sequence of n tokens stands at position n - rows + r. A row of negative
+ * position (a sequence shorter than its rows: padding on the left) comes out as zeros, and so does every row of a sequence
+ * whose length lies outside 0 .. capacity, which counts as empty. Keys and values that no row of the call may see are never
+ * used, whatever they hold. Scores, weights' sums and products are FP32, weights are rounded to BF16 for the product with the
+ * values, outputs once. The context's device has to be the current one; device pointers must belong to it. Nothing is
+ * allocated; results do not change from call to call. */
+
+/* Rotation tables for contexts longer than a model was trained on. EI_ROPE_LINEAR: every angle is divided by `factor`.
+ * EI_ROPE_YARN: frequencies that turn more than `fast` times over `original_positions` stay, those below `slow` turns are
+ * divided, a ramp over the pairs in between. EI_ROPE_BANDS: the same with the ramp over the number of turns. `length`
+ * multiplies sines and cosines; 0 means 1, for EI_ROPE_YARN 0.1 ln(factor) + 1 (1 where factor <= 1). */
+enum { EI_ROPE_PLAIN = 0, EI_ROPE_LINEAR = 1, EI_ROPE_YARN = 2, EI_ROPE_BANDS = 3 };
+typedef struct ei_rope_scaling {
+  int32_t kind;
+  double factor, original_positions, fast, slow, length;
+} ei_rope_scaling;
+/* Host table [max_positions, rotary_dim] as ei_build_rope_table lays it out ([2i] = sin, [2i+1] = cos), angles in 64 bits.
+ * `scaling` may be null. */
+ei_status ei_build_rope_table_scaled(float* host_table, size_t max_positions, size_t rotary_dim, double theta,
+                                     const ei_rope_scaling* scaling);
+/* Norms of queries [rows, heads, width] and keys [rows, kv_heads, width] for each head (q_weight, k_weight [width]; null data:
+ * no norm) and the rotation of the first rotary_dim = table.shape[1] values, in one pass, in FP32 with one rounding. Pairs are
+ * (i, i + rotary_dim / 2) or, interleaved != 0, (2i, 2i + 1). positions [rows] (device) or, null, offset + row; a row whose
+ * device-side position lies outside the table comes out as zeros. Outputs replace their inputs (same view) or lie apart from
+ * them: a slice of a cache stores the keys where attention reads them. width and rotary_dim: multiples of 16, width <= 512. */
+ei_status ei_qk_norm_rope_bf16(const ei_context* ctx, ei_view3 q, ei_view3 k, ei_view2 table, const int32_t* positions,
+                               size_t offset, ei_view1 q_weight, ei_view1 k_weight, float epsilon, int32_t interleaved,
+                               ei_view3 q_out, ei_view3 k_out);
+/* Causal attention with a sliding window: a row at position p sees the tokens t <= p with t > p - window or t < sinks.
+ * window >= 1. Only what some row sees is read. */
+ei_status ei_attention_window_bf16(const ei_context* ctx, ei_view3 q, ei_view4 k, ei_view4 v, ei_view3 out,
+                                   const int32_t* lengths, size_t length, size_t window, size_t sinks);
+/* Causal attention of sequences whose first tokens are the same: every row sees all of prefix_k, prefix_v
+ * [prefix, kv_heads, 128], which are read once for all sequences, and behind them its own cache as above (lengths and
+ * positions count the own tokens alone). An empty prefix is allowed. */
+size_t ei_attention_shared_prefix_scratch_bytes(size_t q_rows, size_t query_heads, size_t kv_heads, size_t prefix_length);
+ei_status ei_attention_shared_prefix_bf16(const ei_context* ctx, ei_view3 q, ei_view3 prefix_k, ei_view3 prefix_v, ei_view4 k,
+                                          ei_view4 v, ei_view3 out, const int32_t* lengths, size_t length, void* scratch,
+                                          size_t scratch_bytes);
+/* Causal attention that adds up what every cached token received: scores_out[s][j][t] = scores[s][j][t] + the softmax weights
+ * of token t, over the call's rows and the query heads of KV head j, for every token t of sequence s; FP32
+ * [sequences, kv_heads, capacity]. Places behind a sequence's length are left as they were. scores_out may be `scores` itself;
+ * scores with null data count as zeros. For steps of a few rows: 32 of rows * (heads / kv_heads) share a launch. */
+size_t ei_attention_accumulate_scratch_bytes(size_t sequences, size_t rows, size_t query_heads, size_t kv_heads, size_t capacity);
+ei_status ei_attention_accumulate_bf16(const ei_context* ctx, ei_view3 q, ei_view4 k, ei_view4 v, ei_view3 out,
+                                       const int32_t* lengths, size_t length, ei_view3 scores, ei_view3 scores_out, void* scratch,
+                                       size_t scratch_bytes);
+/* Cuts caches to a budget = k_out.shape[1]. A sequence of at most that many tokens is copied; of a longer one each KV head keeps
+ * its first `sinks`, its last `recent` and, of the others, the tokens with the largest scores (equal ones: the lowest positions;
+ * NaN ranks last), in order of position. kept [sequences, kv_heads, budget] int32 receives their positions, -1 behind them;
+ * lengths_out [sequences] the new lengths; scores_out [sequences, kv_heads, budget] the kept scores. Rows and scores behind a new
+ * length are left as they were. sinks + recent <= budget. Outputs lie apart from inputs. */
+ei_status ei_evict_kv_bf16(const ei_context* ctx, ei_view4 k, ei_view4 v, ei_view3 scores, const int32_t* lengths, size_t length,
+                           size_t sinks, size_t recent, ei_view4 k_out, ei_view4 v_out, ei_view3 scores_out, ei_view3 kept,
+                           int32_t* lengths_out);
 
 /* ---- greedy sampling and acceptance -------------------------------------------------------------- */
 /* Bytes of scratch for ei_sample_greedy_bf16. */
