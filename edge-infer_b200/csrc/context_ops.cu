@@ -3,6 +3,7 @@
 #include "abi_checks.cuh"
 #include "abi_util.cuh"
 #include "context_kernels.cuh"
+#include "span_attention.cuh"
 #include "step_choice.hpp"
 
 #include <algorithm>
@@ -14,6 +15,10 @@ using namespace ei;
 namespace {
 
 constexpr size_t kHeadWidth = 128;
+// From so many stacked rows (rows x query heads of a KV head) on the tensor-core kernel of many rows takes over.
+constexpr size_t kSpanWindowRows = 128;
+constexpr size_t kSpanPrefixRows = 128;
+constexpr int kSpanBlocks = 148;  // that a prefix is cut into at most: the blocks that fit this chip at once
 constexpr size_t kMostTokens = size_t(1) << 30;  // of a cache: positions and windows stay clear of 2^31
 
 // The context's device has to be the current one: launches, tensor maps and kernel attributes go there. Asked for last, so
@@ -113,8 +118,18 @@ StepAttentionParams attention_of(const ei_view3& q, const ei_view4& k, const ei_
   return p;
 }
 void encode_maps(StepAttentionParams* p, const CacheStrides& keys, const CacheStrides& values) {
-  encode_cache_map(&p->k_map, keys, size_t(p->capacity), size_t(p->kv_heads), size_t(p->sequences), kStepTile);
-  encode_cache_map(&p->v_map, values, size_t(p->capacity), size_t(p->kv_heads), size_t(p->sequences), kStepTile);
+  encode_cache_map(&p->k_map, keys, size_t(p->capacity), size_t(p->kv_heads), size_t(p->sequences), kStepTile, 2);
+  encode_cache_map(&p->v_map, values, size_t(p->capacity), size_t(p->kv_heads), size_t(p->sequences), kStepTile, 2);
+}
+// The same rows and caches for the many-row kernel.
+SpanAttentionParams span_of(const StepAttentionParams& p, const CacheStrides& keys, const CacheStrides& values) {
+  SpanAttentionParams s{};
+  s.q = p.q, s.q_stride = p.q_stride, s.out = p.out, s.out_stride = p.out_stride;
+  s.rows = p.rows, s.heads = p.heads, s.kv_heads = p.kv_heads, s.sequences = p.sequences, s.capacity = p.capacity;
+  s.lengths = p.lengths, s.length = p.length, s.window = p.window, s.sinks = p.sinks, s.together = p.together;
+  encode_cache_map(&s.k_map, keys, size_t(p.capacity), size_t(p.kv_heads), size_t(p.sequences), kSpanBox, 1);
+  encode_cache_map(&s.v_map, values, size_t(p.capacity), size_t(p.kv_heads), size_t(p.sequences), kSpanBox, 1);
+  return s;
 }
 size_t most_tokens(const StepAttentionParams& p) { return size_t(p.lengths ? p.capacity : p.length); }
 
@@ -234,6 +249,11 @@ ei_status ei_attention_window_bf16(const ei_context* ctx, ei_view3 q, ei_view4 k
     p.window = int(std::min(window, kMostTokens));
     p.sinks = int(std::min(sinks, kMostTokens));
     expect_current_device(ctx);
+    const size_t stacked = size_t(p.rows) * (p.heads / p.kv_heads);
+    if (stacked >= kSpanWindowRows) {
+      launch_span_attention(span_of(p, keys, values), stream);
+      return;
+    }
     encode_maps(&p, keys, values);
     const size_t seen = std::min(most_tokens(p), size_t(p.window) + size_t(p.sinks) + kStepRows);
     launch_step_attention(p, seen, stream, false);
@@ -241,8 +261,12 @@ ei_status ei_attention_window_bf16(const ei_context* ctx, ei_view3 q, ei_view4 k
 }
 
 size_t ei_attention_shared_prefix_scratch_bytes(size_t q_rows, size_t query_heads, size_t kv_heads, size_t prefix_length) {
-  (void)kv_heads;
-  return prefix_length ? q_rows * query_heads * kStepPartial * sizeof(float) : 0;
+  if (!prefix_length || !kv_heads) return 0;
+  const size_t stacked = q_rows * (query_heads / kv_heads);
+  size_t partials = 1;
+  if (stacked >= kSpanPrefixRows)
+    partials = size_t(span_splits((stacked + kSpanRows - 1) / kSpanRows, prefix_length, int(kv_heads), kSpanBlocks).partials());
+  return partials * q_rows * query_heads * kStepPartial * sizeof(float);
 }
 
 ei_status ei_attention_shared_prefix_bf16(const ei_context* ctx, ei_view3 q, ei_view3 prefix_k, ei_view3 prefix_v, ei_view4 k, ei_view4 v,
@@ -274,10 +298,22 @@ ei_status ei_attention_shared_prefix_bf16(const ei_context* ctx, ei_view3 q, ei_
       first.together = true;
       first.groups = step_groups(first.rows, first.heads / first.kv_heads);
       first.partial = static_cast<float*>(scratch);
-      encode_maps(&first, first_keys, first_values);
-      launch_step_attention(first, prefix, stream, false);
-      own.joined = static_cast<const float*>(scratch);
-      own.joined_count = 1;
+      own.joined = first.partial;
+      own.joined_border = 0;
+      own.joined_counts[1] = 1;
+      const size_t stacked = q.shape[0] * (q.shape[1] / k.shape[2]);
+      if (stacked >= kSpanPrefixRows) {
+        SpanAttentionParams span = span_of(first, first_keys, first_values);
+        span.splits = span_splits((stacked + kSpanRows - 1) / kSpanRows, prefix, first.kv_heads, kSpanBlocks);
+        span.partial = first.partial;
+        own.joined_border = span.splits.pairs * 2 * kSpanRows;
+        own.joined_counts[0] = span.splits.pair_splits;
+        own.joined_counts[1] = 2 * span.splits.single_splits;
+        launch_span_attention(span, stream);
+      } else {
+        encode_maps(&first, first_keys, first_values);
+        launch_step_attention(first, prefix, stream, false);
+      }
     }
     launch_step_attention(own, most_tokens(own), stream, prefix > 0);
   });

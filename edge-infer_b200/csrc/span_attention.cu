@@ -1,0 +1,468 @@
+// Attention of many query rows over caches on tcgen05: prompts with a sliding window and first tokens that stay visible, and
+// the rows of all sequences over a prefix that they share.
+//
+// A block owns two query tiles of 128 stacked rows (row x query head of one KV head) and walks its tokens in tiles of 128. Per
+// tile and query tile: S = Q K^T into tensor memory, a thread per row takes its 128 scores out, makes the weights relative to
+// its running maximum and puts them back as BF16 over the scores, from where they are the A operand of O += P V (V as it stands
+// in the cache is that product's N-major B operand). While one query tile's weights are made, the tensor cores work for the
+// other: 512 columns of tensor memory are the two tiles' scores and outputs. The bound is the chain's slower side, 2 x 128 x 128
+// exponentials at 16 a cycle and four products of 128 x 128 x 128 at 8192 multiply-adds a cycle: 2048 cycles either way.
+//
+// A running maximum may lag the true one by 2^8 (weights up to 256 are as exact in BF16 as those up to 1), so that the
+// outputs are hardly ever taken out of tensor memory to be rescaled; the sum is of the rounded weights, so that those used
+// add up to one exactly and a row that one token dominates comes out as that token's values.
+//
+// Tokens are a list of boxes of 32, first those of the sinks, then those of the window of the block's rows; four make a tile, so
+// that a few sinks do not cost a tile of their own. What a box holds beyond its stretch is masked in the scores and cleared
+// in V. A prefix is cut into stretches over the blocks (span_choice.hpp); an odd last query tile has both halves of its
+// blocks, which then take every other tile of tokens.
+//
+// Roles of the twelve warps: 0-3 and 4-7 the weights of one half each, 8 the copies, 9 and 10 the MMAs of one half each, 11 the
+// tensor memory. K and V tiles of 32 KB go through a ring of five buffers. Every wait is bounded: a role whose wait runs out
+// raises `abort`, which every other wait polls; when all roles have left, the copies and MMAs in flight are waited for
+// (bounded), the block's rows come out as NaN and the tensor memory is freed.
+#include "span_attention.cuh"
+
+#include "prompt_attention.cuh"
+
+#include <algorithm>
+
+namespace ei {
+namespace {
+
+constexpr int kDim = 128;
+constexpr int kThreads = 384;
+constexpr int kHalfBytes = kSpanTile * 128;  // 64 values of a tile's tokens
+constexpr int kBufferBytes = 2 * kHalfBytes;
+constexpr int kBoxBytes = kSpanBox * 128;
+constexpr int kBoxes = kSpanTile / kSpanBox;
+constexpr int kBuffers = 5;
+constexpr int kQueryBytes = 2 * kSpanRows * 128;
+constexpr float kSlack = 8.0f;  // powers of two
+constexpr size_t kSpanSharedBytes = size_t(2) * kQueryBytes + size_t(kBuffers) * kBufferBytes + 1024 + 512;
+static_assert(kSpanSharedBytes <= 227 * 1024, "a block's buffers fit an SM");
+
+struct SpanShared {
+  uint64_t full[kBuffers], empty[kBuffers];  // K and V tiles in turn
+  uint64_t queries[2];                       // a query tile is in shared memory
+  uint64_t scores[2], weights[2];            // of a half: S computed, P written
+  uint64_t added[2];                         // O holds the tile's product
+  uint64_t done;                             // every MMA issued has completed
+  uint32_t tmem_base;
+  volatile int abort;
+  int issued, query_tiles;  // items, and a bit for each query tile, whose copies were requested
+};
+static_assert(sizeof(SpanShared) <= 512, "the block's state lies behind the ring");
+
+__device__ __forceinline__ void tmem_request32(uint32_t address, uint32_t* r) {
+  __syncwarp();
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(address)
+      : "memory");
+}
+// Waits for the loads requested; the registers pass through so that nothing reads them earlier.
+__device__ __forceinline__ void tmem_loaded32(uint32_t* r) {
+  __syncwarp();
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+                 "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+                 "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
+
+__global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __grid_constant__ SpanAttentionParams p) {
+  extern __shared__ unsigned char span_smem_raw[];
+  unsigned char* const smem = span_smem_raw + ((1024u - (smem_address(span_smem_raw) & 1023u)) & 1023u);
+  unsigned char* const ring = smem + 2 * kQueryBytes;
+  SpanShared* const sh = reinterpret_cast<SpanShared*>(ring + kBuffers * kBufferBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kv_head = blockIdx.x, sequence = blockIdx.z;
+  const int group = p.heads / p.kv_heads, stacked = p.rows * group;
+
+  // ---- what this block does ----
+  int length = p.lengths ? p.lengths[sequence] : p.length;
+  if (length < 0 || length > p.capacity) length = 0;
+  int first_tile;             // query tile of half 0
+  bool shared_tokens = true;  // both halves read every tile of tokens (of two query tiles); else every other (of one)
+  int partial_index[2] = {0, 0};
+  int box_begin = 0, low = 0, sink_end = 0, sink_boxes = 0, box_end, end;
+  int first_position[2], last_position[2];  // of a half's rows
+  const int base = length - p.rows;
+  if (p.together) {
+    const int y = blockIdx.y;
+    int split, splits;
+    if (y < p.splits.pairs * p.splits.pair_splits) {
+      first_tile = y / p.splits.pair_splits * 2;
+      splits = p.splits.pair_splits;
+      split = y - first_tile / 2 * splits;
+      partial_index[0] = partial_index[1] = split;
+    } else {
+      first_tile = p.splits.pairs * 2;
+      shared_tokens = false;
+      splits = p.splits.single_splits;
+      split = y - p.splits.pairs * p.splits.pair_splits;
+      partial_index[0] = 2 * split, partial_index[1] = 2 * split + 1;
+    }
+    const int tiles = (length + kSpanTile - 1) / kSpanTile;
+    box_begin = int((long long)tiles * split / splits) * kBoxes;
+    end = length;
+    box_end = min(int((long long)tiles * (split + 1) / splits) * kBoxes, (end + kSpanBox - 1) / kSpanBox);
+    first_position[0] = first_position[1] = last_position[0] = last_position[1] = length - 1;
+  } else {
+    first_tile = (int(gridDim.y) - 1 - int(blockIdx.y)) * 2;  // the longest histories first
+    for (int half = 0; half < 2; ++half) {
+      const int from = (first_tile + half) * kSpanRows;
+      first_position[half] = base + min(from, stacked - 1) / group;
+      last_position[half] = base + min(from + kSpanRows - 1, stacked - 1) / group;
+    }
+    end = max(0, last_position[1] + 1);
+    low = max(0, min(first_position[0] - p.window + 1, end));
+    sink_end = min(p.sinks, low);
+    sink_boxes = (sink_end + kSpanBox - 1) / kSpanBox;
+    box_end = sink_boxes + (end - low + kSpanBox - 1) / kSpanBox;
+  }
+  const int items = (box_end - box_begin + kBoxes - 1) / kBoxes;  // tiles of tokens
+  auto start_of = [&](int box) { return box < sink_boxes ? box * kSpanBox : low + (box - sink_boxes) * kSpanBox; };
+  auto stop_of = [&](int box) { return box >= box_end ? 0 : box < sink_boxes ? sink_end : end; };
+  // Tiles that a half takes: all up to its last row's position, or every other.
+  auto tiles_of = [&](int half) {
+    if (!shared_tokens) return (items + 1 - half) / 2;
+    if ((first_tile + half) * kSpanRows >= stacked) return 0;
+    if (p.together) return items;
+    const int position = last_position[half];
+    if (position < 0) return 0;
+    const int boxes = position < low ? (min(sink_end, position + 1) + kSpanBox - 1) / kSpanBox : sink_boxes + (position - low) / kSpanBox + 1;
+    return min(items, (boxes + kBoxes - 1) / kBoxes);
+  };
+  const int tiles[2] = {tiles_of(0), tiles_of(1)};
+  auto item_of = [&](int half, int t) { return shared_tokens ? t : 2 * t + half; };
+
+  if (threadIdx.x == 0) {
+    for (int b = 0; b < kBuffers; ++b) {
+      mbarrier_init(&sh->full[b], 1);
+      mbarrier_init(&sh->empty[b], shared_tokens ? 2 : 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbarrier_init(&sh->queries[i], p.copied_queries ? 1 : 4);
+      mbarrier_init(&sh->scores[i], 1);
+      mbarrier_init(&sh->weights[i], 4);
+      mbarrier_init(&sh->added[i], 1);
+    }
+    mbarrier_init(&sh->done, 2);
+    sh->abort = 0;
+    sh->issued = sh->query_tiles = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 11) tmem_alloc(&sh->tmem_base, 512);
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = sh->tmem_base;
+  if (p.together) grid_launch_dependents();  // launched in plain stream order: all that came before has completed
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (mbarrier_test_wait(bar, parity)) return true;
+    for (uint32_t polls = 0; polls < kTmaWaitLimit; ++polls) {
+      if (mbarrier_try_wait(bar, parity)) return true;
+      if (sh->abort) return false;
+    }
+    sh->abort = 1;
+    return false;
+  };
+  auto query_tile_of = [&](int half) { return shared_tokens ? first_tile + half : first_tile; };
+  const long long row0 = (long long)sequence * p.rows;
+
+  // The row of a softmax thread.
+  const int half = (warp >> 2) & 1, row_of_tile = threadIdx.x & (kSpanRows - 1);
+  const int index = query_tile_of(half) * kSpanRows + row_of_tile;
+  const bool live = warp < 8 && index < stacked;
+  const int row = live ? index / group : 0, head = kv_head * group + (live ? index - row * group : 0);
+  float* const partial =
+      p.partial + ((size_t(partial_index[half]) * p.sequences * p.rows + row0 + row) * p.heads + head) * kStepPartial;
+  bf16* const out = p.out + (row0 + row) * p.out_stride + size_t(head) * kDim;
+
+  if (warp < 8) {
+    // ---- weights: thread = query row ----
+    if (!p.copied_queries && (shared_tokens || half == 0)) {
+      unsigned char* const own = smem + half * kQueryBytes + row_of_tile * 128;
+      const bf16* q = p.q + (row0 + row) * p.q_stride + size_t(head) * kDim;
+#pragma unroll 1
+      for (int part = 0; part < 2; ++part) {
+        uint4 held[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) held[i] = live ? reinterpret_cast<const uint4*>(q + part * 64)[i] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(own + part * kSpanRows * 128 + ((i ^ (row_of_tile & 7)) << 4)) = held[i];
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbarrier_arrive(&sh->queries[half]);
+    }
+    const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+    const uint32_t at = tmem + lanes + half * 256, outputs = at + 128;
+    const int last = p.together ? length - 1 : base + row;
+    const bool some_live = __any_sync(0xffffffffu, live);
+    const float exponent_scale = rsqrtf(float(kDim)) * kLog2e;
+    float maximum = -INFINITY, sum = 0.0f;
+    bool ok = true;
+    for (int t = 0; t < tiles[half]; ++t) {
+      const int item = item_of(half, t), box0 = box_begin + item * kBoxes;
+      ok = __all_sync(0xffffffffu, wait(&sh->scores[half], t & 1));
+      if (!ok) break;
+      tcgen05_fence_after();
+      // Whether the tile holds anything that some row of the half does not see, or that is no token of the list.
+      bool masked = false, partial_tile = false;
+#pragma unroll
+      for (int b = 0; b < kBoxes; ++b) {
+        const int start = start_of(box0 + b), stop = stop_of(box0 + b);
+        partial_tile |= start + kSpanBox > stop;
+        masked |= start + kSpanBox > min(stop, first_position[half] + 1) ||
+                  (start <= last_position[half] - p.window && start + kSpanBox > p.sinks);
+      }
+      if (some_live) {
+        uint32_t s[4][32];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tmem_request32(at + i * 32, s[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tmem_loaded32(s[i]);
+        if (masked) {
+#pragma unroll
+          for (int b = 0; b < kBoxes; ++b) {
+            const int start = start_of(box0 + b);
+            const int visible = min(stop_of(box0 + b), last + 1) - start;                // places below it
+            const int hidden = p.sinks - start, shown = last - p.window - start;         // but not hidden .. shown
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j >= visible || (j >= hidden && j <= shown)) s[b][j] = 0xff800000u;
+          }
+        }
+        float tops[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          tops[i] = __uint_as_float(s[i][0]);
+#pragma unroll
+          for (int j = 1; j < 32; ++j) tops[i] = fmaxf(tops[i], __uint_as_float(s[i][j]));
+        }
+        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        const bool moved = maximum == -INFINITY ? top != -INFINITY : (top - maximum) * exponent_scale > kSlack;
+        const float previous = maximum;
+        if (moved) maximum = top;
+        // A row with nothing visible yet keeps -inf; 0 as the exponent's base then makes every weight 0.
+        const float reference = maximum == -INFINITY ? 0.0f : maximum, shift = -reference * exponent_scale;
+        const float rescale = moved ? power_of_two((previous - reference) * exponent_scale) : 1.0f;
+        const float2 scales = make_float2(exponent_scale, exponent_scale), shifts = make_float2(shift, shift);
+        float2 parts[2] = {};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t packed[16];
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const float2 x = fma_pair(make_float2(__uint_as_float(s[i][j]), __uint_as_float(s[i][j + 1])), scales, shifts);
+            const uint32_t both = pack_bf16(power_of_two(x.x), power_of_two(x.y));
+            packed[j / 2] = both;
+            parts[j / 2 & 1] = add_pair(parts[j / 2 & 1], make_float2(bf16_lo(both), bf16_hi(both)));
+          }
+          tmem_store16(at + i * 16, packed);
+        }
+        const float2 total = add_pair(parts[0], parts[1]);
+        sum = sum * rescale + (total.x + total.y);
+        if (t > 0 && __any_sync(0xffffffffu, moved)) {
+          ok = __all_sync(0xffffffffu, wait(&sh->added[half], (t - 1) & 1));
+          if (!ok) break;
+          tcgen05_fence_after();
+#pragma unroll 1
+          for (int i = 0; i < 4; ++i) {
+            uint32_t a[32];
+            tmem_request32(outputs + i * 32, a);
+            tmem_loaded32(a);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) a[j] = __float_as_uint(__uint_as_float(a[j]) * rescale);
+            tmem_store16(outputs + i * 32, *reinterpret_cast<uint32_t(*)[16]>(a));
+            tmem_store16(outputs + i * 32 + 16, *reinterpret_cast<uint32_t(*)[16]>(a + 16));
+          }
+        }
+      }
+      if (partial_tile) {
+        // V's rows that are no token of the list are cleared: nothing there may pass through a zero weight. (Both halves'
+        // warps do it before they hand over their weights, with the same zeros.)
+        const int v_item = 2 * item + 1;
+        ok = __all_sync(0xffffffffu, wait(&sh->full[v_item % kBuffers], (v_item / kBuffers) & 1));
+        if (!ok) break;
+        unsigned char* values = ring + (v_item % kBuffers) * kBufferBytes;
+#pragma unroll
+        for (int b = 0; b < kBoxes; ++b) {
+          const int have = min(kSpanBox, max(0, stop_of(box0 + b) - start_of(box0 + b)));
+          for (int i = row_of_tile; i < (kSpanBox - have) * 16; i += kSpanRows)
+            *reinterpret_cast<uint4*>(values + (i & 1) * kHalfBytes + (b * kSpanBox + have + (i >> 4)) * 128 + ((i >> 1) & 7) * 16) =
+                make_uint4(0, 0, 0, 0);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
+      tmem_stored();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbarrier_arrive(&sh->weights[half]);
+    }
+    const bool any = tiles[half] > 0;
+    if (any) ok = ok && __all_sync(0xffffffffu, wait(&sh->added[half], (tiles[half] - 1) & 1));
+    if (ok) {
+      tcgen05_fence_after();
+      const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+        uint32_t v[32];
+        if (any) {
+          tmem_request32(outputs + i * 32, v);
+          tmem_loaded32(v);
+        }
+        if (!live) continue;
+        if (p.together) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<uint4*>(partial + i * 32 + j) =
+                any ? make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]) : make_uint4(0, 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            uint4 packed = make_uint4(0, 0, 0, 0);
+            if (inverse != 0.0f) {  // also a NaN
+              packed.x = pack_bf16(__uint_as_float(v[j]) * inverse, __uint_as_float(v[j + 1]) * inverse);
+              packed.y = pack_bf16(__uint_as_float(v[j + 2]) * inverse, __uint_as_float(v[j + 3]) * inverse);
+              packed.z = pack_bf16(__uint_as_float(v[j + 4]) * inverse, __uint_as_float(v[j + 5]) * inverse);
+              packed.w = pack_bf16(__uint_as_float(v[j + 6]) * inverse, __uint_as_float(v[j + 7]) * inverse);
+            }
+            *reinterpret_cast<uint4*>(out + i * 32 + j) = packed;
+          }
+        }
+      }
+      if (live && p.together) *reinterpret_cast<float2*>(partial + kDim) = make_float2(maximum * exponent_scale, sum);
+    }
+  } else if (warp == 8) {
+    // ---- copies ----
+    if (lane == 0) {
+      if (p.copied_queries)
+        for (int i = 0; i < (shared_tokens ? 2 : 1); ++i) {
+          if (tiles[i] == 0) continue;
+          mbarrier_expect_tx(&sh->queries[i], uint32_t(kQueryBytes));
+          for (int part = 0; part < 2; ++part)
+            tma_load_5d(smem + i * kQueryBytes + part * kSpanRows * 128, &p.q_map, 0, 0, int(row0) + query_tile_of(i) * kSpanRows / group, part,
+                        kv_head, &sh->queries[i]);
+          sh->query_tiles |= 1 << i;
+        }
+      const int most = shared_tokens ? max(tiles[0], tiles[1]) : items;
+      for (int i = 0; i < 2 * most; ++i) {
+        const int b = i % kBuffers;
+        if (i >= kBuffers && !wait(&sh->empty[b], (i / kBuffers - 1) & 1)) break;
+        const int box0 = box_begin + (i >> 1) * kBoxes, boxes = min(kBoxes, box_end - box0);
+        mbarrier_expect_tx(&sh->full[b], uint32_t(boxes) * 2 * kBoxBytes);
+        const CUtensorMap* map = (i & 1) ? &p.v_map : &p.k_map;
+        for (int j = 0; j < boxes; ++j)
+          for (int part = 0; part < 2; ++part)
+            tma_load_5d(ring + b * kBufferBytes + part * kHalfBytes + j * kBoxBytes, map, 0, start_of(box0 + j), part, kv_head, sequence,
+                        &sh->full[b]);
+        sh->issued = i + 1;
+      }
+    }
+  } else if (warp < 11) {
+    // ---- MMAs of one half ----
+    const int mine = warp - 9, n = tiles[mine];
+    const uint32_t leader = elect_one();
+    constexpr uint32_t kScores = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(kSpanTile >> 3) << 17) | (uint32_t(kSpanRows >> 4) << 24);
+    // The values' 128 columns are N-major: bit 16.
+    constexpr uint32_t kOutputs = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (uint32_t(kDim >> 3) << 17) | (uint32_t(kSpanRows >> 4) << 24);
+    const uint32_t query_desc = umma_desc_low(smem_address(smem) + (shared_tokens ? mine : 0) * kQueryBytes);
+    const uint32_t scores = tmem + mine * 256, outputs = scores + 128;
+    bool ok = n == 0 || __all_sync(0xffffffffu, wait(&sh->queries[shared_tokens ? mine : 0], 0));
+    // Every item is waited for in its turn, whoever's it is: a wait for a buffer's next item must not find the one before it
+    // still on its way.
+    const int all = shared_tokens ? max(tiles[0], tiles[1]) : items;
+    for (int i = 0, t = 0; i < all && ok; ++i) {
+      const int k_item = 2 * i, v_item = k_item + 1, kb = k_item % kBuffers, vb = v_item % kBuffers;
+      ok = __all_sync(0xffffffffu, wait(&sh->full[kb], (k_item / kBuffers) & 1));
+      if (!ok) break;
+      if (shared_tokens ? i >= n : (i & 1) != mine) {
+        // The other half's alone. A tile that both count is given back when it is there, not earlier, so that an arrival
+        // cannot count for the buffer's previous item.
+        ok = __all_sync(0xffffffffu, wait(&sh->full[vb], (v_item / kBuffers) & 1));
+        if (ok && shared_tokens && leader) mbarrier_arrive(&sh->empty[kb]), mbarrier_arrive(&sh->empty[vb]);
+        continue;
+      }
+      tcgen05_fence_after();
+      if (leader) {
+        const uint32_t keys = umma_desc_low(smem_address(ring) + kb * kBufferBytes);
+#pragma unroll
+        for (int k = 0; k < kDim / 16; ++k)
+          umma_bf16_ss(scores, query_desc + (k >> 2) * (kSpanRows * 128 >> 4) + (k & 3) * 2, keys + (k >> 2) * (kHalfBytes >> 4) + (k & 3) * 2,
+                       kUmmaDescHigh, kScores, k > 0 ? 1u : 0u);
+        tcgen05_commit(&sh->scores[mine]);
+        tcgen05_commit(&sh->empty[kb]);
+      }
+      ok = __all_sync(0xffffffffu, wait(&sh->full[vb], (v_item / kBuffers) & 1)) && __all_sync(0xffffffffu, wait(&sh->weights[mine], t & 1));
+      if (!ok) break;
+      tcgen05_fence_after();
+      if (leader) {
+        // 64 values of a token are a 128-byte row; the other 64 values' rows kHalfBytes on; eight tokens 1024 bytes.
+        const uint32_t values = (((smem_address(ring) + vb * kBufferBytes) & 0x3ffffu) >> 4) | (uint32_t(kHalfBytes >> 4) << 16);
+#pragma unroll
+        for (int k = 0; k < kSpanTile / 16; ++k)
+          umma_bf16_ts(outputs, scores + k * 8, values + k * (16 * 128 >> 4), kUmmaDescHigh, kOutputs, k > 0 ? 1u : uint32_t(t > 0));
+        tcgen05_commit(&sh->empty[vb]);
+        tcgen05_commit(&sh->added[mine]);
+      }
+      ++t;
+    }
+    if (leader) tcgen05_commit(&sh->done);
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  if (sh->abort) {  // no role is left to raise it: block-uniform
+    if (threadIdx.x == 0) {
+      for (uint32_t polls = 0; polls < kTmaWaitLimit && !mbarrier_try_wait(&sh->done, 0); ++polls) {
+      }
+      for (int i = 0; i < 2; ++i)
+        if (sh->query_tiles >> i & 1) mbarrier_wait(&sh->queries[i], 0);
+      for (int i = max(0, sh->issued - kBuffers); i < sh->issued; ++i) mbarrier_wait(&sh->full[i % kBuffers], (i / kBuffers) & 1);
+    }
+    __syncthreads();
+    if (live) {
+      const uint32_t nan = 0x7fffffffu;
+      for (int j = 0; j < kDim; ++j) {
+        if (p.together) partial[j] = __uint_as_float(nan);
+        else reinterpret_cast<uint16_t*>(out)[j] = 0x7fff;
+      }
+      if (p.together) *reinterpret_cast<float2*>(partial + kDim) = make_float2(0.0f, __uint_as_float(nan));
+    }
+  }
+  tcgen05_fence_after();
+  if (warp == 11) {
+    __syncwarp();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace
+
+void launch_span_attention(const SpanAttentionParams& given, cudaStream_t stream) {
+  static thread_local int configured_device = -1;
+  int device = 0;
+  EI_CUDA(cudaGetDevice(&device));
+  if (configured_device != device) {
+    EI_CUDA(cudaFuncSetAttribute(span_attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSpanSharedBytes)));
+    configured_device = device;
+  }
+  SpanAttentionParams p = given;
+  const int group = p.heads / p.kv_heads;
+  const long long all_rows = (long long)p.rows * p.sequences;
+  p.copied_queries = p.q_stride < (1ll << 31) && all_rows < (1ll << 31) &&
+                     encode_query_map(&p.q_map, p.q, int(all_rows), int(p.q_stride), group, p.kv_heads, kDim);
+  const size_t query_tiles = (size_t(p.rows) * group + kSpanRows - 1) / kSpanRows;
+  const dim3 grid(unsigned(p.kv_heads), p.together ? unsigned(p.splits.blocks()) : unsigned((query_tiles + 1) / 2), unsigned(p.sequences));
+  launch(span_attention_kernel, grid, dim3(kThreads), kSpanSharedBytes, stream, false, p);
+}
+
+}  // namespace ei

@@ -17,6 +17,7 @@
 // own. What a box brings beyond a stretch (other tokens, rows never written) is masked in the scores and cleared in V.
 #include "step_attention.cuh"
 
+#include "span_choice.hpp"
 #include "step_choice.hpp"
 
 #include <algorithm>
@@ -37,6 +38,7 @@ struct StepShared {
   float maximum[kStepRows], sum[kStepRows];
   float factor[kStepMaxSplits][kStepRows];  // weight of each block's result in the joined one
   float top[kStepRows], inverse[kStepRows];
+  float other[kSpanMostPartials][kStepRows];  // the same of what is joined
 };
 constexpr size_t step_shared(int row_tiles) {
   return size_t(kStepWarps) * kBuffers * kBuffer + (row_tiles > 1 ? size_t(kStepRows) * kDim * 2 : 0) + sizeof(StepShared) + 1024;
@@ -129,6 +131,7 @@ __global__ void __launch_bounds__(kThreads, 2) step_attention_kernel(const __gri
   // Row i of the unit: stacked row first_stacked + i = query row * group + head of the group.
   const long long row0 = (long long)sequence * p.rows;
   auto row_of = [&](int i) { return (first_stacked + i) / group; };
+  auto joined_of = [&](int i) { return p.joined_counts[row0 * group + first_stacked + i < p.joined_border ? 0 : 1]; };
   auto query_at = [&](int i) {
     const int r = row_of(i), h = first_stacked + i - r * group;
     return p.q + (row0 + r) * p.q_stride + size_t(kv_head * group + h) * kDim;
@@ -394,16 +397,19 @@ __global__ void __launch_bounds__(kThreads, 2) step_attention_kernel(const __gri
       const int r = row_of(i);
       slot = size_t(row0 + r) * p.heads + kv_head * group + (first_stacked + i - r * group);
     }
-    for (int j = 0; j < p.joined_count && real; ++j) top = fmaxf(top, p.joined[(j * slots + slot) * kStepPartial + 128]);
+    const int others = real && p.joined ? joined_of(i) : 0;
+    for (int j = 0; j < others; ++j) top = fmaxf(top, p.joined[(j * slots + slot) * kStepPartial + 128]);
     for (uint32_t r = 0; r < splits; ++r) {
       const float part = remote_float(&sh->sum[i], r);
       const float factor = part == 0.0f ? 0.0f : power_of_two(remote_float(&sh->maximum[i], r) - top);
       sh->factor[r][i] = factor;
       if (part != 0.0f) sum += part * factor;
     }
-    for (int j = 0; j < p.joined_count && real; ++j) {
+    for (int j = 0; j < others; ++j) {
       const float* from = p.joined + (j * slots + slot) * kStepPartial;
-      if (from[129] != 0.0f) sum += from[129] * power_of_two(from[128] - top);
+      const float part = from[129], factor = part == 0.0f ? 0.0f : power_of_two(from[128] - top);
+      sh->other[j][i] = factor;
+      if (part != 0.0f) sum += part * factor;
     }
     sh->top[i] = top;
     sh->inverse[i] = !real || sum == 0.0f ? 0.0f : p.partial ? sum : 1.0f / sum;
@@ -426,11 +432,11 @@ __global__ void __launch_bounds__(kThreads, 2) step_attention_kernel(const __gri
       }
       const int r = row_of(i), h = kv_head * group + first_stacked + i - r * group;
       const size_t slot = size_t(row0 + r) * p.heads + h;
-      for (int j = 0; j < p.joined_count; ++j) {
-        const float* other = p.joined + (j * slots + slot) * kStepPartial;
-        if (other[129] == 0.0f) continue;
-        const float factor = power_of_two(other[128] - sh->top[i]);
-        const float4 v = *reinterpret_cast<const float4*>(other + quad * 4);
+      const int others = p.joined && (p.together || base + r >= 0) ? joined_of(i) : 0;
+#pragma unroll 4
+      for (int j = 0; j < others; ++j) {
+        const float factor = sh->other[j][i];
+        const float4 v = *reinterpret_cast<const float4*>(p.joined + (j * slots + slot) * kStepPartial + quad * 4);
         total.x = fmaf(v.x, factor, total.x), total.y = fmaf(v.y, factor, total.y);
         total.z = fmaf(v.z, factor, total.z), total.w = fmaf(v.w, factor, total.w);
       }
@@ -486,12 +492,13 @@ void configure_step_kernels() {
 
 }  // namespace
 
-void encode_cache_map(CUtensorMap* map, const CacheStrides& cache, size_t capacity, size_t kv_heads, size_t sequences, int box_tokens) {
+void encode_cache_map(CUtensorMap* map, const CacheStrides& cache, size_t capacity, size_t kv_heads, size_t sequences, int box_tokens,
+                      int box_halves) {
   const cuuint64_t dims[5] = {64, cuuint64_t(capacity), 2, cuuint64_t(kv_heads), cuuint64_t(sequences)};
   // An axis of extent 1 is not stepped along; its stride only has to be one that the encoder takes.
   const cuuint64_t strides[4] = {cuuint64_t(capacity > 1 ? cache.token : kDim) * 2, 128, cuuint64_t(kv_heads > 1 ? cache.head : kDim) * 2,
                                  cuuint64_t(sequences > 1 ? cache.sequence : kDim) * 2};
-  const cuuint32_t box[5] = {64, cuuint32_t(box_tokens), 2, 1, 1};
+  const cuuint32_t box[5] = {64, cuuint32_t(box_tokens), cuuint32_t(box_halves), 1, 1};
   encode_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, cache.data, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, "K / V cache");
 }
 

@@ -12,9 +12,10 @@ struct CacheStrides {
   const bf16* data;
   size_t token, head, sequence;
 };
-// Map of a cache for boxes of `box` tokens of one head: (64 values, token, half of the head, KV head, sequence), so that a
-// box lands as [half][token][128 B] with the 128-byte swizzle. Tokens from `capacity` on read as zero.
-void encode_cache_map(CUtensorMap* map, const CacheStrides& cache, size_t capacity, size_t kv_heads, size_t sequences, int box);
+// Map of a cache for boxes of one head's tokens: (64 values, token, half of the head, KV head, sequence), so that a box lands as
+// [half][token][128 B] with the 128-byte swizzle. Tokens from `capacity` on read as zero.
+void encode_cache_map(CUtensorMap* map, const CacheStrides& cache, size_t capacity, size_t kv_heads, size_t sequences, int box_tokens,
+                      int box_halves);
 
 struct StepAttentionParams {
   CUtensorMap k_map, v_map;   // boxes of kStepTile tokens
@@ -29,9 +30,10 @@ struct StepAttentionParams {
   int window, sinks;          // a row at position p sees t <= p with t > p - window or t < sinks
   bool together;              // every row stands at the last token (a prefix that all rows see)
   int first_group, groups;    // groups of kStepRows stacked rows that this launch takes
-  // Results of other stretches of tokens to be joined: [joined][sequences * rows][heads][kStepPartial].
+  // Results of other stretches of tokens to be joined: [joined][sequences * rows][heads][kStepPartial]. Of all sequences' stacked
+  // rows of a KV head (all_row * group + head of the group) those below joined_border have joined_counts[0], the others [1].
   const float* joined;
-  int joined_count;
+  int joined_border, joined_counts[2];
   float* partial;             // leave (sums, maximum, sum) here in that layout instead of normalised rows in `out`
   // Weights: scores_out[s][j][t] = scores[s][j][t] + the weights of token t, summed over this launch's rows and the group's
   // heads; every token of the sequence is written. raw: [sequences][kv_heads][raw_rows][raw_stride] FP32.

@@ -129,19 +129,20 @@ def attention_verify(ctx, q, k_capacity, v_capacity, output, device_offset, scra
 ROPE_SCALINGS = {"plain": 0, "linear": 1, "yarn": 2, "bands": 3}
 
 
-def _expect(ctx, dtype: str, **tensors) -> None:
-    """Device, type and rank of what a C call only sees as pointers; `name=(tensor, rank)`."""
-    for name, (t, rank) in tensors.items():
-        if t.device.type != "cuda" or t.device.index != ctx.device:
-            raise ValueError(f"{name} is on {t.device}, the execution context on cuda:{ctx.device}")
+def _expect(ctx, dtype: str, rank: int, *tensors) -> None:
+    """Device, type and rank of what a C call only sees as pointers."""
+    device = ctx.device
+    for t in tensors:
+        if t.get_device() != device:
+            raise ValueError(f"a tensor is on {t.device}, the execution context on cuda:{device}")
         if str(t.dtype) != dtype or t.dim() != rank:
-            raise ValueError(f"{name} must be a {dtype} tensor with {rank} axes, not {t.dtype} with {t.dim()}")
+            raise ValueError(f"expected a {dtype} tensor with {rank} axes, not {t.dtype} with {t.dim()}")
 
 
 def _lengths(ctx, lengths, sequences: int):
     if lengths is None:
         return None
-    _expect(ctx, "torch.int32", lengths=(lengths, 1))
+    _expect(ctx, "torch.int32", 1, lengths)
     if lengths.shape[0] != sequences or not lengths.is_contiguous():
         raise ValueError("lengths must hold one packed value per sequence")
     return lengths.data_ptr()
@@ -164,13 +165,13 @@ def qk_norm_rope(ctx, q, k, table, q_out, k_out, *, positions=None, offset: int 
                  epsilon: float = 1e-6, interleaved: bool = False) -> None:
     """Norm of every query and key head (where a weight is given) and rotation of its first table.shape[1] values, in one
     pass with one rounding. positions: int32 [rows] on the device, else offset + row. Outputs may be the inputs."""
-    _expect(ctx, "torch.bfloat16", q=(q, 3), k=(k, 3), q_out=(q_out, 3), k_out=(k_out, 3))
-    _expect(ctx, "torch.float32", table=(table, 2))
+    _expect(ctx, "torch.bfloat16", 3, q, k, q_out, k_out)
+    _expect(ctx, "torch.float32", 2, table)
     for weight in (q_weight, k_weight):
         if weight is not None:
-            _expect(ctx, "torch.bfloat16", weight=(weight, 1))
+            _expect(ctx, "torch.bfloat16", 1, weight)
     if positions is not None:
-        _expect(ctx, "torch.int32", positions=(positions, 1))
+        _expect(ctx, "torch.int32", 1, positions)
         if positions.shape[0] != q.shape[0] or not positions.is_contiguous():
             raise ValueError("positions must hold one packed value per row")
     abi.check(_lib().ei_qk_norm_rope_bf16(
@@ -182,7 +183,8 @@ def attention_window(ctx, q, k, v, output, window: int, sinks: int = 0, *, lengt
     """Causal attention of [sequences * rows, heads, 128] queries over caches [sequences, capacity, kv_heads, 128]: a row at
     position p sees the tokens t <= p with t > p - window or t < sinks. lengths: int32 [sequences] on the device, the rows'
     own tokens included, else `length` for all."""
-    _expect(ctx, "torch.bfloat16", q=(q, 3), k=(k, 4), v=(v, 4), output=(output, 3))
+    _expect(ctx, "torch.bfloat16", 3, q, output)
+    _expect(ctx, "torch.bfloat16", 4, k, v)
     abi.check(_lib().ei_attention_window_bf16(C.byref(ctx), abi.view3(q), abi.view4(k), abi.view4(v), abi.view3(output),
                                               _lengths(ctx, lengths, k.shape[0]), length, window, sinks))
 
@@ -194,9 +196,10 @@ def attention_shared_prefix_scratch_bytes(q_rows: int, query_heads: int, kv_head
 def attention_shared_prefix(ctx, q, prefix_k, prefix_v, k, v, output, scratch, *, lengths=None, length: int = 0) -> None:
     """Causal attention of sequences that share their first tokens, prefix_k / prefix_v [prefix, kv_heads, 128], read once for
     all of them; lengths and positions count each sequence's own tokens in k / v."""
-    _expect(ctx, "torch.bfloat16", q=(q, 3), prefix_k=(prefix_k, 3), prefix_v=(prefix_v, 3), k=(k, 4), v=(v, 4), output=(output, 3))
+    _expect(ctx, "torch.bfloat16", 3, q, prefix_k, prefix_v, output)
+    _expect(ctx, "torch.bfloat16", 4, k, v)
     if scratch is not None:
-        _expect(ctx, str(scratch.dtype), scratch=(scratch, scratch.dim()))
+        _expect(ctx, str(scratch.dtype), scratch.dim(), scratch)
     ptr, size = _scratch(scratch)
     abi.check(_lib().ei_attention_shared_prefix_bf16(
         C.byref(ctx), abi.view3(q), abi.view3(prefix_k), abi.view3(prefix_v), abi.view4(k), abi.view4(v), abi.view3(output),
@@ -210,12 +213,13 @@ def attention_accumulate_scratch_bytes(sequences: int, rows: int, query_heads: i
 def attention_accumulate(ctx, q, k, v, output, scores, scores_out, scratch, *, lengths=None, length: int = 0) -> None:
     """Causal attention that also adds every token's softmax weights, over rows and a KV head's query heads, to scores
     (FP32 [sequences, kv_heads, capacity]; None counts as zeros) and leaves them in scores_out (which may be scores)."""
-    _expect(ctx, "torch.bfloat16", q=(q, 3), k=(k, 4), v=(v, 4), output=(output, 3))
-    _expect(ctx, "torch.float32", scores_out=(scores_out, 3))
+    _expect(ctx, "torch.bfloat16", 3, q, output)
+    _expect(ctx, "torch.bfloat16", 4, k, v)
+    _expect(ctx, "torch.float32", 3, scores_out)
     if scores is not None:
-        _expect(ctx, "torch.float32", scores=(scores, 3))
+        _expect(ctx, "torch.float32", 3, scores)
     if scratch is not None:
-        _expect(ctx, str(scratch.dtype), scratch=(scratch, scratch.dim()))
+        _expect(ctx, str(scratch.dtype), scratch.dim(), scratch)
     ptr, size = _scratch(scratch)
     abi.check(_lib().ei_attention_accumulate_bf16(
         C.byref(ctx), abi.view3(q), abi.view4(k), abi.view4(v), abi.view3(output), _lengths(ctx, lengths, k.shape[0]), length,
@@ -226,9 +230,9 @@ def evict_kv(ctx, k, v, scores, k_out, v_out, scores_out, kept, lengths_out, sin
              length: int = 0) -> None:
     """Cuts caches to the k_out.shape[1] tokens that are first, latest or heaviest, each KV head its own, in order of
     position; kept (int32) receives their positions, -1 behind them, lengths_out (int32) the new lengths."""
-    _expect(ctx, "torch.bfloat16", k=(k, 4), v=(v, 4), k_out=(k_out, 4), v_out=(v_out, 4))
-    _expect(ctx, "torch.float32", scores=(scores, 3), scores_out=(scores_out, 3))
-    _expect(ctx, "torch.int32", kept=(kept, 3))
+    _expect(ctx, "torch.bfloat16", 4, k, v, k_out, v_out)
+    _expect(ctx, "torch.float32", 3, scores, scores_out)
+    _expect(ctx, "torch.int32", 3, kept)
     abi.check(_lib().ei_evict_kv_bf16(
         C.byref(ctx), abi.view4(k), abi.view4(v), abi.view3(scores), _lengths(ctx, lengths, k.shape[0]), length, sinks, recent,
         abi.view4(k_out), abi.view4(v_out), abi.view3(scores_out), abi.view3(kept), _lengths(ctx, lengths_out, k.shape[0])))
