@@ -18,7 +18,7 @@
 // blocks, which then take every other tile of tokens.
 //
 // Roles of the twelve warps: 0-3 and 4-7 the weights of one half each, 8 the copies, 9 and 10 the MMAs of one half each, 11 the
-// tensor memory. K and V tiles of 32 KB go through a ring of five buffers. Every wait is bounded: a role whose wait runs out
+// tensor memory. K and V tiles of 16 KB go through a ring of eight buffers. Every wait is bounded: a role whose wait runs out
 // raises `abort`, which every other wait polls; when all roles have left, the copies and MMAs in flight are waited for
 // (bounded), the block's rows come out as NaN and the tensor memory is freed.
 #include "span_attention.cuh"
@@ -36,7 +36,7 @@ constexpr int kHalfBytes = kSpanTile * 128;  // 64 values of a tile's tokens
 constexpr int kBufferBytes = 2 * kHalfBytes;
 constexpr int kBoxBytes = kSpanBox * 128;
 constexpr int kBoxes = kSpanTile / kSpanBox;
-constexpr int kBuffers = 5;
+constexpr int kBuffers = 8;
 constexpr int kQueryBytes = 2 * kSpanRows * 128;
 constexpr float kSlack = 8.0f;  // powers of two
 constexpr size_t kSpanSharedBytes = size_t(2) * kQueryBytes + size_t(kBuffers) * kBufferBytes + 1024 + 512;
@@ -45,7 +45,7 @@ static_assert(kSpanSharedBytes <= 227 * 1024, "a block's buffers fit an SM");
 struct SpanShared {
   uint64_t full[kBuffers], empty[kBuffers];  // K and V tiles in turn
   uint64_t queries[2];                       // a query tile is in shared memory
-  uint64_t scores[2], weights[2];            // of a half: S computed, P written
+  uint64_t scores[2][2], weights[2][2];      // [half][place]: S computed, P written
   uint64_t added[2];                         // O holds the tile's product
   uint64_t done;                             // every MMA issued has completed
   uint32_t tmem_base;
@@ -66,6 +66,8 @@ __device__ __forceinline__ void tmem_request32(uint32_t address, uint32_t* r) {
       : "r"(address)
       : "memory");
 }
+// The lowest `count` bits, of any sign and size.
+__device__ __forceinline__ uint32_t below(int count) { return count >= 32 ? 0xffffffffu : count <= 0 ? 0u : (1u << count) - 1; }
 // Waits for the loads requested; the registers pass through so that nothing reads them earlier.
 __device__ __forceinline__ void tmem_loaded32(uint32_t* r) {
   __syncwarp();
@@ -90,9 +92,9 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
   if (length < 0 || length > p.capacity) length = 0;
   int first_tile;             // query tile of half 0
   bool shared_tokens = true;  // both halves read every tile of tokens (of two query tiles); else every other (of one)
-  int partial_index[2] = {0, 0};
+  int partial_first = 0;      // of half 0's result among the prefix's
   int box_begin = 0, low = 0, sink_end = 0, sink_boxes = 0, box_end, end;
-  int first_position[2], last_position[2];  // of a half's rows
+  int first_position0, last_position0, first_position1, last_position1;  // of the halves' rows
   const int base = length - p.rows;
   if (p.together) {
     const int y = blockIdx.y;
@@ -101,28 +103,27 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
       first_tile = y / p.splits.pair_splits * 2;
       splits = p.splits.pair_splits;
       split = y - first_tile / 2 * splits;
-      partial_index[0] = partial_index[1] = split;
+      partial_first = split;
     } else {
       first_tile = p.splits.pairs * 2;
       shared_tokens = false;
       splits = p.splits.single_splits;
       split = y - p.splits.pairs * p.splits.pair_splits;
-      partial_index[0] = 2 * split, partial_index[1] = 2 * split + 1;
+      partial_first = 2 * split;
     }
     const int tiles = (length + kSpanTile - 1) / kSpanTile;
     box_begin = int((long long)tiles * split / splits) * kBoxes;
     end = length;
     box_end = min(int((long long)tiles * (split + 1) / splits) * kBoxes, (end + kSpanBox - 1) / kSpanBox);
-    first_position[0] = first_position[1] = last_position[0] = last_position[1] = length - 1;
+    first_position0 = first_position1 = last_position0 = last_position1 = length - 1;
   } else {
     first_tile = (int(gridDim.y) - 1 - int(blockIdx.y)) * 2;  // the longest histories first
-    for (int half = 0; half < 2; ++half) {
-      const int from = (first_tile + half) * kSpanRows;
-      first_position[half] = base + min(from, stacked - 1) / group;
-      last_position[half] = base + min(from + kSpanRows - 1, stacked - 1) / group;
-    }
-    end = max(0, last_position[1] + 1);
-    low = max(0, min(first_position[0] - p.window + 1, end));
+    auto position_of = [&](int i) { return base + min(i, stacked - 1) / group; };
+    const int from = first_tile * kSpanRows;
+    first_position0 = position_of(from), last_position0 = position_of(from + kSpanRows - 1);
+    first_position1 = position_of(from + kSpanRows), last_position1 = position_of(from + 2 * kSpanRows - 1);
+    end = max(0, last_position1 + 1);
+    low = max(0, min(first_position0 - p.window + 1, end));
     sink_end = min(p.sinks, low);
     sink_boxes = (sink_end + kSpanBox - 1) / kSpanBox;
     box_end = sink_boxes + (end - low + kSpanBox - 1) / kSpanBox;
@@ -135,12 +136,12 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
     if (!shared_tokens) return (items + 1 - half) / 2;
     if ((first_tile + half) * kSpanRows >= stacked) return 0;
     if (p.together) return items;
-    const int position = last_position[half];
+    const int position = half ? last_position1 : last_position0;
     if (position < 0) return 0;
     const int boxes = position < low ? (min(sink_end, position + 1) + kSpanBox - 1) / kSpanBox : sink_boxes + (position - low) / kSpanBox + 1;
     return min(items, (boxes + kBoxes - 1) / kBoxes);
   };
-  const int tiles[2] = {tiles_of(0), tiles_of(1)};
+  const int tiles0 = tiles_of(0), tiles1 = tiles_of(1);
   auto item_of = [&](int half, int t) { return shared_tokens ? t : 2 * t + half; };
 
   if (threadIdx.x == 0) {
@@ -150,8 +151,10 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
     }
     for (int i = 0; i < 2; ++i) {
       mbarrier_init(&sh->queries[i], p.copied_queries ? 1 : 4);
-      mbarrier_init(&sh->scores[i], 1);
-      mbarrier_init(&sh->weights[i], 4);
+      for (int place = 0; place < 2; ++place) {
+        mbarrier_init(&sh->scores[i][place], 1);
+        mbarrier_init(&sh->weights[i][place], 4);
+      }
       mbarrier_init(&sh->added[i], 1);
     }
     mbarrier_init(&sh->done, 2);
@@ -183,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
   const bool live = warp < 8 && index < stacked;
   const int row = live ? index / group : 0, head = kv_head * group + (live ? index - row * group : 0);
   float* const partial =
-      p.partial + ((size_t(partial_index[half]) * p.sequences * p.rows + row0 + row) * p.heads + head) * kStepPartial;
+      p.partial + ((size_t(partial_first + (shared_tokens ? 0 : half)) * p.sequences * p.rows + row0 + row) * p.heads + head) * kStepPartial;
   bf16* const out = p.out + (row0 + row) * p.out_stride + size_t(head) * kDim;
 
   if (warp < 8) {
@@ -204,97 +207,69 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
       if (lane == 0) mbarrier_arrive(&sh->queries[half]);
     }
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-    const uint32_t at = tmem + lanes + half * 256, outputs = at + 128;
+    const uint32_t places = tmem + lanes + half * 256, outputs = places + 128;
     const int last = p.together ? length - 1 : base + row;
     const bool some_live = __any_sync(0xffffffffu, live);
     const float exponent_scale = rsqrtf(float(kDim)) * kLog2e;
     float maximum = -INFINITY, sum = 0.0f;
+    const float2 scales = make_float2(exponent_scale, exponent_scale);
+    const int tiles = half ? tiles1 : tiles0;
+    // Boxes that every row of the half sees whole.
+    const int clean_begin = sink_boxes + (max(0, (half ? last_position1 : last_position0) - p.window + 1 - low) + kSpanBox - 1) / kSpanBox;
+    const int clean_end = sink_boxes + max(0, min(end, (half ? first_position1 : first_position0) + 1) - low) / kSpanBox;
     bool ok = true;
-    for (int t = 0; t < tiles[half]; ++t) {
+    for (int t = 0; t < tiles; ++t) {
       const int item = item_of(half, t), box0 = box_begin + item * kBoxes;
-      ok = __all_sync(0xffffffffu, wait(&sh->scores[half], t & 1));
+      const bool clean = box0 >= clean_begin && box0 + kBoxes <= clean_end;
+      const uint32_t at = places + (t & 1) * 64;
+      ok = __all_sync(0xffffffffu, wait(&sh->scores[half][t & 1], (t >> 1) & 1));
       if (!ok) break;
       tcgen05_fence_after();
-      // Whether the tile holds anything that some row of the half does not see, or that is no token of the list.
-      bool masked = false, partial_tile = false;
-#pragma unroll
-      for (int b = 0; b < kBoxes; ++b) {
-        const int start = start_of(box0 + b), stop = stop_of(box0 + b);
-        partial_tile |= start + kSpanBox > stop;
-        masked |= start + kSpanBox > min(stop, first_position[half] + 1) ||
-                  (start <= last_position[half] - p.window && start + kSpanBox > p.sinks);
-      }
+      uint32_t s[2][32];
+      float2 shifts = make_float2(0.0f, 0.0f);
+      float rescale = 1.0f;
+      bool moved_some = false;
       if (some_live) {
-        uint32_t s[4][32];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_request32(at + i * 32, s[i]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_loaded32(s[i]);
-        if (masked) {
-#pragma unroll
-          for (int b = 0; b < kBoxes; ++b) {
-            const int start = start_of(box0 + b);
-            const int visible = min(stop_of(box0 + b), last + 1) - start;                // places below it
-            const int hidden = p.sinks - start, shown = last - p.window - start;         // but not hidden .. shown
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j >= visible || (j >= hidden && j <= shown)) s[b][j] = 0xff800000u;
-          }
-        }
+        tmem_request32(at, s[0]);
+        tmem_request32(at + 32, s[1]);
+        tmem_loaded32(s[0]);
+        tmem_loaded32(s[1]);
         float tops[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          tops[i] = __uint_as_float(s[i][0]);
+        for (int i = 0; i < 2; ++i) {
+          if (!clean) {
+            const int start = start_of(box0 + i);
+            const uint32_t seen = below(min(stop_of(box0 + i), last + 1) - start) &
+                                  (below(p.sinks - start) | ~below(last - p.window + 1 - start));
 #pragma unroll
-          for (int j = 1; j < 32; ++j) tops[i] = fmaxf(tops[i], __uint_as_float(s[i][j]));
+            for (int j = 0; j < 32; ++j) s[i][j] = seen >> j & 1 ? s[i][j] : 0xff800000u;
+          }
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            float& most = tops[2 * i + part];
+            most = __uint_as_float(s[i][16 * part]);
+#pragma unroll
+            for (int j = 1; j < 16; ++j) most = fmaxf(most, __uint_as_float(s[i][16 * part + j]));
+          }
         }
         const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         const bool moved = maximum == -INFINITY ? top != -INFINITY : (top - maximum) * exponent_scale > kSlack;
         const float previous = maximum;
         if (moved) maximum = top;
         // A row with nothing visible yet keeps -inf; 0 as the exponent's base then makes every weight 0.
-        const float reference = maximum == -INFINITY ? 0.0f : maximum, shift = -reference * exponent_scale;
-        const float rescale = moved ? power_of_two((previous - reference) * exponent_scale) : 1.0f;
-        const float2 scales = make_float2(exponent_scale, exponent_scale), shifts = make_float2(shift, shift);
-        float2 parts[2] = {};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t packed[16];
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const float2 x = fma_pair(make_float2(__uint_as_float(s[i][j]), __uint_as_float(s[i][j + 1])), scales, shifts);
-            const uint32_t both = pack_bf16(power_of_two(x.x), power_of_two(x.y));
-            packed[j / 2] = both;
-            parts[j / 2 & 1] = add_pair(parts[j / 2 & 1], make_float2(bf16_lo(both), bf16_hi(both)));
-          }
-          tmem_store16(at + i * 16, packed);
-        }
-        const float2 total = add_pair(parts[0], parts[1]);
-        sum = sum * rescale + (total.x + total.y);
-        if (t > 0 && __any_sync(0xffffffffu, moved)) {
-          ok = __all_sync(0xffffffffu, wait(&sh->added[half], (t - 1) & 1));
-          if (!ok) break;
-          tcgen05_fence_after();
-#pragma unroll 1
-          for (int i = 0; i < 4; ++i) {
-            uint32_t a[32];
-            tmem_request32(outputs + i * 32, a);
-            tmem_loaded32(a);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) a[j] = __float_as_uint(__uint_as_float(a[j]) * rescale);
-            tmem_store16(outputs + i * 32, *reinterpret_cast<uint32_t(*)[16]>(a));
-            tmem_store16(outputs + i * 32 + 16, *reinterpret_cast<uint32_t(*)[16]>(a + 16));
-          }
-        }
+        const float reference = maximum == -INFINITY ? 0.0f : maximum;
+        shifts.x = shifts.y = -reference * exponent_scale;
+        if (moved) rescale = power_of_two((previous - reference) * exponent_scale);
+        moved_some = __any_sync(0xffffffffu, moved);
       }
-      if (partial_tile) {
+      if (!clean) {
         // V's rows that are no token of the list are cleared: nothing there may pass through a zero weight. (Both halves'
         // warps do it before they hand over their weights, with the same zeros.)
         const int v_item = 2 * item + 1;
         ok = __all_sync(0xffffffffu, wait(&sh->full[v_item % kBuffers], (v_item / kBuffers) & 1));
         if (!ok) break;
         unsigned char* values = ring + (v_item % kBuffers) * kBufferBytes;
-#pragma unroll
+#pragma unroll 1
         for (int b = 0; b < kBoxes; ++b) {
           const int have = min(kSpanBox, max(0, stop_of(box0 + b) - start_of(box0 + b)));
           for (int i = row_of_tile; i < (kSpanBox - have) * 16; i += kSpanRows)
@@ -303,13 +278,67 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
+      if (some_live) {
+        // In groups of 16, a group's exponentials ahead of the conversions of the one before it: taken pair by pair, each
+        // conversion waited for its own two exponentials, 20 cycles a value instead of 8.
+        float2 parts[2] = {};
+        uint32_t packed[2][16];
+        auto exponentials = [&](int group) {
+          uint32_t* const v = &s[group >> 1][(group & 1) * 16];
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) {
+            const float2 x = fma_pair(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), scales, shifts);
+            v[j] = __float_as_uint(x.x), v[j + 1] = __float_as_uint(x.y);
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+r"(v[j]));
+        };
+        auto convert = [&](int group) {
+          const uint32_t* const v = &s[group >> 1][(group & 1) * 16];
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) {
+            uint32_t both;
+            asm volatile("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(both) : "f"(__uint_as_float(v[j + 1])), "f"(__uint_as_float(v[j])));
+            packed[group >> 1][(group & 1) * 8 + j / 2] = both;
+            parts[j / 2 & 1] = add_pair(parts[j / 2 & 1], make_float2(bf16_lo(both), bf16_hi(both)));
+          }
+        };
+        exponentials(0);
+        exponentials(1);
+        convert(0);
+        exponentials(2);
+        convert(1);
+        tmem_store16(at, packed[0]);
+        exponentials(3);
+        convert(2);
+        convert(3);
+        tmem_store16(at + 16, packed[1]);
+        const float2 total = add_pair(parts[0], parts[1]);
+        sum = sum * rescale + (total.x + total.y);
+      }
+      if (t > 0) {
+        ok = __all_sync(0xffffffffu, wait(&sh->added[half], (t - 1) & 1));  // each in its turn: phases are told apart by parity
+        if (!ok) break;
+        if (moved_some) {
+          tcgen05_fence_after();
+#pragma unroll 1
+          for (int i = 0; i < 8; ++i) {
+            uint32_t a[16];
+            tmem_request16(outputs + i * 16, a);
+            tmem_loaded(a);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) a[j] = __float_as_uint(__uint_as_float(a[j]) * rescale);
+            tmem_store16(outputs + i * 16, a);
+          }
+        }
+      }
       tmem_stored();
       tcgen05_fence_before();
       __syncwarp();
-      if (lane == 0) mbarrier_arrive(&sh->weights[half]);
+      if (lane == 0) mbarrier_arrive(&sh->weights[half][t & 1]);
     }
-    const bool any = tiles[half] > 0;
-    if (any) ok = ok && __all_sync(0xffffffffu, wait(&sh->added[half], (tiles[half] - 1) & 1));
+    const bool any = tiles > 0;
+    if (any) ok = ok && __all_sync(0xffffffffu, wait(&sh->added[half], (tiles - 1) & 1));
     if (ok) {
       tcgen05_fence_after();
       const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -347,14 +376,14 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
     if (lane == 0) {
       if (p.copied_queries)
         for (int i = 0; i < (shared_tokens ? 2 : 1); ++i) {
-          if (tiles[i] == 0) continue;
+          if ((i ? tiles1 : tiles0) == 0) continue;
           mbarrier_expect_tx(&sh->queries[i], uint32_t(kQueryBytes));
           for (int part = 0; part < 2; ++part)
             tma_load_5d(smem + i * kQueryBytes + part * kSpanRows * 128, &p.q_map, 0, 0, int(row0) + query_tile_of(i) * kSpanRows / group, part,
                         kv_head, &sh->queries[i]);
           sh->query_tiles |= 1 << i;
         }
-      const int most = shared_tokens ? max(tiles[0], tiles[1]) : items;
+      const int most = shared_tokens ? max(tiles0, tiles1) : items;
       for (int i = 0; i < 2 * most; ++i) {
         const int b = i % kBuffers;
         if (i >= kBuffers && !wait(&sh->empty[b], (i / kBuffers - 1) & 1)) break;
@@ -368,53 +397,70 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
         sh->issued = i + 1;
       }
     }
-  } else if (warp < 11) {
+  } else if (warp == 9 || warp == 10) {
     // ---- MMAs of one half ----
-    const int mine = warp - 9, n = tiles[mine];
+    const int mine = warp - 9, n = mine ? tiles1 : tiles0;
     const uint32_t leader = elect_one();
     constexpr uint32_t kScores = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(kSpanTile >> 3) << 17) | (uint32_t(kSpanRows >> 4) << 24);
     // The values' 128 columns are N-major: bit 16.
     constexpr uint32_t kOutputs = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (uint32_t(kDim >> 3) << 17) | (uint32_t(kSpanRows >> 4) << 24);
     const uint32_t query_desc = umma_desc_low(smem_address(smem) + (shared_tokens ? mine : 0) * kQueryBytes);
-    const uint32_t scores = tmem + mine * 256, outputs = scores + 128;
-    bool ok = n == 0 || __all_sync(0xffffffffu, wait(&sh->queries[shared_tokens ? mine : 0], 0));
+    const uint32_t outputs = tmem + mine * 256 + 128;
     // Every item is waited for in its turn, whoever's it is: a wait for a buffer's next item must not find the one before it
     // still on its way.
-    const int all = shared_tokens ? max(tiles[0], tiles[1]) : items;
-    for (int i = 0, t = 0; i < all && ok; ++i) {
-      const int k_item = 2 * i, v_item = k_item + 1, kb = k_item % kBuffers, vb = v_item % kBuffers;
-      ok = __all_sync(0xffffffffu, wait(&sh->full[kb], (k_item / kBuffers) & 1));
-      if (!ok) break;
-      if (shared_tokens ? i >= n : (i & 1) != mine) {
-        // The other half's alone. A tile that both count is given back when it is there, not earlier, so that an arrival
-        // cannot count for the buffer's previous item.
-        ok = __all_sync(0xffffffffu, wait(&sh->full[vb], (v_item / kBuffers) & 1));
-        if (ok && shared_tokens && leader) mbarrier_arrive(&sh->empty[kb]), mbarrier_arrive(&sh->empty[vb]);
-        continue;
-      }
+    const int all = shared_tokens ? max(tiles0, tiles1) : items;
+    bool ok = n == 0 || __all_sync(0xffffffffu, wait(&sh->queries[shared_tokens ? mine : 0], 0));
+    auto is_own = [&](int i) { return shared_tokens ? i < n : (i & 1) == mine; };
+    auto own_index = [&](int i) { return shared_tokens ? i : i >> 1; };
+    auto await = [&](int item) { return __all_sync(0xffffffffu, wait(&sh->full[item % kBuffers], (item / kBuffers) & 1)); };
+    auto score = [&](int i) {
+      if (!await(2 * i)) return false;
+      if (!is_own(i)) return true;
       tcgen05_fence_after();
       if (leader) {
-        const uint32_t keys = umma_desc_low(smem_address(ring) + kb * kBufferBytes);
+        const int b = 2 * i % kBuffers, place = own_index(i) & 1;
+        const uint32_t keys = umma_desc_low(smem_address(ring) + b * kBufferBytes);
 #pragma unroll
         for (int k = 0; k < kDim / 16; ++k)
-          umma_bf16_ss(scores, query_desc + (k >> 2) * (kSpanRows * 128 >> 4) + (k & 3) * 2, keys + (k >> 2) * (kHalfBytes >> 4) + (k & 3) * 2,
-                       kUmmaDescHigh, kScores, k > 0 ? 1u : 0u);
-        tcgen05_commit(&sh->scores[mine]);
-        tcgen05_commit(&sh->empty[kb]);
+          umma_bf16_ss(tmem + mine * 256 + place * 64, query_desc + (k >> 2) * (kSpanRows * 128 >> 4) + (k & 3) * 2,
+                       keys + (k >> 2) * (kHalfBytes >> 4) + (k & 3) * 2, kUmmaDescHigh, kScores, k > 0 ? 1u : 0u);
+        tcgen05_commit(&sh->scores[mine][place]);
+        tcgen05_commit(&sh->empty[b]);
       }
-      ok = __all_sync(0xffffffffu, wait(&sh->full[vb], (v_item / kBuffers) & 1)) && __all_sync(0xffffffffu, wait(&sh->weights[mine], t & 1));
+      return true;
+    };
+    int ahead = 0;  // items whose scores have been asked for
+    for (int i = 0; i < all && ok; ++i) {
+      // The scores of the half's next tile, ahead of this one's product: they have a place of their own.
+      const int next = min(all, i + (shared_tokens ? 2 : is_own(i) ? 3 : 1));
+      for (; ahead < next && ok; ++ahead) {
+        // Items in order: K of an item comes before its V, and V of the ones between has been waited for by then.
+        ok = score(ahead);
+      }
+      ok = ok && await(2 * i + 1);
       if (!ok) break;
-      tcgen05_fence_after();
-      if (leader) {
-        // 64 values of a token are a 128-byte row; the other 64 values' rows kHalfBytes on; eight tokens 1024 bytes.
-        const uint32_t values = (((smem_address(ring) + vb * kBufferBytes) & 0x3ffffu) >> 4) | (uint32_t(kHalfBytes >> 4) << 16);
+      const int b = (2 * i + 1) % kBuffers;
+      if (is_own(i)) {
+        const int t = own_index(i);
+        ok = __all_sync(0xffffffffu, wait(&sh->weights[mine][t & 1], (t >> 1) & 1));
+        if (!ok) break;
+        tcgen05_fence_after();
+        if (leader) {
+          // 64 values of a token are a 128-byte row; the other 64 values' rows kHalfBytes on; eight tokens 1024 bytes.
+          const uint32_t values = (((smem_address(ring) + b * kBufferBytes) & 0x3ffffu) >> 4) | (uint32_t(kHalfBytes >> 4) << 16);
 #pragma unroll
-        for (int k = 0; k < kSpanTile / 16; ++k)
-          umma_bf16_ts(outputs, scores + k * 8, values + k * (16 * 128 >> 4), kUmmaDescHigh, kOutputs, k > 0 ? 1u : uint32_t(t > 0));
-        tcgen05_commit(&sh->empty[vb]);
-        tcgen05_commit(&sh->added[mine]);
+          for (int k = 0; k < kSpanTile / 16; ++k)
+            umma_bf16_ts(outputs, tmem + mine * 256 + (t & 1) * 64 + k * 8, values + k * (16 * 128 >> 4), kUmmaDescHigh, kOutputs,
+                         k > 0 ? 1u : uint32_t(t > 0));
+          tcgen05_commit(&sh->empty[b]);
+          tcgen05_commit(&sh->added[mine]);
+        }
+      } else if (shared_tokens && leader) {
+        // A tile that both halves count and only the other sees is given back when it is there, not earlier, so that an
+        // arrival cannot count for the buffer's previous item.
+        mbarrier_arrive(&sh->empty[2 * i % kBuffers]);
+        mbarrier_arrive(&sh->empty[b]);
       }
-      ++t;
     }
     if (leader) tcgen05_commit(&sh->done);
   }

@@ -6,7 +6,7 @@
 
 namespace ei {
 
-constexpr int kSpanTile = 128;   // tokens of a tile
+constexpr int kSpanTile = 64;    // tokens of a tile
 constexpr int kSpanBox = 32;     // tokens of a copy: a tile may be put together from several stretches
 constexpr int kSpanRows = 128;   // stacked query rows of a query tile; a block has two
 
