@@ -31,7 +31,7 @@ namespace ei {
 namespace {
 
 constexpr int kDim = 128;
-constexpr int kThreads = 384;
+constexpr int kThreads = 640;
 constexpr int kHalfBytes = kSpanTile * 128;  // 64 values of a tile's tokens
 constexpr int kBufferBytes = 2 * kHalfBytes;
 constexpr int kBoxBytes = kSpanBox * 128;
@@ -39,20 +39,25 @@ constexpr int kBoxes = kSpanTile / kSpanBox;
 constexpr int kBuffers = 8;
 constexpr int kQueryBytes = 2 * kSpanRows * 128;
 constexpr float kSlack = 8.0f;  // powers of two
-constexpr size_t kSpanSharedBytes = size_t(2) * kQueryBytes + size_t(kBuffers) * kBufferBytes + 1024 + 512;
+constexpr size_t kStateBytes = 4096;
+constexpr size_t kSpanSharedBytes = size_t(2) * kQueryBytes + size_t(kBuffers) * kBufferBytes + 1024 + kStateBytes;
 static_assert(kSpanSharedBytes <= 227 * 1024, "a block's buffers fit an SM");
 
 struct SpanShared {
   uint64_t full[kBuffers], empty[kBuffers];  // K and V tiles in turn
   uint64_t queries[2];                       // a query tile is in shared memory
   uint64_t scores[2][2], weights[2][2];      // [half][place]: S computed, P written
-  uint64_t added[2];                         // O holds the tile's product
+  uint64_t added[2][2];                      // [half][tile & 1]: O holds the tile's product
+  uint64_t decided[2][4][2];                 // [half][warp of four][tile & 1]: what the tile's weights are relative to
+  uint64_t pairs[2][4];                      // both warps of 32 rows have left their sums
   uint64_t done;                             // every MMA issued has completed
   uint32_t tmem_base;
   volatile int abort;
+  float reference[2][kSpanRows];  // [half][row]: the running maximum that weights are relative to
+  float sums[2][2][kSpanRows];    // [half][turn][row]
   int issued, query_tiles;  // items, and a bit for each query tile, whose copies were requested
 };
-static_assert(sizeof(SpanShared) <= 512, "the block's state lies behind the ring");
+static_assert(sizeof(SpanShared) <= kStateBytes, "the block's state lies behind the ring");
 
 __device__ __forceinline__ void tmem_request32(uint32_t address, uint32_t* r) {
   __syncwarp();
@@ -154,15 +159,19 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
       for (int place = 0; place < 2; ++place) {
         mbarrier_init(&sh->scores[i][place], 1);
         mbarrier_init(&sh->weights[i][place], 4);
+        mbarrier_init(&sh->added[i][place], 1);
+        for (int w = 0; w < 4; ++w) mbarrier_init(&sh->decided[i][w][place], 1);
       }
-      mbarrier_init(&sh->added[i], 1);
     }
+    for (int i = 0; i < 2; ++i)
+      for (int w = 0; w < 4; ++w) mbarrier_init(&sh->pairs[i][w], 2);
     mbarrier_init(&sh->done, 2);
     sh->abort = 0;
     sh->issued = sh->query_tiles = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 11) tmem_alloc(&sh->tmem_base, 512);
+  if (threadIdx.x < 2 * kSpanRows) sh->reference[threadIdx.x / kSpanRows][threadIdx.x % kSpanRows] = -INFINITY;
+  if (warp == 19) tmem_alloc(&sh->tmem_base, 512);
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
@@ -181,17 +190,18 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
   const long long row0 = (long long)sequence * p.rows;
 
   // The row of a softmax thread.
-  const int half = (warp >> 2) & 1, row_of_tile = threadIdx.x & (kSpanRows - 1);
+  const int half = (warp >> 3) & 1, turn = (warp >> 2) & 1, row_of_tile = threadIdx.x & (kSpanRows - 1);
   const int index = query_tile_of(half) * kSpanRows + row_of_tile;
-  const bool live = warp < 8 && index < stacked;
+  const bool live = warp < 16 && index < stacked;
   const int row = live ? index / group : 0, head = kv_head * group + (live ? index - row * group : 0);
-  float* const partial =
-      p.partial + ((size_t(partial_first + (shared_tokens ? 0 : half)) * p.sequences * p.rows + row0 + row) * p.heads + head) * kStepPartial;
-  bf16* const out = p.out + (row0 + row) * p.out_stride + size_t(head) * kDim;
+  auto partial_of_row = [&] {
+    return p.partial + ((size_t(partial_first + (shared_tokens ? 0 : half)) * p.sequences * p.rows + row0 + row) * p.heads + head) * kStepPartial;
+  };
+  auto out_of_row = [&] { return p.out + (row0 + row) * p.out_stride + size_t(head) * kDim; };
 
-  if (warp < 8) {
-    // ---- weights: thread = query row ----
-    if (!p.copied_queries && (shared_tokens || half == 0)) {
+  if (warp < 16) {
+    // ---- weights: thread = query row, of every other tile ----
+    if (!p.copied_queries && turn == 0 && (shared_tokens || half == 0)) {
       unsigned char* const own = smem + half * kQueryBytes + row_of_tile * 128;
       const bf16* q = p.q + (row0 + row) * p.q_stride + size_t(head) * kDim;
 #pragma unroll 1
@@ -211,56 +221,68 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
     const int last = p.together ? length - 1 : base + row;
     const bool some_live = __any_sync(0xffffffffu, live);
     const float exponent_scale = rsqrtf(float(kDim)) * kLog2e;
-    float maximum = -INFINITY, sum = 0.0f;
+    float maximum = -INFINITY, sum = 0.0f;  // the sum is relative to `maximum`, the reference as this thread last saw it
     const float2 scales = make_float2(exponent_scale, exponent_scale);
     const int tiles = half ? tiles1 : tiles0;
     // Boxes that every row of the half sees whole.
     const int clean_begin = sink_boxes + (max(0, (half ? last_position1 : last_position0) - p.window + 1 - low) + kSpanBox - 1) / kSpanBox;
     const int clean_end = sink_boxes + max(0, min(end, (half ? first_position1 : first_position0) + 1) - low) / kSpanBox;
     bool ok = true;
-    for (int t = 0; t < tiles; ++t) {
+    for (int t = turn; t < tiles; t += 2) {
       const int item = item_of(half, t), box0 = box_begin + item * kBoxes;
       const bool clean = box0 >= clean_begin && box0 + kBoxes <= clean_end;
       const uint32_t at = places + (t & 1) * 64;
       ok = __all_sync(0xffffffffu, wait(&sh->scores[half][t & 1], (t >> 1) & 1));
       if (!ok) break;
       tcgen05_fence_after();
-      uint32_t s[2][32];
+      uint32_t s[32];
       float2 shifts = make_float2(0.0f, 0.0f);
       float rescale = 1.0f;
       bool moved_some = false;
-      if (some_live) {
-        tmem_request32(at, s[0]);
-        tmem_request32(at + 32, s[1]);
-        tmem_loaded32(s[0]);
-        tmem_loaded32(s[1]);
-        float tops[4];
+      auto fetch = [&](int box) {
+        tmem_request32(at + box * 32, s);
+        tmem_loaded32(s);
+        if (!clean) {
+          const int start = start_of(box0 + box);
+          const uint32_t seen = below(min(stop_of(box0 + box), last + 1) - start) &
+                                (below(p.sinks - start) | ~below(last - p.window + 1 - start));
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (!clean) {
-            const int start = start_of(box0 + i);
-            const uint32_t seen = below(min(stop_of(box0 + i), last + 1) - start) &
-                                  (below(p.sinks - start) | ~below(last - p.window + 1 - start));
-#pragma unroll
-            for (int j = 0; j < 32; ++j) s[i][j] = seen >> j & 1 ? s[i][j] : 0xff800000u;
-          }
-#pragma unroll
-          for (int part = 0; part < 2; ++part) {
-            float& most = tops[2 * i + part];
-            most = __uint_as_float(s[i][16 * part]);
-#pragma unroll
-            for (int j = 1; j < 16; ++j) most = fmaxf(most, __uint_as_float(s[i][16 * part + j]));
-          }
+          for (int j = 0; j < 32; ++j) s[j] = seen >> j & 1 ? s[j] : 0xff800000u;
         }
-        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-        const bool moved = maximum == -INFINITY ? top != -INFINITY : (top - maximum) * exponent_scale > kSlack;
-        const float previous = maximum;
-        if (moved) maximum = top;
-        // A row with nothing visible yet keeps -inf; 0 as the exponent's base then makes every weight 0.
-        const float reference = maximum == -INFINITY ? 0.0f : maximum;
-        shifts.x = shifts.y = -reference * exponent_scale;
-        if (moved) rescale = power_of_two((previous - reference) * exponent_scale);
+      };
+      auto largest = [&] {
+        float tops[2];
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          tops[part] = __uint_as_float(s[16 * part]);
+#pragma unroll
+          for (int j = 1; j < 16; ++j) tops[part] = fmaxf(tops[part], __uint_as_float(s[16 * part + j]));
+        }
+        return fmaxf(tops[0], tops[1]);
+      };
+      if (some_live) {
+        fetch(0);
+        float top = largest();
+        fetch(1);  // stays in registers, the other box is fetched once more
+        top = fmaxf(top, largest());
+        // The reference as the other warp of these rows left it with the tile before.
+        if (t > 0) {
+          ok = __all_sync(0xffffffffu, wait(&sh->decided[half][warp & 3][(t - 1) & 1], ((t - 1) >> 1) & 1));
+          if (!ok) break;
+        }
+        const float previous = sh->reference[half][row_of_tile];
+        const bool moved = previous == -INFINITY ? top != -INFINITY : (top - previous) * exponent_scale > kSlack;
+        const float current = moved ? top : previous;
         moved_some = __any_sync(0xffffffffu, moved);
+        if (moved) sh->reference[half][row_of_tile] = current;
+        __syncwarp();
+        if (lane == 0) mbarrier_arrive(&sh->decided[half][warp & 3][t & 1]);
+        // A row with nothing visible yet keeps -inf; 0 as the exponent's base then makes every weight 0.
+        const float base_of = current == -INFINITY ? 0.0f : current;
+        shifts.x = shifts.y = -base_of * exponent_scale;
+        if (moved) rescale = power_of_two((previous - base_of) * exponent_scale);
+        if (current != maximum) sum *= power_of_two((maximum - base_of) * exponent_scale);
+        maximum = current;
       }
       if (!clean) {
         // V's rows that are no token of the list are cleared: nothing there may pass through a zero weight. (Both halves'
@@ -282,9 +304,8 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
         // In groups of 16, a group's exponentials ahead of the conversions of the one before it: taken pair by pair, each
         // conversion waited for its own two exponentials, 20 cycles a value instead of 8.
         float2 parts[2] = {};
-        uint32_t packed[2][16];
         auto exponentials = [&](int group) {
-          uint32_t* const v = &s[group >> 1][(group & 1) * 16];
+          uint32_t* const v = &s[group * 16];
 #pragma unroll
           for (int j = 0; j < 16; j += 2) {
             const float2 x = fma_pair(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), scales, shifts);
@@ -293,33 +314,38 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
 #pragma unroll
           for (int j = 0; j < 16; ++j) asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+r"(v[j]));
         };
-        auto convert = [&](int group) {
-          const uint32_t* const v = &s[group >> 1][(group & 1) * 16];
+        auto convert = [&](int group, uint32_t* packed) {
+          const uint32_t* const v = &s[group * 16];
 #pragma unroll
           for (int j = 0; j < 16; j += 2) {
             uint32_t both;
             asm volatile("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(both) : "f"(__uint_as_float(v[j + 1])), "f"(__uint_as_float(v[j])));
-            packed[group >> 1][(group & 1) * 8 + j / 2] = both;
+            packed[j / 2] = both;
             parts[j / 2 & 1] = add_pair(parts[j / 2 & 1], make_float2(bf16_lo(both), bf16_hi(both)));
           }
         };
+        uint32_t last_box[16];
         exponentials(0);
         exponentials(1);
-        convert(0);
-        exponentials(2);
-        convert(1);
-        tmem_store16(at, packed[0]);
-        exponentials(3);
-        convert(2);
-        convert(3);
-        tmem_store16(at + 16, packed[1]);
+        convert(0, last_box);
+        convert(1, last_box + 8);
+        fetch(0);
+        // Both boxes' scores have been read: the weights may lie over them.
+        tmem_store16(at + 16, last_box);
+        uint32_t first_box[16];
+        exponentials(0);
+        exponentials(1);
+        convert(0, first_box);
+        convert(1, first_box + 8);
+        tmem_store16(at, first_box);
         const float2 total = add_pair(parts[0], parts[1]);
-        sum = sum * rescale + (total.x + total.y);
+        sum += total.x + total.y;
       }
-      if (t > 0) {
-        ok = __all_sync(0xffffffffu, wait(&sh->added[half], (t - 1) & 1));  // each in its turn: phases are told apart by parity
+      if (moved_some) {
+        // Scores of this tile were asked for behind the product of the last but one: only the last one's may be missing.
+        ok = t == 0 || __all_sync(0xffffffffu, wait(&sh->added[half][(t - 1) & 1], ((t - 1) >> 1) & 1));
         if (!ok) break;
-        if (moved_some) {
+        if (t > 0) {
           tcgen05_fence_after();
 #pragma unroll 1
           for (int i = 0; i < 8; ++i) {
@@ -338,12 +364,29 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
       if (lane == 0) mbarrier_arrive(&sh->weights[half][t & 1]);
     }
     const bool any = tiles > 0;
-    if (any) ok = ok && __all_sync(0xffffffffu, wait(&sh->added[half], (tiles - 1) & 1));
+    // The last product but one, whose phase might else be taken for the last one's, then the last.
+    if (tiles > 1) ok = ok && __all_sync(0xffffffffu, wait(&sh->added[half][tiles & 1], ((tiles - 2) >> 1) & 1));
+    if (any) ok = ok && __all_sync(0xffffffffu, wait(&sh->added[half][(tiles - 1) & 1], ((tiles - 1) >> 1) & 1));
+    if (any && some_live && ((tiles - 1) & 1) != turn)
+      ok = ok && __all_sync(0xffffffffu, wait(&sh->decided[half][warp & 3][(tiles - 1) & 1], ((tiles - 1) >> 1) & 1));
+    if (any && some_live && ok) {
+      // The row's sum is that of both its threads, relative to the final reference.
+      const float reference = sh->reference[half][row_of_tile];
+      if (maximum != reference) sum = maximum == -INFINITY ? 0.0f : sum * power_of_two((maximum - reference) * exponent_scale);
+      maximum = reference;
+      sh->sums[half][turn][row_of_tile] = sum;
+      __syncwarp();
+      if (lane == 0) mbarrier_arrive(&sh->pairs[half][warp & 3]);
+      ok = __all_sync(0xffffffffu, wait(&sh->pairs[half][warp & 3], 0));
+      sum = sh->sums[half][0][row_of_tile] + sh->sums[half][1][row_of_tile];
+    }
     if (ok) {
       tcgen05_fence_after();
+      float* const partial = partial_of_row();
+      bf16* const out = out_of_row();
       const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll 1
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 2 * turn; i < 2 * turn + 2; ++i) {
         uint32_t v[32];
         if (any) {
           tmem_request32(outputs + i * 32, v);
@@ -369,9 +412,9 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
           }
         }
       }
-      if (live && p.together) *reinterpret_cast<float2*>(partial + kDim) = make_float2(maximum * exponent_scale, sum);
+      if (live && p.together && turn == 0) *reinterpret_cast<float2*>(partial + kDim) = make_float2(maximum * exponent_scale, sum);
     }
-  } else if (warp == 8) {
+  } else if (warp == 16) {
     // ---- copies ----
     if (lane == 0) {
       if (p.copied_queries)
@@ -397,9 +440,9 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
         sh->issued = i + 1;
       }
     }
-  } else if (warp == 9 || warp == 10) {
+  } else if (warp < 19) {
     // ---- MMAs of one half ----
-    const int mine = warp - 9, n = mine ? tiles1 : tiles0;
+    const int mine = warp - 17, n = mine ? tiles1 : tiles0;
     const uint32_t leader = elect_one();
     constexpr uint32_t kScores = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(kSpanTile >> 3) << 17) | (uint32_t(kSpanRows >> 4) << 24);
     // The values' 128 columns are N-major: bit 16.
@@ -453,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
             umma_bf16_ts(outputs, tmem + mine * 256 + (t & 1) * 64 + k * 8, values + k * (16 * 128 >> 4), kUmmaDescHigh, kOutputs,
                          k > 0 ? 1u : uint32_t(t > 0));
           tcgen05_commit(&sh->empty[b]);
-          tcgen05_commit(&sh->added[mine]);
+          tcgen05_commit(&sh->added[mine][t & 1]);
         }
       } else if (shared_tokens && leader) {
         // A tile that both halves count and only the other sees is given back when it is there, not earlier, so that an
@@ -477,6 +520,8 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
     __syncthreads();
     if (live) {
       const uint32_t nan = 0x7fffffffu;
+      float* const partial = partial_of_row();
+      bf16* const out = out_of_row();
       for (int j = 0; j < kDim; ++j) {
         if (p.together) partial[j] = __uint_as_float(nan);
         else reinterpret_cast<uint16_t*>(out)[j] = 0x7fff;
@@ -485,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
     }
   }
   tcgen05_fence_after();
-  if (warp == 11) {
+  if (warp == 19) {
     __syncwarp();
     tmem_dealloc(tmem, 512);
   }

@@ -27,22 +27,25 @@ namespace ei {
 namespace {
 
 constexpr int kDim = 128;
-constexpr int kThreads = kStepWarps * 32;
 constexpr int kBuffer = kStepTile * kDim * 2;
 constexpr int kBuffers = 3;
 
+template <int kWarps>
 struct StepShared {
-  uint64_t full[kStepWarps][kBuffers];
-  float maxima[kStepWarps][kStepRows], sums[kStepWarps][kStepRows];
-  // Of the block, read by the others of the cluster.
-  float maximum[kStepRows], sum[kStepRows];
-  float factor[kStepMaxSplits][kStepRows];  // weight of each block's result in the joined one
+  uint64_t full[kWarps][kBuffers];
+  float maxima[kWarps][kStepRows], sums[kWarps][kStepRows];
+  float2 blocks[kStepMaxSplits][kStepRows];  // maximum and sum of every block of the cluster; each block leaves its own everywhere
+  float factor[kStepMaxSplits][kStepRows];   // weight of each block's result in the joined one
   float top[kStepRows], inverse[kStepRows];
-  float other[kSpanMostPartials][kStepRows];  // the same of what is joined
 };
-constexpr size_t step_shared(int row_tiles) {
-  return size_t(kStepWarps) * kBuffers * kBuffer + (row_tiles > 1 ? size_t(kStepRows) * kDim * 2 : 0) + sizeof(StepShared) + 1024;
+constexpr size_t step_shared(int warps, int row_tiles) {
+  return size_t(warps) * kBuffers * kBuffer + (row_tiles > 1 ? size_t(kStepRows) * kDim * 2 : 0) +
+         (warps == 8 ? sizeof(StepShared<8>) : sizeof(StepShared<4>)) + 1024;
 }
+static_assert(2 * (step_shared(4, 2) + 1024) <= 228 * 1024 && step_shared(8, 2) <= 227 * 1024, "two small blocks or a large one fit an SM");
+// When the ring is done with, a warp's part of it holds its sums in front, and behind the second warp's lies what joined results
+// say of themselves.
+static_assert(kStepRows * kDim * 4 + kSpanMostPartials * kStepRows * 8 <= kBuffers * kBuffer, "sums and joined results fit");
 
 __device__ __forceinline__ int tile_offset(int token, int chunk) {
   return (chunk >> 3) * (kStepTile * 128) + token * 128 + (((chunk & 7) ^ (token & 7)) << 4);
@@ -60,6 +63,15 @@ __device__ __forceinline__ uint32_t cluster_size() {
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
+// Every block of the cluster has started: only then may its shared memory be written.
+__device__ __forceinline__ void cluster_started() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait_started() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void cluster_sync() {
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -69,10 +81,8 @@ __device__ __forceinline__ uint32_t remote_address(const void* own, uint32_t ran
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_address(own)), "r"(rank));
   return a;
 }
-__device__ __forceinline__ float remote_float(const void* own, uint32_t rank) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote_address(own, rank)) : "memory");
-  return v;
+__device__ __forceinline__ void remote_store(const void* own, uint32_t rank, float2 v) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(remote_address(own, rank)), "f"(v.x), "f"(v.y) : "memory");
 }
 __device__ __forceinline__ float4 remote_float4(const void* own, uint32_t rank) {
   float4 v;
@@ -83,14 +93,17 @@ __device__ __forceinline__ float4 remote_float4(const void* own, uint32_t rank) 
   return v;
 }
 
-template <int kRowTiles, bool kWeights>
-__global__ void __launch_bounds__(kThreads, 2) step_attention_kernel(const __grid_constant__ StepAttentionParams p) {
+template <int kWarps, int kRowTiles, bool kWeights>
+__global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attention_kernel(const __grid_constant__ StepAttentionParams p) {
+  constexpr int kThreads = kWarps * 32;
   extern __shared__ unsigned char step_smem_raw[];
   unsigned char* const smem = step_smem_raw + ((1024u - (smem_address(step_smem_raw) & 1023u)) & 1023u);
-  unsigned char* const queries = smem + kStepWarps * kBuffers * kBuffer;
-  StepShared* const sh = reinterpret_cast<StepShared*>(queries + (kRowTiles > 1 ? kStepRows * kDim * 2 : 0));
+  unsigned char* const queries = smem + kWarps * kBuffers * kBuffer;
+  using Shared = StepShared<kWarps>;
+  Shared* const sh = reinterpret_cast<Shared*>(queries + (kRowTiles > 1 ? kStepRows * kDim * 2 : 0));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const uint32_t rank = cluster_rank(), splits = cluster_size();
+  cluster_started();
   const int kv_head = blockIdx.x / splits, sequence = blockIdx.y;
   const int group = p.heads / p.kv_heads, stacked = p.rows * group;
   const int first_stacked = (p.first_group + int(blockIdx.z)) * kStepRows;
@@ -114,7 +127,7 @@ __global__ void __launch_bounds__(kThreads, 2) step_attention_kernel(const __gri
   auto start_of = [&](int tile) { return tile < sink_tiles ? tile * kStepTile : low + (tile - sink_tiles) * kStepTile; };
   // Item 2n is K and 2n + 1 V of this warp's n-th tile; item i lies in buffer i % 3.
   auto request = [&](int item) {
-    const int tile = first_tile + warp + (item >> 1) * kStepWarps;
+    const int tile = first_tile + warp + (item >> 1) * kWarps;
     if (tile >= last_tile) return;
     uint64_t* bar = &full[item % kBuffers];
     mbarrier_expect_tx(bar, kBuffer);
@@ -181,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 2) step_attention_kernel(const __gri
   bool ok = true;
   int item = 0, buffer = 0;
   uint32_t parity = 0;
-  for (int tile = first_tile + warp; tile < last_tile; tile += kStepWarps) {
+  for (int tile = first_tile + warp; tile < last_tile; tile += kWarps) {
     ok = __all_sync(0xffffffffu, mbarrier_wait(&full[buffer], parity));
     if (!ok) break;
     const unsigned char* ks = ring + buffer * kBuffer;
@@ -321,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 2) step_attention_kernel(const __gri
     // anything else, and the unit's rows come out as NaN.
     if (lane == 0) {
       for (int i = item; i < item + kBuffers; ++i) {
-        if (first_tile + warp + (i >> 1) * kStepWarps < last_tile) mbarrier_wait(&full[i % kBuffers], (i / kBuffers) & 1);
+        if (first_tile + warp + (i >> 1) * kWarps < last_tile) mbarrier_wait(&full[i % kBuffers], (i / kBuffers) & 1);
       }
     }
     __syncwarp();
@@ -345,18 +358,35 @@ __global__ void __launch_bounds__(kThreads, 2) step_attention_kernel(const __gri
     }
   __syncthreads();
   constexpr int kUnitRows = kRowTiles * 16;
-  if (threadIdx.x < kUnitRows) {
-    const int i = threadIdx.x;
+  const size_t slots = size_t(p.sequences) * p.rows * p.heads;
+  auto slot_of = [&](int i) {
+    const int r = row_of(i);
+    return size_t(row0 + r) * p.heads + kv_head * group + (first_stacked + i - r * group);
+  };
+  auto real = [&](int i) { return i < have && (p.together || base + row_of(i) >= 0); };
+  auto others_of = [&](int i) { return p.joined && real(i) ? joined_of(i) : 0; };
+  // Results to be joined say their maximum and sum: requested by all threads at once.
+  float2(*const others)[kStepRows] =
+      reinterpret_cast<float2(*)[kStepRows]>(smem + 2 * kBuffers * kBuffer - kSpanMostPartials * kStepRows * sizeof(float2));
+  if (p.joined) {
+    for (int e = threadIdx.x; e < kSpanMostPartials * kUnitRows; e += kThreads) {
+      const int j = e / kUnitRows, i = e % kUnitRows;
+      if (j < others_of(i)) others[j][i] = *reinterpret_cast<const float2*>(p.joined + (j * slots + slot_of(i)) * kStepPartial + kDim);
+    }
+  }
+  cluster_wait_started();
+  // The block's maximum and sum of a row go to every block of the cluster, so that joining starts with values at hand.
+  for (int e = threadIdx.x; e < kUnitRows * int(splits); e += kThreads) {
+    const int i = e % kUnitRows;
     float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kStepWarps; ++w) top = fmaxf(top, sh->maxima[w][i]);
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sh->maxima[w][i]);
 #pragma unroll
-    for (int w = 0; w < kStepWarps; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
       const float part = sh->sums[w][i];
       if (part != 0.0f) sum += part * power_of_two(sh->maxima[w][i] - top);  // a warp without a visible token has none
     }
-    sh->maximum[i] = top;
-    sh->sum[i] = sum;
+    remote_store(&sh->blocks[rank][i], e / kUnitRows, make_float2(top, sum));
   }
   float* const area = reinterpret_cast<float*>(ring);  // [rows][128]
 #pragma unroll
@@ -364,7 +394,9 @@ __global__ void __launch_bounds__(kThreads, 2) step_attention_kernel(const __gri
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int i = rt * 16 + half * 8 + g;
-      const float top = fmaxf(fmaxf(sh->maxima[0][i], sh->maxima[1][i]), fmaxf(sh->maxima[2][i], sh->maxima[3][i]));
+      float top = sh->maxima[0][i];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sh->maxima[w][i]);
       const float factor = m[rt][half] == -INFINITY ? 0.0f : power_of_two(m[rt][half] - top);
 #pragma unroll
       for (int d = 0; d < 16; ++d)
@@ -373,10 +405,10 @@ __global__ void __launch_bounds__(kThreads, 2) step_attention_kernel(const __gri
     }
   __syncthreads();
   float* const block_area = reinterpret_cast<float*>(smem);
-  for (int i = threadIdx.x; i < kUnitRows * (kDim / 4); i += kThreads) {
+  for (int i = threadIdx.x; i < min(kUnitRows, have) * (kDim / 4); i += kThreads) {
     float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-    for (int w = 0; w < kStepWarps; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
       const float4 v = reinterpret_cast<const float4*>(smem + w * kBuffers * kBuffer)[i];
       total.x += v.x, total.y += v.y, total.z += v.z, total.w += v.w;
     }
@@ -388,105 +420,125 @@ __global__ void __launch_bounds__(kThreads, 2) step_attention_kernel(const __gri
   // Joined over the cluster and with what other kernels left.
   if (threadIdx.x < kUnitRows) {
     const int i = threadIdx.x;
-    const bool real = i < have && (p.together || base + row_of(i) >= 0);
+    const int count = others_of(i);
     float top = -INFINITY, sum = 0.0f;
-    for (uint32_t r = 0; r < splits; ++r) top = fmaxf(top, remote_float(&sh->maximum[i], r));
-    const size_t slots = size_t(p.sequences) * p.rows * p.heads;
-    size_t slot = 0;
-    if (i < have) {
-      const int r = row_of(i);
-      slot = size_t(row0 + r) * p.heads + kv_head * group + (first_stacked + i - r * group);
-    }
-    const int others = real && p.joined ? joined_of(i) : 0;
-    for (int j = 0; j < others; ++j) top = fmaxf(top, p.joined[(j * slots + slot) * kStepPartial + 128]);
+    for (uint32_t r = 0; r < splits; ++r) top = fmaxf(top, sh->blocks[r][i].x);
+    for (int j = 0; j < count; ++j) top = fmaxf(top, others[j][i].x);
     for (uint32_t r = 0; r < splits; ++r) {
-      const float part = remote_float(&sh->sum[i], r);
-      const float factor = part == 0.0f ? 0.0f : power_of_two(remote_float(&sh->maximum[i], r) - top);
+      const float2 part = sh->blocks[r][i];
+      const float factor = part.y == 0.0f ? 0.0f : power_of_two(part.x - top);
       sh->factor[r][i] = factor;
-      if (part != 0.0f) sum += part * factor;
+      if (part.y != 0.0f) sum += part.y * factor;
     }
-    for (int j = 0; j < others; ++j) {
-      const float* from = p.joined + (j * slots + slot) * kStepPartial;
-      const float part = from[129], factor = part == 0.0f ? 0.0f : power_of_two(from[128] - top);
-      sh->other[j][i] = factor;
-      if (part != 0.0f) sum += part * factor;
+    for (int j = 0; j < count; ++j) {
+      const float2 part = others[j][i];
+      const float factor = part.y == 0.0f ? 0.0f : power_of_two(part.x - top);
+      others[j][i].x = factor;
+      if (part.y != 0.0f) sum += part.y * factor;
     }
     sh->top[i] = top;
-    sh->inverse[i] = !real || sum == 0.0f ? 0.0f : p.partial ? sum : 1.0f / sum;
+    sh->inverse[i] = !real(i) || sum == 0.0f ? 0.0f : p.partial ? sum : 1.0f / sum;
   }
   __syncthreads();
   {
     const int quads = have * (kDim / 4);
     const int from = int((long long)quads * rank / splits), to = int((long long)quads * (rank + 1) / splits);
-    const size_t slots = size_t(p.sequences) * p.rows * p.heads;
     for (int e = from + int(threadIdx.x); e < to; e += kThreads) {
       const int i = e / (kDim / 4), quad = e % (kDim / 4);
       const float* own = block_area + i * kDim + ((quad * 4) ^ ((i & 3) << 3));
       float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      for (uint32_t r = 0; r < splits; ++r) {
-        const float factor = sh->factor[r][i];
-        if (factor == 0.0f) continue;
-        const float4 v = remote_float4(own, r);
+      auto add = [&](float4 v, float factor) {
+        if (factor == 0.0f) return;  // nothing visible there: not even a product that is no number counts
         total.x = fmaf(v.x, factor, total.x), total.y = fmaf(v.y, factor, total.y);
         total.z = fmaf(v.z, factor, total.z), total.w = fmaf(v.w, factor, total.w);
+      };
+#pragma unroll 1
+      for (uint32_t r0 = 0; r0 < splits; r0 += 8) {
+        float4 v[8];
+#pragma unroll
+        for (uint32_t u = 0; u < 8; ++u)
+          if (r0 + u < splits) v[u] = remote_float4(own, r0 + u);
+#pragma unroll
+        for (uint32_t u = 0; u < 8; ++u)
+          if (r0 + u < splits) add(v[u], sh->factor[r0 + u][i]);
       }
-      const int r = row_of(i), h = kv_head * group + first_stacked + i - r * group;
-      const size_t slot = size_t(row0 + r) * p.heads + h;
-      const int others = p.joined && (p.together || base + r >= 0) ? joined_of(i) : 0;
-#pragma unroll 4
-      for (int j = 0; j < others; ++j) {
-        const float factor = sh->other[j][i];
-        const float4 v = *reinterpret_cast<const float4*>(p.joined + (j * slots + slot) * kStepPartial + quad * 4);
-        total.x = fmaf(v.x, factor, total.x), total.y = fmaf(v.y, factor, total.y);
-        total.z = fmaf(v.z, factor, total.z), total.w = fmaf(v.w, factor, total.w);
+      const size_t slot = slot_of(i);
+      const int count = others_of(i);
+#pragma unroll 1
+      for (int j0 = 0; j0 < count; j0 += 8) {
+        float4 v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (j0 + u < count) v[u] = *reinterpret_cast<const float4*>(p.joined + ((j0 + u) * slots + slot) * kStepPartial + quad * 4);
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (j0 + u < count) add(v[u], others[j0 + u][i].x);
       }
       const float inverse = sh->inverse[i];
       if (p.partial) {
         float* to_slot = p.partial + slot * kStepPartial;
         *reinterpret_cast<float4*>(to_slot + quad * 4) = total;
-        if (quad == 0) to_slot[128] = sh->top[i], to_slot[129] = inverse;
+        if (quad == 0) *reinterpret_cast<float2*>(to_slot + kDim) = make_float2(sh->top[i], inverse);
       } else {
         uint2 packed = make_uint2(0u, 0u);
         if (inverse != 0.0f) {  // also a NaN
           packed.x = pack_bf16(total.x * inverse, total.y * inverse);
           packed.y = pack_bf16(total.z * inverse, total.w * inverse);
         }
-        *reinterpret_cast<uint2*>(p.out + (row0 + r) * p.out_stride + size_t(h) * kDim + quad * 4) = packed;
+        const int r = row_of(i);
+        *reinterpret_cast<uint2*>(p.out + (row0 + r) * p.out_stride + size_t(kv_head * group + first_stacked + i - r * group) * kDim + quad * 4) =
+            packed;
       }
     }
   }
   if (kWeights) {
-    // This block's tokens: the sum over the rows, in their order.
+    // This block's tokens: the sum over the rows, in their order. A thread has four tokens under way.
     const float* scores = p.scores ? p.scores + sequence * p.scores_sequence + kv_head * p.scores_head : nullptr;
     float* scores_out = p.scores_out + sequence * p.out_sequence + kv_head * p.out_head;
     const int stop = min(last_tile * kStepTile, end);
-    for (int t = first_tile * kStepTile + int(threadIdx.x); t < stop; t += kThreads) {
-      float sum = 0.0f;
+    for (int t0 = first_tile * kStepTile + int(threadIdx.x); t0 < stop; t0 += 4 * kThreads) {
+      float sum[4] = {}, old[4] = {};
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (scores && t0 + u * kThreads < stop) old[u] = scores[t0 + u * kThreads];
+#pragma unroll 2
       for (int i = 0; i < have; ++i) {
-        const float inverse = sh->inverse[i];
-        if (inverse != 0.0f) sum = fmaf(power_of_two(raw[size_t(i) * p.raw_stride + t] - sh->top[i]), inverse, sum);
+        const float inverse = sh->inverse[i], top = inverse == 0.0f ? 0.0f : sh->top[i];
+        float score[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          score[u] = t0 + u * kThreads < stop ? raw[size_t(i) * p.raw_stride + t0 + u * kThreads] : -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (inverse != 0.0f) sum[u] = fmaf(power_of_two(score[u] - top), inverse, sum[u]);
       }
-      scores_out[t] = (scores ? scores[t] : 0.0f) + sum;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (t0 + u * kThreads < stop) scores_out[t0 + u * kThreads] = old[u] + sum[u];
     }
   }
   if (splits > 1) cluster_sync();  // no block leaves while another reads its shared memory
 }
 
+template <int kWarps>
 auto step_kernel(bool two, bool weights) {
-  return two ? (weights ? step_attention_kernel<2, true> : step_attention_kernel<2, false>)
-             : (weights ? step_attention_kernel<1, true> : step_attention_kernel<1, false>);
+  return two ? (weights ? step_attention_kernel<kWarps, 2, true> : step_attention_kernel<kWarps, 2, false>)
+             : (weights ? step_attention_kernel<kWarps, 1, true> : step_attention_kernel<kWarps, 1, false>);
 }
+auto step_kernel(int warps, bool two, bool weights) { return warps == 8 ? step_kernel<8>(two, weights) : step_kernel<4>(two, weights); }
 
 void configure_step_kernels() {
   static thread_local int configured_device = -1;
   int device = 0;
   EI_CUDA(cudaGetDevice(&device));
   if (configured_device == device) return;
-  for (const bool two : {false, true})
-    for (const bool weights : {false, true}) {
-      EI_CUDA(cudaFuncSetAttribute(step_kernel(two, weights), cudaFuncAttributeMaxDynamicSharedMemorySize, int(step_shared(two ? 2 : 1))));
-      EI_CUDA(cudaFuncSetAttribute(step_kernel(two, weights), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    }
+  for (const int warps : {4, 8})
+    for (const bool two : {false, true})
+      for (const bool weights : {false, true}) {
+        EI_CUDA(cudaFuncSetAttribute(step_kernel(warps, two, weights), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     int(step_shared(warps, two ? 2 : 1))));
+        EI_CUDA(cudaFuncSetAttribute(step_kernel(warps, two, weights), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+      }
   configured_device = device;
 }
 
@@ -507,21 +559,21 @@ void launch_step_attention(const StepAttentionParams& p, size_t tokens, cudaStre
   const int group = p.heads / p.kv_heads;
   const bool two = size_t(p.rows) * group > 16;
   const size_t units = size_t(p.kv_heads) * p.sequences * p.groups;
-  const int splits = step_splits(units, tokens, device_multiprocessors());
+  const StepShape shape = step_shape(units, tokens, device_multiprocessors());
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(unsigned(p.kv_heads * splits), unsigned(p.sequences), unsigned(p.groups));
-  config.blockDim = dim3(kThreads);
-  config.dynamicSmemBytes = step_shared(two ? 2 : 1);
+  config.gridDim = dim3(unsigned(p.kv_heads * shape.splits), unsigned(p.sequences), unsigned(p.groups));
+  config.blockDim = dim3(unsigned(shape.warps * 32));
+  config.dynamicSmemBytes = step_shared(shape.warps, two ? 2 : 1);
   config.stream = stream;
   cudaLaunchAttribute attributes[2]{};
   attributes[0].id = cudaLaunchAttributeClusterDimension;
-  attributes[0].val.clusterDim.x = unsigned(splits);
+  attributes[0].val.clusterDim.x = unsigned(shape.splits);
   attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
   attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attributes[1].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attributes;
   config.numAttrs = pdl ? 2 : 1;
-  check_cuda(cudaLaunchKernelEx(&config, step_kernel(two, p.raw != nullptr), p), "cudaLaunchKernelEx");
+  check_cuda(cudaLaunchKernelEx(&config, step_kernel(shape.warps, two, p.raw != nullptr), p), "cudaLaunchKernelEx");
 }
 
 }  // namespace ei

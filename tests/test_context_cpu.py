@@ -61,22 +61,42 @@ def test_scaled_rope_table_refuses_odd_widths(package):
         package.operators.build_rope_table_scaled(8, 63, 1e4)
 
 
-def test_step_splits(tmp_path):
-    """Powers of two, at most 16, no more than two tiles a warp allow, and enough blocks where there are tokens."""
-    source = tmp_path / "splits.cpp"
-    source.write_text('#include "step_choice.hpp"\n#include <cstdio>\n#include <cstdlib>\n'
-                      'int main(int, char** a) { std::printf("%d", ei::step_splits(atoll(a[1]), atoll(a[2]), 148)); }\n')
-    program = tmp_path / "splits"
+def run_choice(tmp_path, header, expression):
+    source = tmp_path / "choice.cpp"
+    source.write_text(f'#include "{header}"\n#include <cstdio>\n#include <cstdlib>\n'
+                      f'int main(int, char** a) {{ {expression} }}\n')
+    program = tmp_path / "choice"
     subprocess.run(["g++", "-std=c++17", "-I", str(ROOT / "edge-infer_b200" / "csrc"), "-o", str(program), str(source)], check=True)
+    return lambda *values: [int(x) for x in subprocess.run([str(program), *map(str, values)], check=True, capture_output=True,
+                                                           text=True).stdout.split()]
 
-    def splits(units, tokens):
-        return int(subprocess.run([str(program), str(units), str(tokens)], check=True, capture_output=True, text=True).stdout)
 
-    for units in (1, 4, 8, 40, 296, 512):
+def test_step_shape(tmp_path):
+    """Powers of two, at most 16, no more blocks than fit at once, no warp of a split unit without a tile."""
+    choose = run_choice(tmp_path, "step_choice.hpp", 'auto s = ei::step_shape(atoll(a[1]), atoll(a[2]), 148); '
+                                                     'std::printf("%d %d", s.splits, s.warps);')
+    for units in (1, 4, 8, 40, 149, 296, 512):
         for tokens in (0, 1, 31, 300, 5000, 200000):
-            n = splits(units, tokens)
-            assert n in (1, 2, 4, 8, 16)
-    assert splits(8, 0) == 1 and splits(512, 100000) == 1 and splits(8, 200000) == 16
+            splits, warps = choose(units, tokens)
+            assert splits in (1, 2, 4, 8, 16) and warps in (4, 8)
+            assert splits == 1 or (units * splits <= 148 and (tokens + 31) // 32 > splits // 2 * 8)
+    assert choose(8, 0) == [1, 8] and choose(512, 100000) == [1, 4] and choose(8, 200000) == [16, 8]
+
+
+def test_span_splits(tmp_path):
+    """Blocks fit the chip, rows have no more partial results than are joined, every stretch has tokens."""
+    choose = run_choice(tmp_path, "span_choice.hpp", 'auto s = ei::span_splits(atoll(a[1]), atoll(a[2]), atoi(a[3]), 148); '
+                                                     'std::printf("%d %d %d %d %d", s.pairs, s.pair_splits, s.single_splits, s.blocks(), '
+                                                     's.partials());')
+    for query_tiles in (1, 2, 3, 5, 8, 50, 400):
+        for tokens in (1, 63, 64, 65, 1000, 30011, 200000):
+            for kv_heads in (1, 4, 8):
+                pairs, pair_splits, single_splits, blocks, partials = choose(query_tiles, tokens, kv_heads)
+                tiles = (tokens + 63) // 64
+                assert pairs == query_tiles // 2 and (single_splits > 0) == (query_tiles % 2 == 1)
+                assert 1 <= partials <= 32 and blocks == pairs * pair_splits + single_splits
+                assert blocks * kv_heads <= 148 or (pair_splits == 1 and single_splits <= 1)
+                assert pair_splits <= tiles and single_splits <= tiles
 
 
 # ---- refusals: addresses are never looked at ------------------------------------------------------------------------------
