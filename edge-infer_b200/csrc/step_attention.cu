@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
 #pragma unroll
       for (int u = 0; u < 4; ++u)
         if (scores && t0 + u * kThreads < stop) old[u] = scores[t0 + u * kThreads];
-#pragma unroll 2
+#pragma unroll 4
       for (int i = 0; i < have; ++i) {
         const float inverse = sh->inverse[i], top = inverse == 0.0f ? 0.0f : sh->top[i];
         float score[4];
@@ -527,19 +527,42 @@ auto step_kernel(bool two, bool weights) {
 }
 auto step_kernel(int warps, bool two, bool weights) { return warps == 8 ? step_kernel<8>(two, weights) : step_kernel<4>(two, weights); }
 
-void configure_step_kernels() {
+cudaLaunchConfig_t step_config(const StepShape& shape, bool two, unsigned heads, unsigned sequences, unsigned groups,
+                               cudaLaunchAttribute* cluster) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(heads * unsigned(shape.splits), sequences, groups);
+  config.blockDim = dim3(unsigned(shape.warps * 32));
+  config.dynamicSmemBytes = step_shared(shape.warps, two ? 2 : 1);
+  cluster->id = cudaLaunchAttributeClusterDimension;
+  cluster->val.clusterDim.x = unsigned(shape.splits);
+  cluster->val.clusterDim.y = cluster->val.clusterDim.z = 1;
+  config.attrs = cluster;
+  config.numAttrs = 1;
+  return config;
+}
+
+// Sets the kernels up on the current device and says how many clusters it runs at once.
+const StepCapacity& configure_step_kernels() {
   static thread_local int configured_device = -1;
+  static thread_local StepCapacity capacity;
   int device = 0;
   EI_CUDA(cudaGetDevice(&device));
-  if (configured_device == device) return;
-  for (const int warps : {4, 8})
+  if (configured_device == device) return capacity;
+  for (const int warps : {4, 8}) {
     for (const bool two : {false, true})
       for (const bool weights : {false, true}) {
         EI_CUDA(cudaFuncSetAttribute(step_kernel(warps, two, weights), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      int(step_shared(warps, two ? 2 : 1))));
         EI_CUDA(cudaFuncSetAttribute(step_kernel(warps, two, weights), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
       }
+    for (int power = 0; power < 5; ++power) {
+      cudaLaunchAttribute cluster{};
+      const cudaLaunchConfig_t config = step_config({1 << power, warps}, true, 64, 1, 1, &cluster);
+      EI_CUDA(cudaOccupancyMaxActiveClusters(&(warps == 4 ? capacity.four : capacity.eight)[power], step_kernel(warps, true, true), &config));
+    }
+  }
   configured_device = device;
+  return capacity;
 }
 
 }  // namespace
@@ -555,24 +578,16 @@ void encode_cache_map(CUtensorMap* map, const CacheStrides& cache, size_t capaci
 }
 
 void launch_step_attention(const StepAttentionParams& p, size_t tokens, cudaStream_t stream, bool pdl) {
-  configure_step_kernels();
+  const StepCapacity& capacity = configure_step_kernels();
   const int group = p.heads / p.kv_heads;
   const bool two = size_t(p.rows) * group > 16;
-  const size_t units = size_t(p.kv_heads) * p.sequences * p.groups;
-  const StepShape shape = step_shape(units, tokens, device_multiprocessors());
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3(unsigned(p.kv_heads * shape.splits), unsigned(p.sequences), unsigned(p.groups));
-  config.blockDim = dim3(unsigned(shape.warps * 32));
-  config.dynamicSmemBytes = step_shared(shape.warps, two ? 2 : 1);
-  config.stream = stream;
+  const StepShape shape = step_shape(size_t(p.kv_heads) * p.sequences * p.groups, tokens, capacity);
   cudaLaunchAttribute attributes[2]{};
-  attributes[0].id = cudaLaunchAttributeClusterDimension;
-  attributes[0].val.clusterDim.x = unsigned(shape.splits);
-  attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t config = step_config(shape, two, unsigned(p.kv_heads), unsigned(p.sequences), unsigned(p.groups), attributes);
+  config.stream = stream;
   attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attributes[1].val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = attributes;
-  config.numAttrs = pdl ? 2 : 1;
+  if (pdl) config.numAttrs = 2;
   check_cuda(cudaLaunchKernelEx(&config, step_kernel(shape.warps, two, p.raw != nullptr), p), "cudaLaunchKernelEx");
 }
 

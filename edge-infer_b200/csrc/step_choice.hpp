@@ -9,20 +9,31 @@ namespace ei {
 constexpr int kStepTile = 32;   // tokens of a tile; a warp has one at a time
 constexpr int kStepMaxSplits = 16;
 
-// A unit's tokens are shared by the blocks of one cluster: a power of two of them, at most 16. `units` = sequences x KV heads x
-// groups of rows, `tokens` = most tokens a unit may read. One block of eight warps or two of four fit an SM.
+// A unit's tokens are shared by the blocks of one cluster: a power of two of them, at most 16, of four warps (two blocks fit
+// an SM) or eight.
 struct StepShape {
   int splits, warps;
 };
-inline StepShape step_shape(size_t units, size_t tokens, int multiprocessors) {
+// Clusters of 1, 2, 4, 8, 16 blocks that run at once. (A cluster stays within one group of SMs, and their sizes differ: of 16
+// blocks of eight warps a B200 takes 7, of four warps 14; an eighth of the former started 26 us late.)
+struct StepCapacity {
+  int four[5], eight[5];
+};
+
+// `units` = sequences x KV heads x groups of rows, `tokens` = most tokens a unit may read: as many warps at work as there are
+// while all clusters run at once and no warp is without a tile; of equal shapes the one of fewer, larger blocks, whose clusters
+// are smaller (8 units of 30000 tokens, 16 blocks of four warps or 8 of eight: 28.7 and 26.7 us).
+inline StepShape step_shape(size_t units, size_t tokens, const StepCapacity& capacity) {
   const size_t tiles = (tokens + kStepTile - 1) / kStepTile;
-  // Few units: eight warps a block, as many blocks as fit at once while every warp has a tile.
-  if (units <= size_t(multiprocessors)) {
-    int splits = 1;
-    while (splits < kStepMaxSplits && units * splits * 2 <= size_t(multiprocessors) && tiles > size_t(splits) * 8) splits *= 2;
-    return {splits, 8};
-  }
-  return {1, 4};
+  StepShape best{1, 4};
+  for (const int warps : {4, 8})
+    for (int power = 0; power < 5; ++power) {
+      const int splits = 1 << power;
+      const int fit = (warps == 4 ? capacity.four : capacity.eight)[power];
+      if (units > size_t(fit) || size_t(splits) * warps > std::max<size_t>(tiles, 4)) continue;
+      if (splits * warps >= best.splits * best.warps) best = {splits, warps};
+    }
+  return best;
 }
 
 }  // namespace ei

@@ -72,15 +72,18 @@ def run_choice(tmp_path, header, expression):
 
 
 def test_step_shape(tmp_path):
-    """Powers of two, at most 16, no more blocks than fit at once, no warp of a split unit without a tile."""
-    choose = run_choice(tmp_path, "step_choice.hpp", 'auto s = ei::step_shape(atoll(a[1]), atoll(a[2]), 148); '
+    """Powers of two, at most 16, all clusters at once where a unit is split at all, no warp of a split unit without a tile."""
+    four, eight = [296, 148, 71, 33, 14], [148, 74, 33, 15, 7]
+    choose = run_choice(tmp_path, "step_choice.hpp", f'ei::StepCapacity c{{{{{str(four)[1:-1]}}}, {{{str(eight)[1:-1]}}}}}; '
+                                                     'auto s = ei::step_shape(atoll(a[1]), atoll(a[2]), c); '
                                                      'std::printf("%d %d", s.splits, s.warps);')
     for units in (1, 4, 8, 40, 149, 296, 512):
         for tokens in (0, 1, 31, 300, 5000, 200000):
             splits, warps = choose(units, tokens)
             assert splits in (1, 2, 4, 8, 16) and warps in (4, 8)
-            assert splits == 1 or (units * splits <= 148 and (tokens + 31) // 32 > splits // 2 * 8)
-    assert choose(8, 0) == [1, 8] and choose(512, 100000) == [1, 4] and choose(8, 200000) == [16, 8]
+            fit = (four if warps == 4 else eight)[splits.bit_length() - 1]
+            assert (splits, warps) == (1, 4) or (units <= fit and splits * warps <= max(4, (tokens + 31) // 32))
+    assert choose(8, 0) == [1, 4] and choose(512, 100000) == [1, 4] and choose(7, 200000) == [16, 8] and choose(8, 200000) == [8, 8]
 
 
 def test_span_splits(tmp_path):
