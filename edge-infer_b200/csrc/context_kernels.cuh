@@ -17,7 +17,7 @@ struct QkRopeParams {
   float epsilon;
   bool interleaved;
 };
-void launch_qk_norm_rope(const QkRopeParams& p, int multiprocessors, cudaStream_t stream);
+void launch_qk_norm_rope(const QkRopeParams& p, cudaStream_t stream);
 
 struct EvictParams {
   CacheStrides k, v;

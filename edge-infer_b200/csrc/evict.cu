@@ -1,11 +1,11 @@
 // A cache cut to a budget: per sequence and KV head the first `sinks` tokens, the last `recent` and, of the others, those with
 // the largest accumulated weight, moved in order of position into another cache.
 //
-// Selection is exact: the place-th largest score is found bit by bit (two bits of the order-preserving integer key a step,
-// three counts each), scores above it stay, of those equal to it the ones with the lowest positions. Bound: the scores once,
-// the kept rows in and out; the selection's 16 steps are a chain of block-wide counts, some microseconds however few tokens,
-// so that the blocks which share a head's rows each repeat it (from their own copy of the keys in shared memory) instead of
-// waiting for one another, and then move a part of the rows each.
+// Selection is exact: the place-th largest score is found digit by digit (11, 11 and 10 bits of the order-preserving integer key,
+// a histogram each of the keys that share the digits before), scores above it stay, of those equal to it the ones with the
+// lowest positions. Bound: the scores once, the kept rows in and out. The selection is a chain of some microseconds however few
+// tokens there are, so that the blocks which share a head's rows each repeat it (from their own copy of the keys in shared
+// memory) instead of waiting for one another, and then move a part of the rows each.
 #include "context_kernels.cuh"
 
 #include <algorithm>
@@ -18,8 +18,12 @@ constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMoves = 4;          // tokens a warp has under way
 constexpr int kCachedKeys = 40960;  // keys that a block holds itself (160 KB); further ones are made from the scores again
 
+constexpr int kBins = 2048;
+
 struct EvictShared {
-  int counts[2][kWarps][4];
+  int4 bins[kBins / 4];
+  int totals[kWarps];
+  int digit, before;
   int above[kWarps], ties[kWarps];
 };
 
@@ -28,6 +32,37 @@ __device__ __forceinline__ uint32_t key_of(float score) {
   if (score != score) return 0u;
   const uint32_t bits = __float_as_uint(score + 0.0f);
   return bits ^ ((bits >> 31) ? 0xffffffffu : 0x80000000u);
+}
+
+// The digit of the place-th largest of the histogram's keys, and how many keys have a larger one; the histogram is cleared.
+__device__ __forceinline__ int2 find_digit(EvictShared* sh, int place) {
+  static_assert(kBins == 4 * kThreads, "a thread has four bins");
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = kThreads - 1 - int(threadIdx.x);  // the largest digits first
+  const int4 bins = sh->bins[mine];
+  sh->bins[mine] = make_int4(0, 0, 0, 0);
+  const int own = bins.x + bins.y + bins.z + bins.w;
+  int sum = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int other = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += other;
+  }
+  if (lane == 31) sh->totals[warp] = sum;
+  __syncthreads();
+  int before = sum - own;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w)
+    if (w < warp) before += sh->totals[w];
+  if (before < place && place <= before + own) {
+    const int counts[4] = {bins.w, bins.z, bins.y, bins.x};
+    int digit = 4 * mine + 3;
+    for (int i = 0; i < 3 && before + counts[i] < place; ++i, --digit) before += counts[i];
+    sh->digit = digit;
+    sh->before = before;
+  }
+  __syncthreads();
+  return make_int2(sh->digit, sh->before);
 }
 
 // Block (part of the kept rows, KV head, sequence).
@@ -49,42 +84,39 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const EvictParams p, in
   } else {
     // The tokens that compete: [sinks, length - recent).
     const int from = p.sinks, to = length - p.recent;
-    for (int t = from + int(threadIdx.x); t < min(to, from + cached); t += kThreads) keys[t - from] = key_of(scores[t]);
-    __syncthreads();
     auto key_at = [&](int t) { return t - from < cached ? keys[t - from] : key_of(scores[t]); };
+    int* const bins = reinterpret_cast<int*>(sh->bins);
     const int place = p.budget - p.sinks - p.recent;  // of them stay
     uint32_t threshold = 0;                            // the place-th largest key
+    sh->bins[threadIdx.x] = make_int4(0, 0, 0, 0);
+    __syncthreads();
     if (place > 0) {
-      for (int shift = 30, step = 0; shift >= 0; shift -= 2, ++step) {
-        const uint32_t unit = 1u << shift;
-        int one = 0, two = 0, three = 0;  // keys at or above threshold + 1, 2, 3 units
-        for (int t = from + int(threadIdx.x); t < to; t += kThreads) {
-          const uint32_t key = key_at(t);
-          one += key >= threshold + unit;
-          two += key >= threshold + 2 * unit;
-          three += key >= threshold + 3 * unit;
-        }
-        one = __reduce_add_sync(0xffffffffu, one);
-        two = __reduce_add_sync(0xffffffffu, two);
-        three = __reduce_add_sync(0xffffffffu, three);
-        int(&mine)[4] = sh->counts[step & 1][warp];
-        if (lane == 0) mine[0] = one, mine[1] = two, mine[2] = three;
-        __syncthreads();
-        one = two = three = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          one += sh->counts[step & 1][w][0];
-          two += sh->counts[step & 1][w][1];
-          three += sh->counts[step & 1][w][2];
-        }
-        threshold += three >= place ? 3 * unit : two >= place ? 2 * unit : one >= place ? unit : 0u;
+#pragma unroll 4
+      for (int t = from + int(threadIdx.x); t < to; t += kThreads) {
+        const uint32_t key = key_of(scores[t]);
+        if (t - from < cached) keys[t - from] = key;
+        atomicAdd(&bins[key >> 21], 1);
       }
+      const int2 high = find_digit(sh, place);
+#pragma unroll 4
+      for (int t = from + int(threadIdx.x); t < to; t += kThreads) {
+        const uint32_t key = key_at(t);
+        if (key >> 21 == uint32_t(high.x)) atomicAdd(&bins[key >> 10 & 2047], 1);
+      }
+      const int2 middle = find_digit(sh, place - high.y);
+      const uint32_t leading = uint32_t(high.x) << 11 | uint32_t(middle.x);
+#pragma unroll 4
+      for (int t = from + int(threadIdx.x); t < to; t += kThreads) {
+        const uint32_t key = key_at(t);
+        if (key >> 10 == leading) atomicAdd(&bins[key & 1023], 1);
+      }
+      threshold = leading << 10 | uint32_t(find_digit(sh, place - high.y - middle.y).x);
     }
     // Positions: a warp takes a stretch of tokens; how many before it stay comes from the other warps' counts.
     const int span = ((to - from + kWarps - 1) / kWarps + 31) / 32 * 32;
     const int first = min(from + warp * span, to), last = min(first + span, to);
     int above = 0, ties = 0;
-    for (int t0 = first; t0 < last; t0 += 32) {
+    for (int t0 = first; t0 < last && place > 0; t0 += 32) {
       const int t = t0 + lane;
       const uint32_t key = t < last ? key_at(t) : 0u;
       above += __popc(__ballot_sync(0xffffffffu, t < last && key > threshold));
@@ -149,8 +181,11 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const EvictParams p, in
 void launch_evict(const EvictParams& p, int multiprocessors, cudaStream_t stream) {
   const int units = p.sequences * p.kv_heads;
   const int cached = std::max(0, std::min(p.capacity - p.sinks - p.recent, kCachedKeys));
-  // Parts of a head's rows: enough blocks for every SM, of 32 rows at least and 8192 at most (their list is in shared memory).
-  int parts = std::max(1, std::min((2 * multiprocessors + units - 1) / units, p.budget / 32));
+  // Parts of a head's rows: a block for every SM and, so that one block's selection hides behind others' copies, no more than
+  // some 512 rows (64 caches of 2304 tokens and 8 heads cut to 2048, parts of 2048, 1024, 512, 256, 128 rows: 196, 182, 176, 177,
+  // 214 us); 32 rows at least and 8192 at most (their list is in shared memory).
+  int parts = std::max(multiprocessors / units, p.budget / 512);
+  parts = std::max(1, std::min(parts, p.budget / 32));
   parts = std::max(parts, (p.budget + 8191) / 8192);
   const int part_rows = (p.budget + parts - 1) / parts;
   const size_t shared = sizeof(EvictShared) + size_t(part_rows) * 4 + size_t(cached) * 4;

@@ -8,8 +8,8 @@
 // Bound by the bytes of q and k, in and out. A thread owns 16 values of a head as two 16-byte vectors, chosen so that both
 // members of every pair are its own: vectors j and j + rotary / 16 of the rotated part (whole neighbours' pairs lie in any
 // vector), two adjacent ones of the rest. So a head is width / 16 lanes, the norm a few shuffles, and nothing passes through
-// shared memory. A thread takes the same place of several heads of a row: the table's 64 bytes for it are read once, and
-// its loads of kHeads heads are under way together.
+// shared memory. A thread takes the same place of kHeads heads of a row, whose loads are under way together, ahead of the position
+// and the table's 64 bytes for that place.
 #include "context_kernels.cuh"
 
 #include <algorithm>
@@ -18,7 +18,7 @@ namespace ei {
 namespace {
 
 constexpr int kHeads = 2;  // heads a thread has under way
-constexpr int kThreads = 128;
+constexpr int kMostThreads = 512;
 
 __device__ __forceinline__ void unpack(const uint4& v, float* x) {
   x[0] = bf16_lo(v.x), x[1] = bf16_hi(v.x), x[2] = bf16_lo(v.y), x[3] = bf16_hi(v.y);
@@ -30,17 +30,28 @@ __device__ __forceinline__ uint4 pack(const float* x) {
 
 // Block (row, chunk of heads); `lanes` (a power of two >= width / 16) threads a head.
 template <bool kInterleaved>
-__global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const QkRopeParams p, int lanes, int heads_per_block) {
+__global__ void __launch_bounds__(kMostThreads) qk_norm_rope_kernel(const QkRopeParams p, int lanes) {
   const int row = blockIdx.x;
-  const int slot = threadIdx.x / lanes, slots = kThreads / lanes, j = threadIdx.x & (lanes - 1);
+  const int slot = threadIdx.x / lanes, slots = blockDim.x / lanes, j = threadIdx.x & (lanes - 1);
   const bool active = j < p.width / 16;
   const int pairs = p.rotary / 16;  // threads of a head that rotate
   const bool turns = j < pairs;
   const int first = (turns ? j : p.rotary / 8 + 2 * (j - pairs)) * 8;
   const int second = turns ? first + pairs * 8 : first + 8;
-  const int all = p.heads + p.kv_heads;
-  const int begin = blockIdx.y * heads_per_block, stop = min(begin + heads_per_block, all);
+  const int stop = p.heads + p.kv_heads, head0 = blockIdx.y * slots * kHeads;
 
+  uint4 held[kHeads][2];
+#pragma unroll
+  for (int u = 0; u < kHeads; ++u) {
+    const int head = head0 + u * slots + slot;
+    held[u][0] = held[u][1] = make_uint4(0, 0, 0, 0);
+    if (active && head < stop) {
+      const bf16* from = head < p.heads ? p.q + row * p.q_row + size_t(head) * p.width
+                                        : p.k + row * p.k_row + size_t(head - p.heads) * p.width;
+      held[u][0] = *reinterpret_cast<const uint4*>(from + first);
+      held[u][1] = *reinterpret_cast<const uint4*>(from + second);
+    }
+  }
   const long long position = p.positions ? p.positions[row] : (long long)p.offset + row;
   const bool known = position >= 0 && position < p.table_rows;
   float turn[16];  // (sine, cosine) of the thread's eight pairs
@@ -56,70 +67,57 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const QkRopePara
       turn[4 * i] = v.x, turn[4 * i + 1] = v.y, turn[4 * i + 2] = v.z, turn[4 * i + 3] = v.w;
     }
   }
-  for (int head0 = begin; head0 < stop; head0 += slots * kHeads) {  // block-uniform: the shuffles below need whole warps
-    uint4 held[kHeads][2];
 #pragma unroll
-    for (int u = 0; u < kHeads; ++u) {
-      const int head = head0 + u * slots + slot;
-      held[u][0] = held[u][1] = make_uint4(0, 0, 0, 0);
-      if (active && head < stop) {
-        const bf16* from = head < p.heads ? p.q + row * p.q_row + size_t(head) * p.width
-                                          : p.k + row * p.k_row + size_t(head - p.heads) * p.width;
-        held[u][0] = *reinterpret_cast<const uint4*>(from + first);
-        held[u][1] = *reinterpret_cast<const uint4*>(from + second);
+  for (int u = 0; u < kHeads; ++u) {
+    const int head = head0 + u * slots + slot;
+    float x[16];
+    unpack(held[u][0], x);
+    unpack(held[u][1], x + 8);
+    const bf16* weight = head < p.heads ? p.q_weight : p.k_weight;
+    float squares = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) squares = fmaf(x[i], x[i], squares);
+    for (int o = lanes >> 1; o > 0; o >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, o);
+    if (!active || head >= stop) continue;
+    if (weight) {
+      const float inverse = rsqrtf(squares / float(p.width) + p.epsilon);
+      float w[16];
+      unpack(__ldg(reinterpret_cast<const uint4*>(weight + first)), w);
+      unpack(__ldg(reinterpret_cast<const uint4*>(weight + second)), w + 8);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] *= inverse * w[i];
+    }
+    if (turns) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int a = kInterleaved ? 2 * i : i, b = kInterleaved ? 2 * i + 1 : i + 8;
+        const float sine = turn[2 * i], cosine = turn[2 * i + 1], xa = x[a], xb = x[b];
+        x[a] = xa * cosine - xb * sine;
+        x[b] = xa * sine + xb * cosine;
       }
     }
+    if (!known) {
 #pragma unroll
-    for (int u = 0; u < kHeads; ++u) {
-      const int head = head0 + u * slots + slot;
-      float x[16];
-      unpack(held[u][0], x);
-      unpack(held[u][1], x + 8);
-      const bf16* weight = head < p.heads ? p.q_weight : p.k_weight;
-      float squares = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) squares = fmaf(x[i], x[i], squares);
-      for (int o = lanes >> 1; o > 0; o >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, o);
-      if (!active || head >= stop) continue;
-      if (weight) {
-        const float inverse = rsqrtf(squares / float(p.width) + p.epsilon);
-        float w[16];
-        unpack(__ldg(reinterpret_cast<const uint4*>(weight + first)), w);
-        unpack(__ldg(reinterpret_cast<const uint4*>(weight + second)), w + 8);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] *= inverse * w[i];
-      }
-      if (turns) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int a = kInterleaved ? 2 * i : i, b = kInterleaved ? 2 * i + 1 : i + 8;
-          const float sine = turn[2 * i], cosine = turn[2 * i + 1], xa = x[a], xb = x[b];
-          x[a] = xa * cosine - xb * sine;
-          x[b] = xa * sine + xb * cosine;
-        }
-      }
-      if (!known) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = 0.0f;
-      }
-      bf16* to = head < p.heads ? p.q_out + row * p.q_out_row + size_t(head) * p.width
-                                : p.k_out + row * p.k_out_row + size_t(head - p.heads) * p.width;
-      *reinterpret_cast<uint4*>(to + first) = pack(x);
-      *reinterpret_cast<uint4*>(to + second) = pack(x + 8);
+      for (int i = 0; i < 16; ++i) x[i] = 0.0f;
     }
+    bf16* to = head < p.heads ? p.q_out + row * p.q_out_row + size_t(head) * p.width
+                              : p.k_out + row * p.k_out_row + size_t(head - p.heads) * p.width;
+    *reinterpret_cast<uint4*>(to + first) = pack(x);
+    *reinterpret_cast<uint4*>(to + second) = pack(x + 8);
   }
 }
 
 }  // namespace
 
-void launch_qk_norm_rope(const QkRopeParams& p, int multiprocessors, cudaStream_t stream) {
+void launch_qk_norm_rope(const QkRopeParams& p, cudaStream_t stream) {
   int lanes = 1;
   while (lanes < p.width / 16) lanes *= 2;
-  const int slots = kThreads / lanes, all = p.heads + p.kv_heads;
-  // A block takes all heads of a row where the rows fill the chip, else as few as keep its threads busy once.
-  const int chunk = p.rows >= 4 * multiprocessors ? all : slots;
+  // A row's heads make a block where they can.
+  const int all = p.heads + p.kv_heads;
+  const int threads = std::min(kMostThreads, ((all + kHeads - 1) / kHeads * lanes + 31) / 32 * 32);
+  const int chunk = threads / lanes * kHeads;
   const dim3 grid(unsigned(p.rows), unsigned((all + chunk - 1) / chunk));
-  launch(p.interleaved ? qk_norm_rope_kernel<true> : qk_norm_rope_kernel<false>, grid, dim3(kThreads), 0, stream, false, p, lanes, chunk);
+  launch(p.interleaved ? qk_norm_rope_kernel<true> : qk_norm_rope_kernel<false>, grid, dim3(unsigned(threads)), 0, stream, false, p, lanes);
 }
 
 }  // namespace ei
