@@ -254,3 +254,13 @@ def test_python_mirror_refuses_what_pointers_do_not_show(package):
         ops.attention_window(ctx, half.bfloat16(), whole.bfloat16(), whole.bfloat16(), half.bfloat16(), 4)
     with pytest.raises(ValueError, match="is on cpu"):
         ops.qk_norm_rope(ctx, half.bfloat16(), half.bfloat16(), torch.zeros(4, 128), half.bfloat16(), half.bfloat16())
+    ctx.device = -1  # what tensors of the CPU call theirs
+    with pytest.raises(ValueError, match="torch.bfloat16"):
+        ops.attention_window(ctx, half, whole.bfloat16(), whole.bfloat16(), half.bfloat16(), 4)
+    with pytest.raises(ValueError, match="4 axes"):
+        ops.attention_window(ctx, half.bfloat16(), half.bfloat16(), whole.bfloat16(), half.bfloat16(), 4)
+    with pytest.raises(ValueError, match="lengths must"):
+        ops.attention_window(ctx, half.bfloat16(), whole.bfloat16(), whole.bfloat16(), half.bfloat16(), 4, lengths=torch.zeros(1))
+    with pytest.raises(ValueError, match="1 packed values"):
+        ops.attention_window(ctx, half.bfloat16(), whole.bfloat16(), whole.bfloat16(), half.bfloat16(), 4,
+                             lengths=torch.zeros(2, dtype=torch.int32))
