@@ -36,26 +36,29 @@ constexpr int kHalfBytes = kSpanTile * 128;  // 64 values of a tile's tokens
 constexpr int kBufferBytes = 2 * kHalfBytes;
 constexpr int kBoxBytes = kSpanBox * 128;
 constexpr int kBoxes = kSpanTile / kSpanBox;
-constexpr int kBuffers = 8;
+constexpr int kStages = 4;  // each a tile's V and the K that the half's next scores are made of
+constexpr int kStageBytes = 2 * kBufferBytes;
 constexpr int kQueryBytes = 2 * kSpanRows * 128;
 constexpr float kSlack = 8.0f;  // powers of two
-constexpr size_t kStateBytes = 4096;
-constexpr size_t kSpanSharedBytes = size_t(2) * kQueryBytes + size_t(kBuffers) * kBufferBytes + 1024 + kStateBytes;
+constexpr size_t kStateBytes = 1664;
+// Queries, first K of each half, ring, state.
+constexpr size_t kSpanSharedBytes = size_t(2) * kQueryBytes + 2 * kBufferBytes + size_t(kStages) * kStageBytes + 1024 + kStateBytes;
 static_assert(kSpanSharedBytes <= 227 * 1024, "a block's buffers fit an SM");
 
 struct SpanShared {
-  uint64_t full[kBuffers], empty[kBuffers];  // K and V tiles in turn
-  uint64_t queries[2];                       // a query tile is in shared memory
-  uint64_t scores[2][2], weights[2][2];      // [half][place]: S computed, P written
-  uint64_t added[2][2];                      // [half][tile & 1]: O holds the tile's product
-  uint64_t decided[2][4][2];                 // [half][warp of four][tile & 1]: what the tile's weights are relative to
-  uint64_t pairs[2][4];                      // both warps of 32 rows have left their sums
-  uint64_t done;                             // every MMA issued has completed
+  uint64_t full[kStages], empty[kStages];
+  uint64_t first;                     // the first K
+  uint64_t queries[2];                // a query tile is in shared memory
+  uint64_t scores[2][2];              // [half][tile & 1]: S computed, and the product of the tile before the last one added
+  uint64_t weights[2][2];             // [half][tile & 1]: P written
+  uint64_t decided[2][4][2];          // [half][warp of four][tile & 1]: what the tile's weights are relative to
+  uint64_t finished[2];               // of a half: all products added
+  uint64_t pairs[2][4];               // both warps of 32 rows have left their sums
+  uint64_t done;                      // every MMA issued has completed
   uint32_t tmem_base;
   volatile int abort;
-  float reference[2][kSpanRows];  // [half][row]: the running maximum that weights are relative to
-  float sums[2][2][kSpanRows];    // [half][turn][row]
-  int issued, query_tiles;  // items, and a bit for each query tile, whose copies were requested
+  float reference[2][kSpanRows];      // [half][row]: the running maximum that weights are relative to
+  int issued, query_tiles;            // stages, and a bit for each query tile, whose copies were requested
 };
 static_assert(sizeof(SpanShared) <= kStateBytes, "the block's state lies behind the ring");
 
@@ -86,8 +89,10 @@ __device__ __forceinline__ void tmem_loaded32(uint32_t* r) {
 __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __grid_constant__ SpanAttentionParams p) {
   extern __shared__ unsigned char span_smem_raw[];
   unsigned char* const smem = span_smem_raw + ((1024u - (smem_address(span_smem_raw) & 1023u)) & 1023u);
-  unsigned char* const ring = smem + 2 * kQueryBytes;
-  SpanShared* const sh = reinterpret_cast<SpanShared*>(ring + kBuffers * kBufferBytes);
+  unsigned char* const first_keys = smem + 2 * kQueryBytes;
+  unsigned char* const ring = first_keys + 2 * kBufferBytes;
+  SpanShared* const sh = reinterpret_cast<SpanShared*>(ring + kStages * kStageBytes);
+
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kv_head = blockIdx.x, sequence = blockIdx.z;
   const int group = p.heads / p.kv_heads, stacked = p.rows * group;
@@ -150,21 +155,21 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
   auto item_of = [&](int half, int t) { return shared_tokens ? t : 2 * t + half; };
 
   if (threadIdx.x == 0) {
-    for (int b = 0; b < kBuffers; ++b) {
+    for (int b = 0; b < kStages; ++b) {
       mbarrier_init(&sh->full[b], 1);
       mbarrier_init(&sh->empty[b], shared_tokens ? 2 : 1);
     }
+    mbarrier_init(&sh->first, 1);
     for (int i = 0; i < 2; ++i) {
       mbarrier_init(&sh->queries[i], p.copied_queries ? 1 : 4);
+      mbarrier_init(&sh->finished[i], 1);
       for (int place = 0; place < 2; ++place) {
         mbarrier_init(&sh->scores[i][place], 1);
         mbarrier_init(&sh->weights[i][place], 4);
-        mbarrier_init(&sh->added[i][place], 1);
         for (int w = 0; w < 4; ++w) mbarrier_init(&sh->decided[i][w][place], 1);
       }
-    }
-    for (int i = 0; i < 2; ++i)
       for (int w = 0; w < 4; ++w) mbarrier_init(&sh->pairs[i][w], 2);
+    }
     mbarrier_init(&sh->done, 2);
     sh->abort = 0;
     sh->issued = sh->query_tiles = 0;
@@ -185,6 +190,11 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
     }
     sh->abort = 1;
     return false;
+  };
+  // The same for a whole warp.
+  auto wait_all = [&](uint64_t* bar, uint32_t parity) {
+    if (__all_sync(0xffffffffu, mbarrier_test_wait(bar, parity))) return true;
+    return __all_sync(0xffffffffu, wait(bar, parity)) != 0;
   };
   auto query_tile_of = [&](int half) { return shared_tokens ? first_tile + half : first_tile; };
   const long long row0 = (long long)sequence * p.rows;
@@ -216,6 +226,9 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
       __syncwarp();
       if (lane == 0) mbarrier_arrive(&sh->queries[half]);
     }
+    // [turn][row], over queries that are done with: the half's own, or those that a single query tile leaves out.
+    float(*const sums)[kSpanRows] =
+        reinterpret_cast<float(*)[kSpanRows]>(smem + (shared_tokens ? half * kQueryBytes : kQueryBytes + half * int(2 * kSpanRows * sizeof(float))));
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
     const uint32_t places = tmem + lanes + half * 256, outputs = places + 128;
     const int last = p.together ? length - 1 : base + row;
@@ -232,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
       const int item = item_of(half, t), box0 = box_begin + item * kBoxes;
       const bool clean = box0 >= clean_begin && box0 + kBoxes <= clean_end;
       const uint32_t at = places + (t & 1) * 64;
-      ok = __all_sync(0xffffffffu, wait(&sh->scores[half][t & 1], (t >> 1) & 1));
+      ok = wait_all(&sh->scores[half][t & 1], (t >> 1) & 1);
       if (!ok) break;
       tcgen05_fence_after();
       uint32_t s[32];
@@ -267,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
         top = fmaxf(top, largest());
         // The reference as the other warp of these rows left it with the tile before.
         if (t > 0) {
-          ok = __all_sync(0xffffffffu, wait(&sh->decided[half][warp & 3][(t - 1) & 1], ((t - 1) >> 1) & 1));
+          ok = wait_all(&sh->decided[half][warp & 3][(t - 1) & 1], ((t - 1) >> 1) & 1);
           if (!ok) break;
         }
         const float previous = sh->reference[half][row_of_tile];
@@ -287,10 +300,9 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
       if (!clean) {
         // V's rows that are no token of the list are cleared: nothing there may pass through a zero weight. (Both halves'
         // warps do it before they hand over their weights, with the same zeros.)
-        const int v_item = 2 * item + 1;
-        ok = __all_sync(0xffffffffu, wait(&sh->full[v_item % kBuffers], (v_item / kBuffers) & 1));
+        ok = wait_all(&sh->full[item % kStages], (item / kStages) & 1);
         if (!ok) break;
-        unsigned char* values = ring + (v_item % kBuffers) * kBufferBytes;
+        unsigned char* values = ring + (item % kStages) * kStageBytes;
 #pragma unroll 1
         for (int b = 0; b < kBoxes; ++b) {
           const int have = min(kSpanBox, max(0, stop_of(box0 + b) - start_of(box0 + b)));
@@ -342,8 +354,8 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
         sum += total.x + total.y;
       }
       if (moved_some) {
-        // Scores of this tile were asked for behind the product of the last but one: only the last one's may be missing.
-        ok = t == 0 || __all_sync(0xffffffffu, wait(&sh->added[half][(t - 1) & 1], ((t - 1) >> 1) & 1));
+        // The product of the tile before is added when the scores of the next one stand (or would, behind the last).
+        ok = t == 0 || wait_all(&sh->scores[half][(t + 1) & 1], ((t + 1) >> 1) & 1);
         if (!ok) break;
         if (t > 0) {
           tcgen05_fence_after();
@@ -364,21 +376,19 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
       if (lane == 0) mbarrier_arrive(&sh->weights[half][t & 1]);
     }
     const bool any = tiles > 0;
-    // The last product but one, whose phase might else be taken for the last one's, then the last.
-    if (tiles > 1) ok = ok && __all_sync(0xffffffffu, wait(&sh->added[half][tiles & 1], ((tiles - 2) >> 1) & 1));
-    if (any) ok = ok && __all_sync(0xffffffffu, wait(&sh->added[half][(tiles - 1) & 1], ((tiles - 1) >> 1) & 1));
+    if (any) ok = ok && wait_all(&sh->finished[half], 0);
     if (any && some_live && ((tiles - 1) & 1) != turn)
-      ok = ok && __all_sync(0xffffffffu, wait(&sh->decided[half][warp & 3][(tiles - 1) & 1], ((tiles - 1) >> 1) & 1));
+      ok = ok && wait_all(&sh->decided[half][warp & 3][(tiles - 1) & 1], ((tiles - 1) >> 1) & 1);
     if (any && some_live && ok) {
       // The row's sum is that of both its threads, relative to the final reference.
       const float reference = sh->reference[half][row_of_tile];
       if (maximum != reference) sum = maximum == -INFINITY ? 0.0f : sum * power_of_two((maximum - reference) * exponent_scale);
       maximum = reference;
-      sh->sums[half][turn][row_of_tile] = sum;
+      sums[turn][row_of_tile] = sum;
       __syncwarp();
       if (lane == 0) mbarrier_arrive(&sh->pairs[half][warp & 3]);
-      ok = __all_sync(0xffffffffu, wait(&sh->pairs[half][warp & 3], 0));
-      sum = sh->sums[half][0][row_of_tile] + sh->sums[half][1][row_of_tile];
+      ok = wait_all(&sh->pairs[half][warp & 3], 0);
+      sum = sums[0][row_of_tile] + sums[1][row_of_tile];
     }
     if (ok) {
       tcgen05_fence_after();
@@ -426,18 +436,25 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
                         kv_head, &sh->queries[i]);
           sh->query_tiles |= 1 << i;
         }
-      const int most = shared_tokens ? max(tiles0, tiles1) : items;
-      for (int i = 0; i < 2 * most; ++i) {
-        const int b = i % kBuffers;
-        if (i >= kBuffers && !wait(&sh->empty[b], (i / kBuffers - 1) & 1)) break;
-        const int box0 = box_begin + (i >> 1) * kBoxes, boxes = min(kBoxes, box_end - box0);
-        mbarrier_expect_tx(&sh->full[b], uint32_t(boxes) * 2 * kBoxBytes);
-        const CUtensorMap* map = (i & 1) ? &p.v_map : &p.k_map;
-        for (int j = 0; j < boxes; ++j)
+      const int most = shared_tokens ? max(tiles0, tiles1) : items, ahead = shared_tokens ? 1 : 2;
+      auto boxes_of = [&](int item) { return item < most ? min(kBoxes, box_end - box_begin - item * kBoxes) : 0; };
+      auto copy = [&](const CUtensorMap* map, int item, unsigned char* to, uint64_t* bar) {
+        for (int j = 0; j < boxes_of(item); ++j)
           for (int part = 0; part < 2; ++part)
-            tma_load_5d(ring + b * kBufferBytes + part * kHalfBytes + j * kBoxBytes, map, 0, start_of(box0 + j), part, kv_head, sequence,
-                        &sh->full[b]);
-        sh->issued = i + 1;
+            tma_load_5d(to + part * kHalfBytes + j * kBoxBytes, map, 0, start_of(box_begin + item * kBoxes + j), part, kv_head, sequence, bar);
+      };
+      if (most > 0) {
+        mbarrier_expect_tx(&sh->first, uint32_t(boxes_of(0) + (ahead > 1 ? boxes_of(1) : 0)) * 2 * kBoxBytes);
+        for (int i = 0; i < ahead; ++i) copy(&p.k_map, i, first_keys + i * kBufferBytes, &sh->first);
+        sh->issued = 1;
+      }
+      for (int i = 0; i < most; ++i) {
+        const int b = i % kStages;
+        if (i >= kStages && !wait(&sh->empty[b], (i / kStages - 1) & 1)) break;
+        mbarrier_expect_tx(&sh->full[b], uint32_t(boxes_of(i) + boxes_of(i + ahead)) * 2 * kBoxBytes);
+        copy(&p.v_map, i, ring + b * kStageBytes, &sh->full[b]);
+        copy(&p.k_map, i + ahead, ring + b * kStageBytes + kBufferBytes, &sh->full[b]);
+        sh->issued = i + 2;
       }
     }
   } else if (warp < 19) {
@@ -449,60 +466,53 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
     constexpr uint32_t kOutputs = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (uint32_t(kDim >> 3) << 17) | (uint32_t(kSpanRows >> 4) << 24);
     const uint32_t query_desc = umma_desc_low(smem_address(smem) + (shared_tokens ? mine : 0) * kQueryBytes);
     const uint32_t outputs = tmem + mine * 256 + 128;
-    // Every item is waited for in its turn, whoever's it is: a wait for a buffer's next item must not find the one before it
-    // still on its way.
+    // A loop of few instructions: with a barrier each for K, V and their buffers it took 1450 cycles a tile with nothing to wait
+    // for, more than the products themselves.
+    auto score = [&](const unsigned char* from, int place) {
+      const uint32_t keys = umma_desc_low(smem_address(from));
+#pragma unroll
+      for (int k = 0; k < kDim / 16; ++k)
+        umma_bf16_ss(tmem + mine * 256 + place * 64, query_desc + (k >> 2) * (kSpanRows * 128 >> 4) + (k & 3) * 2,
+                     keys + (k >> 2) * (kHalfBytes >> 4) + (k & 3) * 2, kUmmaDescHigh, kScores, k > 0 ? 1u : 0u);
+    };
     const int all = shared_tokens ? max(tiles0, tiles1) : items;
-    bool ok = n == 0 || __all_sync(0xffffffffu, wait(&sh->queries[shared_tokens ? mine : 0], 0));
-    auto is_own = [&](int i) { return shared_tokens ? i < n : (i & 1) == mine; };
-    auto own_index = [&](int i) { return shared_tokens ? i : i >> 1; };
-    auto await = [&](int item) { return __all_sync(0xffffffffu, wait(&sh->full[item % kBuffers], (item / kBuffers) & 1)); };
-    auto score = [&](int i) {
-      if (!await(2 * i)) return false;
-      if (!is_own(i)) return true;
+    bool ok = n == 0 || (wait_all(&sh->queries[shared_tokens ? mine : 0], 0) && wait_all(&sh->first, 0));
+    if (n > 0 && ok) {
       tcgen05_fence_after();
       if (leader) {
-        const int b = 2 * i % kBuffers, place = own_index(i) & 1;
-        const uint32_t keys = umma_desc_low(smem_address(ring) + b * kBufferBytes);
-#pragma unroll
-        for (int k = 0; k < kDim / 16; ++k)
-          umma_bf16_ss(tmem + mine * 256 + place * 64, query_desc + (k >> 2) * (kSpanRows * 128 >> 4) + (k & 3) * 2,
-                       keys + (k >> 2) * (kHalfBytes >> 4) + (k & 3) * 2, kUmmaDescHigh, kScores, k > 0 ? 1u : 0u);
-        tcgen05_commit(&sh->scores[mine][place]);
-        tcgen05_commit(&sh->empty[b]);
+        score(first_keys + (shared_tokens ? 0 : mine) * kBufferBytes, 0);
+        tcgen05_commit(&sh->scores[mine][0]);
       }
-      return true;
-    };
-    int ahead = 0;  // items whose scores have been asked for
-    for (int i = 0; i < all && ok; ++i) {
-      // The scores of the half's next tile, ahead of this one's product: they have a place of their own.
-      const int next = min(all, i + (shared_tokens ? 2 : is_own(i) ? 3 : 1));
-      for (; ahead < next && ok; ++ahead) {
-        // Items in order: K of an item comes before its V, and V of the ones between has been waited for by then.
-        ok = score(ahead);
-      }
-      ok = ok && await(2 * i + 1);
+    }
+    for (int i = shared_tokens ? 0 : mine, t = 0; i < all && ok; i += shared_tokens ? 1 : 2, ++t) {
+      const int b = i % kStages;
+      unsigned char* const stage = ring + b * kStageBytes;
+      ok = wait_all(&sh->full[b], (i / kStages) & 1);
       if (!ok) break;
-      const int b = (2 * i + 1) % kBuffers;
-      if (is_own(i)) {
-        const int t = own_index(i);
-        ok = __all_sync(0xffffffffu, wait(&sh->weights[mine][t & 1], (t >> 1) & 1));
-        if (!ok) break;
-        tcgen05_fence_after();
-        if (leader) {
-          // 64 values of a token are a 128-byte row; the other 64 values' rows kHalfBytes on; eight tokens 1024 bytes.
-          const uint32_t values = (((smem_address(ring) + b * kBufferBytes) & 0x3ffffu) >> 4) | (uint32_t(kHalfBytes >> 4) << 16);
+      if (t >= n) {
+        // Both halves count this stage and only the other sees it: given back when it is there, not earlier, so that an arrival
+        // cannot count for its previous tile.
+        if (leader) mbarrier_arrive(&sh->empty[b]);
+        continue;
+      }
+      tcgen05_fence_after();
+      if (leader) {
+        // The scores of the half's next tile, ahead of this one's product: they have a place of their own.
+        if (t + 1 < n) score(stage + kBufferBytes, (t + 1) & 1);
+        tcgen05_commit(&sh->scores[mine][(t + 1) & 1]);
+      }
+      ok = wait_all(&sh->weights[mine][t & 1], (t >> 1) & 1);
+      if (!ok) break;
+      tcgen05_fence_after();
+      if (leader) {
+        // 64 values of a token are a 128-byte row; the other 64 values' rows kHalfBytes on; eight tokens 1024 bytes.
+        const uint32_t values = ((smem_address(stage) & 0x3ffffu) >> 4) | (uint32_t(kHalfBytes >> 4) << 16);
 #pragma unroll
-          for (int k = 0; k < kSpanTile / 16; ++k)
-            umma_bf16_ts(outputs, tmem + mine * 256 + (t & 1) * 64 + k * 8, values + k * (16 * 128 >> 4), kUmmaDescHigh, kOutputs,
-                         k > 0 ? 1u : uint32_t(t > 0));
-          tcgen05_commit(&sh->empty[b]);
-          tcgen05_commit(&sh->added[mine][t & 1]);
-        }
-      } else if (shared_tokens && leader) {
-        // A tile that both halves count and only the other sees is given back when it is there, not earlier, so that an
-        // arrival cannot count for the buffer's previous item.
-        mbarrier_arrive(&sh->empty[2 * i % kBuffers]);
-        mbarrier_arrive(&sh->empty[b]);
+        for (int k = 0; k < kSpanTile / 16; ++k)
+          umma_bf16_ts(outputs, tmem + mine * 256 + (t & 1) * 64 + k * 8, values + k * (16 * 128 >> 4), kUmmaDescHigh, kOutputs,
+                       k > 0 ? 1u : uint32_t(t > 0));
+        tcgen05_commit(&sh->empty[b]);
+        if (t + 1 == n) tcgen05_commit(&sh->finished[mine]);
       }
     }
     if (leader) tcgen05_commit(&sh->done);
@@ -515,7 +525,8 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
       }
       for (int i = 0; i < 2; ++i)
         if (sh->query_tiles >> i & 1) mbarrier_wait(&sh->queries[i], 0);
-      for (int i = max(0, sh->issued - kBuffers); i < sh->issued; ++i) mbarrier_wait(&sh->full[i % kBuffers], (i / kBuffers) & 1);
+      if (sh->issued > 0) mbarrier_wait(&sh->first, 0);
+      for (int i = max(0, sh->issued - 1 - kStages); i < sh->issued - 1; ++i) mbarrier_wait(&sh->full[i % kStages], (i / kStages) & 1);
     }
     __syncthreads();
     if (live) {
