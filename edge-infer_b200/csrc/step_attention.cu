@@ -104,10 +104,32 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const uint32_t rank = cluster_rank(), splits = cluster_size();
   cluster_started();
+  if (threadIdx.x == 32) prefetch_map(&p.k_map), prefetch_map(&p.v_map);
   const int kv_head = blockIdx.x / splits, sequence = blockIdx.y;
   const int group = p.heads / p.kv_heads, stacked = p.rows * group;
   const int first_stacked = (p.first_group + int(blockIdx.z)) * kStepRows;
   const int have = min(kStepRows, stacked - first_stacked);  // rows of this unit
+
+  // Row i of the unit: stacked row first_stacked + i = query row * group + head of the group.
+  const long long row0 = (long long)sequence * p.rows;
+  auto row_of = [&](int i) { return (first_stacked + i) / group; };
+  auto joined_of = [&](int i) { return p.joined_counts[row0 * group + first_stacked + i < p.joined_border ? 0 : 1]; };
+  auto query_at = [&](int i) {
+    const int r = row_of(i), h = first_stacked + i - r * group;
+    return p.q + (row0 + r) * p.q_stride + size_t(kv_head * group + h) * kDim;
+  };
+  uint32_t qa[kRowTiles == 1 ? 8 : 1][4];
+  if (kRowTiles == 1) {
+    const bf16* lo = query_at(g < have ? g : 0);
+    const bf16* hi = query_at(g + 8 < have ? g + 8 : 0);
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) {
+      qa[kRowTiles == 1 ? kk : 0][0] = g < have ? *reinterpret_cast<const uint32_t*>(lo + kk * 16 + 2 * c) : 0u;
+      qa[kRowTiles == 1 ? kk : 0][1] = g + 8 < have ? *reinterpret_cast<const uint32_t*>(hi + kk * 16 + 2 * c) : 0u;
+      qa[kRowTiles == 1 ? kk : 0][2] = g < have ? *reinterpret_cast<const uint32_t*>(lo + kk * 16 + 8 + 2 * c) : 0u;
+      qa[kRowTiles == 1 ? kk : 0][3] = g + 8 < have ? *reinterpret_cast<const uint32_t*>(hi + kk * 16 + 8 + 2 * c) : 0u;
+    }
+  }
 
   int length = p.lengths ? p.lengths[sequence] : p.length;
   if (length < 0 || length > p.capacity) length = 0;
@@ -141,26 +163,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
   __syncwarp();
   if (p.partial) grid_launch_dependents();  // this kernel follows nothing early; what joins its results waits for them
 
-  // Row i of the unit: stacked row first_stacked + i = query row * group + head of the group.
-  const long long row0 = (long long)sequence * p.rows;
-  auto row_of = [&](int i) { return (first_stacked + i) / group; };
-  auto joined_of = [&](int i) { return p.joined_counts[row0 * group + first_stacked + i < p.joined_border ? 0 : 1]; };
-  auto query_at = [&](int i) {
-    const int r = row_of(i), h = first_stacked + i - r * group;
-    return p.q + (row0 + r) * p.q_stride + size_t(kv_head * group + h) * kDim;
-  };
-  uint32_t qa[kRowTiles == 1 ? 8 : 1][4];
-  if (kRowTiles == 1) {
-    const bf16* lo = query_at(g < have ? g : 0);
-    const bf16* hi = query_at(g + 8 < have ? g + 8 : 0);
-#pragma unroll
-    for (int kk = 0; kk < 8; ++kk) {
-      qa[kRowTiles == 1 ? kk : 0][0] = g < have ? *reinterpret_cast<const uint32_t*>(lo + kk * 16 + 2 * c) : 0u;
-      qa[kRowTiles == 1 ? kk : 0][1] = g + 8 < have ? *reinterpret_cast<const uint32_t*>(hi + kk * 16 + 2 * c) : 0u;
-      qa[kRowTiles == 1 ? kk : 0][2] = g < have ? *reinterpret_cast<const uint32_t*>(lo + kk * 16 + 8 + 2 * c) : 0u;
-      qa[kRowTiles == 1 ? kk : 0][3] = g + 8 < have ? *reinterpret_cast<const uint32_t*>(hi + kk * 16 + 8 + 2 * c) : 0u;
-    }
-  } else {
+  if (kRowTiles > 1) {
     for (int i = threadIdx.x; i < kStepRows * 16; i += kThreads) {
       const int row = i >> 4, chunk = i & 15;
       const uint4 v = row < have ? reinterpret_cast<const uint4*>(query_at(row))[chunk] : make_uint4(0, 0, 0, 0);

@@ -52,6 +52,9 @@ __device__ __forceinline__ bool mbarrier_wait(uint64_t* bar, uint32_t parity, ui
     if (mbarrier_try_wait(bar, parity)) return true;
   return false;
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
 // Tiled TMA loads; coordinates run from the innermost dimension outwards. x times the element size must be
 // a multiple of 16 bytes (the callers below only pass multiples of whole slices).
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
