@@ -100,6 +100,7 @@ StepAttentionParams attention_of(const ei_view3& q, const ei_view4& k, const ei_
   if (q.shape[0] % k.shape[0]) reject("query rows must be the same number for every sequence");
   const size_t rows = q.shape[0] / k.shape[0], group = q.shape[1] / k.shape[2];
   if (rows > kMostTokens / group || (rows * group + kStepRows - 1) / kStepRows > 65535) reject("too many query rows");
+  if (q.shape[0] > (size_t(1) << 31) / q.shape[1]) reject("too many query rows");
   if (!lengths && length > k.shape[1]) reject("the length exceeds the caches' capacity");
   StepAttentionParams p{};
   p.q = static_cast<const bf16*>(q.data);

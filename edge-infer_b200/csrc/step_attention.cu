@@ -35,7 +35,9 @@ struct StepShared {
   uint64_t full[kWarps][kBuffers];
   float maxima[kWarps][kStepRows], sums[kWarps][kStepRows];
   float2 blocks[kStepMaxSplits][kStepRows];  // maximum and sum of every block of the cluster; each block leaves its own everywhere
-  float factor[kStepMaxSplits][kStepRows];   // weight of each block's result in the joined one
+  long long out[kStepRows];                  // where a row's output goes
+  uint32_t slot[kStepRows];                  // its place among the partial results
+  int others[kStepRows];                     // results to be joined; -1: no row of the sequence
   float top[kStepRows], inverse[kStepRows];
 };
 constexpr size_t step_shared(int warps, int row_tiles) {
@@ -170,6 +172,16 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
       *reinterpret_cast<uint4*>(queries + query_offset(row, chunk)) = v;
     }
     __syncthreads();
+  }
+
+  constexpr int kUnitRows = kRowTiles * 16;
+  if (threadIdx.x < kUnitRows) {  // read behind the loop
+    const int i = threadIdx.x;
+    const int r = i < have ? row_of(i) : 0, h = kv_head * group + (i < have ? first_stacked + i - r * group : 0);
+    const bool real = i < have && (p.together || base + r >= 0);
+    sh->slot[i] = uint32_t((row0 + r) * p.heads + h);
+    sh->out[i] = (row0 + r) * p.out_stride + (long long)h * kDim;
+    sh->others[i] = !real ? -1 : p.joined ? joined_of(i) : 0;
   }
 
   // Rows' positions: what a row sees is t <= limit and (t >= floor or t < sinks).
@@ -360,21 +372,14 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
       }
     }
   __syncthreads();
-  constexpr int kUnitRows = kRowTiles * 16;
   const size_t slots = size_t(p.sequences) * p.rows * p.heads;
-  auto slot_of = [&](int i) {
-    const int r = row_of(i);
-    return size_t(row0 + r) * p.heads + kv_head * group + (first_stacked + i - r * group);
-  };
-  auto real = [&](int i) { return i < have && (p.together || base + row_of(i) >= 0); };
-  auto others_of = [&](int i) { return p.joined && real(i) ? joined_of(i) : 0; };
   // Results to be joined say their maximum and sum: requested by all threads at once.
   float2(*const others)[kStepRows] =
       reinterpret_cast<float2(*)[kStepRows]>(smem + 2 * kBuffers * kBuffer - kSpanMostPartials * kStepRows * sizeof(float2));
   if (p.joined) {
     for (int e = threadIdx.x; e < kSpanMostPartials * kUnitRows; e += kThreads) {
       const int j = e / kUnitRows, i = e % kUnitRows;
-      if (j < others_of(i)) others[j][i] = *reinterpret_cast<const float2*>(p.joined + (j * slots + slot_of(i)) * kStepPartial + kDim);
+      if (j < sh->others[i]) others[j][i] = *reinterpret_cast<const float2*>(p.joined + (j * slots + sh->slot[i]) * kStepPartial + kDim);
     }
   }
   cluster_wait_started();
@@ -420,27 +425,37 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
   if (splits > 1) cluster_sync();
   else __syncthreads();
 
-  // Joined over the cluster and with what other kernels left.
+  // Joined over the cluster and with what other kernels left: the common maximum, every part's factor and share of the sum
+  // (in place of its maximum and sum), the sum.
   if (threadIdx.x < kUnitRows) {
-    const int i = threadIdx.x;
-    const int count = others_of(i);
-    float top = -INFINITY, sum = 0.0f;
+    const int i = threadIdx.x, count = sh->others[i];
+    float top = -INFINITY;
     for (uint32_t r = 0; r < splits; ++r) top = fmaxf(top, sh->blocks[r][i].x);
+#pragma unroll 4
     for (int j = 0; j < count; ++j) top = fmaxf(top, others[j][i].x);
-    for (uint32_t r = 0; r < splits; ++r) {
-      const float2 part = sh->blocks[r][i];
-      const float factor = part.y == 0.0f ? 0.0f : power_of_two(part.x - top);
-      sh->factor[r][i] = factor;
-      if (part.y != 0.0f) sum += part.y * factor;
-    }
-    for (int j = 0; j < count; ++j) {
-      const float2 part = others[j][i];
-      const float factor = part.y == 0.0f ? 0.0f : power_of_two(part.x - top);
-      others[j][i].x = factor;
-      if (part.y != 0.0f) sum += part.y * factor;
-    }
     sh->top[i] = top;
-    sh->inverse[i] = !real(i) || sum == 0.0f ? 0.0f : p.partial ? sum : 1.0f / sum;
+  }
+  __syncthreads();
+  {
+    auto weigh = [&](float2& part, float top) {
+      const float factor = part.y == 0.0f ? 0.0f : power_of_two(part.x - top);  // nothing visible there counts nothing
+      part = make_float2(factor, part.y == 0.0f ? 0.0f : part.y * factor);
+    };
+    for (int e = threadIdx.x; e < kUnitRows * int(splits); e += kThreads) weigh(sh->blocks[e / kUnitRows][e % kUnitRows], sh->top[e % kUnitRows]);
+    if (p.joined)
+      for (int e = threadIdx.x; e < kSpanMostPartials * kUnitRows; e += kThreads) {
+        const int j = e / kUnitRows, i = e % kUnitRows;
+        if (j < sh->others[i]) weigh(others[j][i], sh->top[i]);
+      }
+  }
+  __syncthreads();
+  if (threadIdx.x < kUnitRows) {
+    const int i = threadIdx.x, count = sh->others[i];
+    float sum = 0.0f;
+    for (uint32_t r = 0; r < splits; ++r) sum += sh->blocks[r][i].y;
+#pragma unroll 4
+    for (int j = 0; j < count; ++j) sum += others[j][i].y;
+    sh->inverse[i] = count < 0 || sum == 0.0f ? 0.0f : p.partial ? sum : 1.0f / sum;
   }
   __syncthreads();
   {
@@ -463,18 +478,18 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
           if (r0 + u < splits) v[u] = remote_float4(own, r0 + u);
 #pragma unroll
         for (uint32_t u = 0; u < 8; ++u)
-          if (r0 + u < splits) add(v[u], sh->factor[r0 + u][i]);
+          if (r0 + u < splits) add(v[u], sh->blocks[r0 + u][i].x);
       }
-      const size_t slot = slot_of(i);
-      const int count = others_of(i);
+      const size_t slot = sh->slot[i];
+      const int count = p.joined ? sh->others[i] : 0;
 #pragma unroll 1
-      for (int j0 = 0; j0 < count; j0 += 8) {
-        float4 v[8];
+      for (int j0 = 0; j0 < count; j0 += 16) {
+        float4 v[16];
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
+        for (int u = 0; u < 16; ++u)
           if (j0 + u < count) v[u] = *reinterpret_cast<const float4*>(p.joined + ((j0 + u) * slots + slot) * kStepPartial + quad * 4);
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
+        for (int u = 0; u < 16; ++u)
           if (j0 + u < count) add(v[u], others[j0 + u][i].x);
       }
       const float inverse = sh->inverse[i];
@@ -488,36 +503,62 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
           packed.x = pack_bf16(total.x * inverse, total.y * inverse);
           packed.y = pack_bf16(total.z * inverse, total.w * inverse);
         }
-        const int r = row_of(i);
-        *reinterpret_cast<uint2*>(p.out + (row0 + r) * p.out_stride + size_t(kv_head * group + first_stacked + i - r * group) * kDim + quad * 4) =
-            packed;
+        *reinterpret_cast<uint2*>(p.out + sh->out[i] + quad * 4) = packed;
       }
     }
   }
   if (kWeights) {
-    // This block's tokens: the sum over the rows, in their order. A thread has four tokens under way.
+    // This block's tokens: the sum over the rows, in their order. A thread has four neighbours and the four a block's width on,
+    // of four rows under way: behind a saturated memory a trip to the L2 takes 2 us.
     const float* scores = p.scores ? p.scores + sequence * p.scores_sequence + kv_head * p.scores_head : nullptr;
     float* scores_out = p.scores_out + sequence * p.out_sequence + kv_head * p.out_head;
+    const bool whole = ((reinterpret_cast<uintptr_t>(scores) | reinterpret_cast<uintptr_t>(scores_out)) & 15) == 0;
     const int stop = min(last_tile * kStepTile, end);
-    for (int t0 = first_tile * kStepTile + int(threadIdx.x); t0 < stop; t0 += 4 * kThreads) {
-      float sum[4] = {}, old[4] = {};
+    for (int t0 = first_tile * kStepTile + 4 * int(threadIdx.x); t0 < stop; t0 += 8 * kThreads) {
+      float sum[8] = {}, old[8] = {};
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (scores && t0 + u * kThreads < stop) old[u] = scores[t0 + u * kThreads];
-#pragma unroll 4
-      for (int i = 0; i < have; ++i) {
-        const float inverse = sh->inverse[i], top = inverse == 0.0f ? 0.0f : sh->top[i];
-        float score[4];
+      for (int u = 0; u < 8; ++u) {
+        const int t = t0 + (u >> 2) * 4 * kThreads + (u & 3);
+        if (scores && t < stop) {
+          if (!whole) old[u] = scores[t];
+          else if ((u & 3) == 0 && t + 3 < stop) *reinterpret_cast<float4*>(old + u) = *reinterpret_cast<const float4*>(scores + t);
+          else if (t - (u & 3) + 3 >= stop) old[u] = scores[t];
+        }
+      }
+      for (int i0 = 0; i0 < have; i0 += 4) {
+        float4 score[4][2];  // whole tiles of them are there
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          score[u] = t0 + u * kThreads < stop ? raw[size_t(i) * p.raw_stride + t0 + u * kThreads] : -INFINITY;
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (inverse != 0.0f) sum[u] = fmaf(power_of_two(score[u] - top), inverse, sum[u]);
+          for (int u = 0; u < 2; ++u) {
+            const int t = t0 + u * 4 * kThreads;
+            if (i0 + i < have && t < stop) score[i][u] = *reinterpret_cast<const float4*>(raw + size_t(i0 + i) * p.raw_stride + t);
+          }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (i0 + i >= have) break;
+          const float inverse = sh->inverse[i0 + i], top = sh->top[i0 + i];
+          if (inverse == 0.0f) continue;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            sum[4 * u] = fmaf(power_of_two(score[i][u].x - top), inverse, sum[4 * u]);
+            sum[4 * u + 1] = fmaf(power_of_two(score[i][u].y - top), inverse, sum[4 * u + 1]);
+            sum[4 * u + 2] = fmaf(power_of_two(score[i][u].z - top), inverse, sum[4 * u + 2]);
+            sum[4 * u + 3] = fmaf(power_of_two(score[i][u].w - top), inverse, sum[4 * u + 3]);
+          }
+        }
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (t0 + u * kThreads < stop) scores_out[t0 + u * kThreads] = old[u] + sum[u];
+      for (int u = 0; u < 8; u += 4) {
+        const int t = t0 + (u >> 2) * 4 * kThreads;
+        if (whole && t + 3 < stop) {
+          *reinterpret_cast<float4*>(scores_out + t) = make_float4(old[u] + sum[u], old[u + 1] + sum[u + 1], old[u + 2] + sum[u + 2], old[u + 3] + sum[u + 3]);
+        } else {
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (t + x < stop) scores_out[t + x] = old[u + x] + sum[u + x];
+        }
+      }
     }
   }
   if (splits > 1) cluster_sync();  // no block leaves while another reads its shared memory
