@@ -6,7 +6,6 @@ Loading fails loudly if the library has not been built: there is no fallback pat
 from __future__ import annotations
 
 import ctypes as C
-import struct
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -231,11 +230,6 @@ def check(status: int) -> None:
 
 
 # ---- view helpers over torch tensors (device memory is torch's; nothing else of torch is used) ----
-# rank -> (from bytes, packer): a view is packed in one go; field by field it takes two microseconds instead of one.
-VIEWS = {rank: (view.from_buffer_copy, struct.Struct(f"{1 + 2 * rank}N").pack)
-         for rank, view in ((1, View1), (2, View2), (3, View3), (4, View4))}
-
-
 def view1(t) -> View1:
     if t is None:
         return View1(None, (0,), (0,))

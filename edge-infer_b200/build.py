@@ -3,13 +3,15 @@
     python edge-infer_b200/build.py            # incremental
     python edge-infer_b200/build.py --force
 
-Output: edge-infer_b200/libedge_infer_b200.so (git-ignored; it travels with the tree).
+Output: edge-infer_b200/libedge_infer_b200.so and _calls.so, the Python calls that take torch tensors apart natively (both
+git-ignored; they travel with the tree).
 """
 from __future__ import annotations
 
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -17,6 +19,7 @@ HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 OBJ = HERE / "build"
 LIB = HERE / "libedge_infer_b200.so"
+CALLS = HERE / "_calls.so"
 SOURCES = ["abi_ops.cu", "smallm_gemm.cu", "prompt_gemm.cu", "elementwise.cu", "attention.cu", "sampling.cu", "runtime.cu",
            "layered.cu", "layered_kernels.cu", "lightning.cu", "sized_attention.cu",
            "parallel_block.cu", "outer_state.cu", "latent_attention.cu", "delta_prompt.cu",
@@ -49,7 +52,8 @@ def _compile(source: str, verbose: bool) -> None:
 
 def build(force: bool = False, verbose: bool = False) -> Path:
     """Compiles every CUDA source for sm_100a and links the shared library."""
-    if not force and LIB.exists() and LIB.stat().st_mtime >= _newest_dependency():
+    newest = _newest_dependency()
+    if not force and all(p.exists() and p.stat().st_mtime >= newest for p in (LIB, CALLS)):
         return LIB
     OBJ.mkdir(exist_ok=True)
     stale = [s for s in SOURCES
@@ -62,6 +66,11 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     result = subprocess.run(link, capture_output=True, text=True)
     if result.returncode:
         raise RuntimeError(f"link failed:\n{result.stdout}\n{result.stderr}")
+    calls = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared", "-I" + sysconfig.get_paths()["include"],
+             str(CSRC / "python_calls.cpp"), "-o", str(CALLS), "-L" + str(HERE), "-ledge_infer_b200", "-Wl,-rpath,$ORIGIN"]
+    result = subprocess.run(calls, capture_output=True, text=True)
+    if result.returncode:
+        raise RuntimeError(f"compilation of the Python calls failed:\n{result.stdout}\n{result.stderr}")
     return LIB
 
 

@@ -8,7 +8,6 @@ launches on the context's stream and allocates nothing (scratch is passed in).
 from __future__ import annotations
 
 import ctypes as C
-import struct
 
 from . import abi
 
@@ -130,40 +129,19 @@ def attention_verify(ctx, q, k_capacity, v_capacity, output, device_offset, scra
 ROPE_SCALINGS = {"plain": 0, "linear": 1, "yarn": 2, "bands": 3}
 
 
-def _views(ctx, dtype: str, rank: int, *tensors):
-    """The tensors as C views; refuses what a C call would only see as pointers: another device, type or rank. One pass
-    over each tensor: a call of a dozen of them would feel more."""
-    device, make, pack = ctx.device, *abi.VIEWS[rank]
-    views = []
-    for t in tensors:
-        if t.get_device() != device:
-            raise ValueError(f"a tensor is on {t.device}, the execution context on cuda:{device}")
-        if str(t.dtype) != dtype:
-            raise ValueError(f"expected a {dtype} tensor, not {t.dtype}")
-        try:
-            views.append(make(pack(t.data_ptr(), *t.shape, *t.stride())))
-        except struct.error:
-            raise ValueError(f"expected a tensor with {rank} axes, not {t.dim()}") from None
-    return views
+_native_calls = None
 
 
-def _values(ctx, t, count: int, name: str):
-    """Address of `count` packed int32 values on the device, or None."""
-    if t is None:
-        return None
-    if t.get_device() != ctx.device or str(t.dtype) != "torch.int32":
-        raise ValueError(f"{name} must be int32 on cuda:{ctx.device}, not {t.dtype} on {t.device}")
-    if t.dim() != 1 or t.shape[0] != count or not t.is_contiguous():
-        raise ValueError(f"{name} must hold {count} packed values")
-    return t.data_ptr()
-
-
-def _device_scratch(ctx, scratch):
-    if scratch is None:
-        return None, 0
-    if scratch.get_device() != ctx.device:
-        raise ValueError(f"scratch is on {scratch.device}, the execution context on cuda:{ctx.device}")
-    return scratch.data_ptr(), scratch.numel() * scratch.element_size()
+def _native():
+    """The calls that take tensors apart natively (csrc/python_calls.cpp); fails loudly if they are not built."""
+    global _native_calls
+    if _native_calls is None:
+        import torch
+        _lib()
+        from . import _calls
+        _calls.configure(torch.bfloat16, torch.float32, torch.int32)
+        _native_calls = _calls
+    return _native_calls
 
 
 def build_rope_table_scaled(max_positions: int, rotary_dim: int, theta: float, kind: str = "plain", factor: float = 1.0,
@@ -183,21 +161,15 @@ def qk_norm_rope(ctx, q, k, table, q_out, k_out, *, positions=None, offset: int 
                  epsilon: float = 1e-6, interleaved: bool = False) -> None:
     """Norm of every query and key head (where a weight is given) and rotation of its first table.shape[1] values, in one
     pass with one rounding. positions: int32 [rows] on the device, else offset + row. Outputs may be the inputs."""
-    views = _views(ctx, "torch.bfloat16", 3, q, k, q_out, k_out)
-    weights = [abi.View1() if w is None else _views(ctx, "torch.bfloat16", 1, w)[0] for w in (q_weight, k_weight)]
-    abi.check(_lib().ei_qk_norm_rope_bf16(
-        C.byref(ctx), views[0], views[1], *_views(ctx, "torch.float32", 2, table), _values(ctx, positions, q.shape[0], "positions"),
-        offset, *weights, epsilon, int(interleaved), views[2], views[3]))
+    abi.check(_native().qk_norm_rope(C.addressof(ctx), q, k, table, q_out, k_out, positions, offset, q_weight, k_weight, epsilon,
+                                     interleaved))
 
 
 def attention_window(ctx, q, k, v, output, window: int, sinks: int = 0, *, lengths=None, length: int = 0) -> None:
     """Causal attention of [sequences * rows, heads, 128] queries over caches [sequences, capacity, kv_heads, 128]: a row at
     position p sees the tokens t <= p with t > p - window or t < sinks. lengths: int32 [sequences] on the device, the rows'
     own tokens included, else `length` for all."""
-    rows, out = _views(ctx, "torch.bfloat16", 3, q, output)
-    keys, values = _views(ctx, "torch.bfloat16", 4, k, v)
-    abi.check(_lib().ei_attention_window_bf16(C.byref(ctx), rows, keys, values, out, _values(ctx, lengths, k.shape[0], "lengths"),
-                                              length, window, sinks))
+    abi.check(_native().attention_window(C.addressof(ctx), q, k, v, output, window, sinks, lengths, length))
 
 
 def attention_shared_prefix_scratch_bytes(q_rows: int, query_heads: int, kv_heads: int, prefix_length: int) -> int:
@@ -207,11 +179,7 @@ def attention_shared_prefix_scratch_bytes(q_rows: int, query_heads: int, kv_head
 def attention_shared_prefix(ctx, q, prefix_k, prefix_v, k, v, output, scratch, *, lengths=None, length: int = 0) -> None:
     """Causal attention of sequences that share their first tokens, prefix_k / prefix_v [prefix, kv_heads, 128], read once for
     all of them; lengths and positions count each sequence's own tokens in k / v."""
-    rows, first_keys, first_values, out = _views(ctx, "torch.bfloat16", 3, q, prefix_k, prefix_v, output)
-    keys, values = _views(ctx, "torch.bfloat16", 4, k, v)
-    abi.check(_lib().ei_attention_shared_prefix_bf16(C.byref(ctx), rows, first_keys, first_values, keys, values, out,
-                                                     _values(ctx, lengths, k.shape[0], "lengths"), length,
-                                                     *_device_scratch(ctx, scratch)))
+    abi.check(_native().attention_shared_prefix(C.addressof(ctx), q, prefix_k, prefix_v, k, v, output, scratch, lengths, length))
 
 
 def attention_accumulate_scratch_bytes(sequences: int, rows: int, query_heads: int, kv_heads: int, capacity: int) -> int:
@@ -221,23 +189,15 @@ def attention_accumulate_scratch_bytes(sequences: int, rows: int, query_heads: i
 def attention_accumulate(ctx, q, k, v, output, scores, scores_out, scratch, *, lengths=None, length: int = 0) -> None:
     """Causal attention that also adds every token's softmax weights, over rows and a KV head's query heads, to scores
     (FP32 [sequences, kv_heads, capacity]; None counts as zeros) and leaves them in scores_out (which may be scores)."""
-    rows, out = _views(ctx, "torch.bfloat16", 3, q, output)
-    keys, values = _views(ctx, "torch.bfloat16", 4, k, v)
-    new, = _views(ctx, "torch.float32", 3, scores_out)
-    old = abi.View3() if scores is None else new if scores is scores_out else _views(ctx, "torch.float32", 3, scores)[0]
-    abi.check(_lib().ei_attention_accumulate_bf16(C.byref(ctx), rows, keys, values, out, _values(ctx, lengths, k.shape[0], "lengths"),
-                                                  length, old, new, *_device_scratch(ctx, scratch)))
+    abi.check(_native().attention_accumulate(C.addressof(ctx), q, k, v, output, scores, scores_out, scratch, lengths, length))
 
 
 def evict_kv(ctx, k, v, scores, k_out, v_out, scores_out, kept, lengths_out, sinks: int = 0, recent: int = 0, *, lengths=None,
              length: int = 0) -> None:
     """Cuts caches to the k_out.shape[1] tokens that are first, latest or heaviest, each KV head its own, in order of
     position; kept (int32) receives their positions, -1 behind them, lengths_out (int32) the new lengths."""
-    keys, values, kept_keys, kept_values = _views(ctx, "torch.bfloat16", 4, k, v, k_out, v_out)
-    old, new = _views(ctx, "torch.float32", 3, scores, scores_out)
-    abi.check(_lib().ei_evict_kv_bf16(
-        C.byref(ctx), keys, values, old, _values(ctx, lengths, k.shape[0], "lengths"), length, sinks, recent, kept_keys, kept_values,
-        new, *_views(ctx, "torch.int32", 3, kept), _values(ctx, lengths_out, k.shape[0], "lengths_out")))
+    abi.check(_native().evict_kv(C.addressof(ctx), k, v, scores, k_out, v_out, scores_out, kept, lengths_out, sinks, recent, lengths,
+                                 length))
 
 
 def sample_scratch_bytes(rows: int, vocabulary: int) -> int:

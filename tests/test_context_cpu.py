@@ -255,12 +255,14 @@ def test_python_mirror_refuses_what_pointers_do_not_show(package):
     with pytest.raises(ValueError, match="is on cpu"):
         ops.qk_norm_rope(ctx, half.bfloat16(), half.bfloat16(), torch.zeros(4, 128), half.bfloat16(), half.bfloat16())
     ctx.device = -1  # what tensors of the CPU call theirs
-    with pytest.raises(ValueError, match="torch.bfloat16"):
+    with pytest.raises(ValueError, match="expected a torch.bfloat16"):
         ops.attention_window(ctx, half, whole.bfloat16(), whole.bfloat16(), half.bfloat16(), 4)
     with pytest.raises(ValueError, match="4 axes"):
         ops.attention_window(ctx, half.bfloat16(), half.bfloat16(), whole.bfloat16(), half.bfloat16(), 4)
-    with pytest.raises(ValueError, match="lengths must"):
+    with pytest.raises(ValueError, match="torch.int32"):
         ops.attention_window(ctx, half.bfloat16(), whole.bfloat16(), whole.bfloat16(), half.bfloat16(), 4, lengths=torch.zeros(1))
     with pytest.raises(ValueError, match="1 packed values"):
         ops.attention_window(ctx, half.bfloat16(), whole.bfloat16(), whole.bfloat16(), half.bfloat16(), 4,
                              lengths=torch.zeros(2, dtype=torch.int32))
+    with pytest.raises(OverflowError):
+        ops.attention_window(ctx, half.bfloat16(), whole.bfloat16(), whole.bfloat16(), half.bfloat16(), -1)
