@@ -14,7 +14,7 @@ struct QkRopeParams {
   int table_rows;
   const int32_t* positions;  // per row, or null: offset + row
   int offset;
-  float epsilon;
+  float epsilon, inverse_width;
   bool interleaved;
 };
 void launch_qk_norm_rope(const QkRopeParams& p, cudaStream_t stream);

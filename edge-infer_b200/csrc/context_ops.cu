@@ -235,6 +235,7 @@ ei_status ei_qk_norm_rope_bf16(const ei_context* ctx, ei_view3 q, ei_view3 k, ei
     p.positions = positions;
     p.offset = positions ? 0 : int(offset);
     p.epsilon = epsilon;
+    p.inverse_width = 1.0f / float(width);
     p.interleaved = interleaved != 0;
     launch_qk_norm_rope(p, stream);
   });
