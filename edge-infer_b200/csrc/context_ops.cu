@@ -130,6 +130,8 @@ SpanAttentionParams span_of(const StepAttentionParams& p, const CacheStrides& ke
   s.lengths = p.lengths, s.length = p.length, s.window = p.window, s.sinks = p.sinks, s.together = p.together;
   encode_cache_map(&s.k_map, keys, size_t(p.capacity), size_t(p.kv_heads), size_t(p.sequences), kSpanBox, 1);
   encode_cache_map(&s.v_map, values, size_t(p.capacity), size_t(p.kv_heads), size_t(p.sequences), kSpanBox, 1);
+  encode_cache_map(&s.k_tile_map, keys, size_t(p.capacity), size_t(p.kv_heads), size_t(p.sequences), kSpanTile, 2);
+  encode_cache_map(&s.v_tile_map, values, size_t(p.capacity), size_t(p.kv_heads), size_t(p.sequences), kSpanTile, 2);
   return s;
 }
 size_t most_tokens(const StepAttentionParams& p) { return size_t(p.lengths ? p.capacity : p.length); }

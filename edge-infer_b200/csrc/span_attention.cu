@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
   SpanShared* const sh = reinterpret_cast<SpanShared*>(ring + kStages * kStageBytes);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 9 * 32) prefetch_map(&p.k_map), prefetch_map(&p.v_map), prefetch_map(&p.q_map);
+  if (threadIdx.x == 9 * 32) prefetch_map(&p.k_tile_map), prefetch_map(&p.v_tile_map), prefetch_map(&p.q_map);
   const int kv_head = blockIdx.x, sequence = blockIdx.z;
   const int group = p.heads / p.kv_heads, stacked = p.rows * group;
 
@@ -155,20 +155,7 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
   auto query_tile_of = [&](int half) { return shared_tokens ? first_tile + half : first_tile; };
   const long long row0 = (long long)sequence * p.rows;
   const int most = shared_tokens ? max(tiles0, tiles1) : items, ahead = shared_tokens ? 1 : 2;
-  auto boxes_of = [&](int item) { return item < most ? min(kBoxes, box_end - box_begin - item * kBoxes) : 0; };
-  auto copy = [&](const CUtensorMap* map, int item, unsigned char* to, uint64_t* bar) {
-    for (int j = 0; j < boxes_of(item); ++j)
-      for (int part = 0; part < 2; ++part)
-        tma_load_5d(to + part * kHalfBytes + j * kBoxBytes, map, 0, start_of(box_begin + item * kBoxes + j), part, kv_head, sequence, bar);
-  };
-  auto request = [&](int i) {
-    const int b = i % kStages;
-    mbarrier_expect_tx(&sh->full[b], uint32_t(boxes_of(i) + boxes_of(i + ahead)) * 2 * kBoxBytes);
-    copy(&p.v_map, i, ring + b * kStageBytes, &sh->full[b]);
-    copy(&p.k_map, i + ahead, ring + b * kStageBytes + kBufferBytes, &sh->full[b]);
-    sh->issued = i + 2;
-  };
-  if (threadIdx.x == 8 * 32) {  // the thread that copies: what there is room for travels while the block sets itself up
+  if (threadIdx.x == 8 * 32) {
     for (int b = 0; b < kStages; ++b) {
       mbarrier_init(&sh->full[b], 1);
       mbarrier_init(&sh->empty[b], shared_tokens ? 2 : 1);
@@ -186,21 +173,6 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
     sh->abort = 0;
     sh->issued = sh->query_tiles = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    if (p.copied_queries)
-      for (int i = 0; i < (shared_tokens ? 2 : 1); ++i) {
-        if ((i ? tiles1 : tiles0) == 0) continue;
-        mbarrier_expect_tx(&sh->queries[i], uint32_t(kQueryBytes));
-        for (int part = 0; part < 2; ++part)
-          tma_load_5d(smem + i * kQueryBytes + part * kSpanRows * 128, &p.q_map, 0, 0, int(row0) + query_tile_of(i) * kSpanRows / group, part,
-                      kv_head, &sh->queries[i]);
-        sh->query_tiles |= 1 << i;
-      }
-    if (most > 0) {
-      mbarrier_expect_tx(&sh->first, uint32_t(boxes_of(0) + (ahead > 1 ? boxes_of(1) : 0)) * 2 * kBoxBytes);
-      for (int i = 0; i < ahead; ++i) copy(&p.k_map, i, first_keys + i * kBufferBytes, &sh->first);
-      sh->issued = 1;
-    }
-    for (int i = 0; i < min(kStages, most); ++i) request(i);
   }
   if (warp == 11) tmem_alloc(&sh->tmem_base, 512);
   tcgen05_fence_before();
@@ -434,9 +406,39 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
   } else if (warp == 8) {
     // ---- copies ----
     if (lane == 0) {
-      for (int i = kStages; i < most; ++i) {
-        if (!wait(&sh->empty[i % kStages], (i / kStages - 1) & 1)) break;
-        request(i);
+      // A tile whose tokens are neighbours is one copy, one that begins with sinks and goes on with the window four. (Of boxes of 32
+      // tokens and half a head alone, a stage took eight, some 800 cycles to ask for.)
+      auto copy = [&](const CUtensorMap& tiles, const CUtensorMap& boxes, int item, unsigned char* to, uint64_t* bar) {
+        const int box = box_begin + item * kBoxes;
+        if (box + 1 < sink_boxes || box >= sink_boxes || box + 1 >= box_end) {
+          tma_load_5d(to, &tiles, 0, start_of(box), 0, kv_head, sequence, bar);
+        } else {
+          for (int j = 0; j < kBoxes; ++j)
+            for (int part = 0; part < 2; ++part)
+              tma_load_5d(to + part * kHalfBytes + j * kBoxBytes, &boxes, 0, start_of(box + j), part, kv_head, sequence, bar);
+        }
+      };
+      if (p.copied_queries)
+        for (int i = 0; i < (shared_tokens ? 2 : 1); ++i) {
+          if ((i ? tiles1 : tiles0) == 0) continue;
+          mbarrier_expect_tx(&sh->queries[i], uint32_t(kQueryBytes));
+          for (int part = 0; part < 2; ++part)
+            tma_load_5d(smem + i * kQueryBytes + part * kSpanRows * 128, &p.q_map, 0, 0, int(row0) + query_tile_of(i) * kSpanRows / group, part,
+                        kv_head, &sh->queries[i]);
+          sh->query_tiles |= 1 << i;
+        }
+      if (most > 0) {
+        mbarrier_expect_tx(&sh->first, uint32_t(min(ahead, most)) * kBufferBytes);
+        for (int i = 0; i < min(ahead, most); ++i) copy(p.k_tile_map, p.k_map, i, first_keys + i * kBufferBytes, &sh->first);
+        sh->issued = 1;
+      }
+      for (int i = 0; i < most; ++i) {
+        const int b = i % kStages;
+        if (i >= kStages && !wait(&sh->empty[b], (i / kStages - 1) & 1)) break;
+        mbarrier_expect_tx(&sh->full[b], uint32_t(i + ahead < most ? 2 : 1) * kBufferBytes);
+        copy(p.v_tile_map, p.v_map, i, ring + b * kStageBytes, &sh->full[b]);
+        if (i + ahead < most) copy(p.k_tile_map, p.k_map, i + ahead, ring + b * kStageBytes + kBufferBytes, &sh->full[b]);
+        sh->issued = i + 2;
       }
     }
   } else if (warp < 11) {

@@ -7,8 +7,9 @@
 namespace ei {
 
 struct SpanAttentionParams {
-  CUtensorMap k_map, v_map;  // boxes of kSpanBox tokens, half a head
-  CUtensorMap q_map;         // filled by the launch function where query tiles are boxes of the queries
+  CUtensorMap k_map, v_map;            // boxes of kSpanBox tokens, half a head
+  CUtensorMap k_tile_map, v_tile_map;  // boxes of kSpanTile tokens
+  CUtensorMap q_map;                   // filled by the launch function where query tiles are boxes of the queries
   bool copied_queries;
   const bf16* q;             // as StepAttentionParams
   long long q_stride;
