@@ -15,10 +15,9 @@ using namespace ei;
 namespace {
 
 constexpr size_t kHeadWidth = 128;
-// From so many stacked rows (rows x query heads of a KV head) on the tensor-core kernel of many rows takes over.
-constexpr size_t kSpanWindowRows = 128;
-constexpr size_t kSpanPrefixRows = 128;
-constexpr int kSpanBlocks = 148;  // that a prefix is cut into at most: the blocks that fit this chip at once
+// From so many stacked rows of a prefix (rows of all sequences x query heads of a KV head) on the tensor-core kernel of many rows
+// takes over.
+constexpr size_t kSpanPrefixRows = 64;
 constexpr size_t kMostTokens = size_t(1) << 30;  // of a cache: positions and windows stay clear of 2^31
 
 // The context's device has to be the current one: launches, tensor maps and kernel attributes go there. Asked for last, so
@@ -253,13 +252,21 @@ ei_status ei_attention_window_bf16(const ei_context* ctx, ei_view3 q, ei_view4 k
     p.window = int(std::min(window, kMostTokens));
     p.sinks = int(std::min(sinks, kMostTokens));
     expect_current_device(ctx);
-    const size_t stacked = size_t(p.rows) * (p.heads / p.kv_heads);
-    if (stacked >= kSpanWindowRows) {
-      launch_span_attention(span_of(p, keys, values), stream);
-      return;
+    const size_t group = size_t(p.heads / p.kv_heads), stacked = size_t(p.rows) * group;
+    // Whichever kernel is the faster by its estimate; the tensor-core kernel's query tile is half empty below 64 stacked rows.
+    auto seen_by = [&](size_t rows) { return std::min(most_tokens(p), size_t(p.window) + size_t(p.sinks) + rows); };
+    if (stacked >= 64) {
+      const SpanWindow span = span_window(size_t(p.sequences), size_t(p.kv_heads), stacked, seen_by((2 * kSpanRows + group - 1) / group));
+      const size_t units = size_t(p.sequences) * size_t(p.kv_heads) * size_t(p.groups);
+      if (span.microseconds < step_microseconds(units, seen_by((kStepRows + group - 1) / group))) {
+        SpanAttentionParams s = span_of(p, keys, values);
+        s.cluster = span.cluster;
+        launch_span_attention(s, stream);
+        return;
+      }
     }
     encode_maps(&p, keys, values);
-    const size_t seen = std::min(most_tokens(p), size_t(p.window) + size_t(p.sinks) + kStepRows);
+    const size_t seen = seen_by(kStepRows);
     launch_step_attention(p, seen, stream, false);
   });
 }
@@ -269,7 +276,7 @@ size_t ei_attention_shared_prefix_scratch_bytes(size_t q_rows, size_t query_head
   const size_t stacked = q_rows * (query_heads / kv_heads);
   size_t partials = 1;
   if (stacked >= kSpanPrefixRows)
-    partials = size_t(span_splits((stacked + kSpanRows - 1) / kSpanRows, prefix_length, int(kv_heads), kSpanBlocks).partials());
+    partials = size_t(span_splits((stacked + kSpanRows - 1) / kSpanRows, prefix_length, int(kv_heads)).partials());
   return partials * q_rows * query_heads * kStepPartial * sizeof(float);
 }
 
@@ -308,11 +315,12 @@ ei_status ei_attention_shared_prefix_bf16(const ei_context* ctx, ei_view3 q, ei_
       const size_t stacked = q.shape[0] * (q.shape[1] / k.shape[2]);
       if (stacked >= kSpanPrefixRows) {
         SpanAttentionParams span = span_of(first, first_keys, first_values);
-        span.splits = span_splits((stacked + kSpanRows - 1) / kSpanRows, prefix, first.kv_heads, kSpanBlocks);
+        span.splits = span_splits((stacked + kSpanRows - 1) / kSpanRows, prefix, first.kv_heads);
         span.partial = first.partial;
         own.joined_border = span.splits.pairs * 2 * kSpanRows;
         own.joined_counts[0] = span.splits.pair_splits;
-        own.joined_counts[1] = 2 * span.splits.single_splits;
+        own.joined_counts[1] = span.splits.single_splits;
+        span.cluster = span.splits.cluster;
         launch_span_attention(span, stream);
       } else {
         encode_maps(&first, first_keys, first_values);

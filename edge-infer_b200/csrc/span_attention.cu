@@ -23,6 +23,7 @@
 // (bounded), the block's rows come out as NaN and the tensor memory is freed.
 #include "span_attention.cuh"
 
+#include "cluster.cuh"
 #include "prompt_attention.cuh"
 
 #include <algorithm>
@@ -98,56 +99,61 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
   // ---- what this block does ----
   int length = p.lengths ? p.lengths[sequence] : p.length;
   if (length < 0 || length > p.capacity) length = 0;
+  const uint32_t rank = cluster_rank(), blocks = cluster_size();
+  const int y = blockIdx.y / blocks;
   int first_tile;             // query tile of half 0
   bool shared_tokens = true;  // both halves read every tile of tokens (of two query tiles); else every other (of one)
-  int partial_first = 0;      // of half 0's result among the prefix's
+  int partial_index = 0;      // of this stretch's result among the prefix's
   int box_begin = 0, low = 0, sink_end = 0, sink_boxes = 0, box_end, end;
   int first_position0, last_position0, first_position1, last_position1;  // of the halves' rows
   const int base = length - p.rows;
   if (p.together) {
-    const int y = blockIdx.y;
-    int split, splits;
-    if (y < p.splits.pairs * p.splits.pair_splits) {
-      first_tile = y / p.splits.pair_splits * 2;
-      splits = p.splits.pair_splits;
-      split = y - first_tile / 2 * splits;
-      partial_first = split;
+    int splits = p.splits.pair_splits;
+    if (y < p.splits.pairs * splits) {
+      first_tile = y / splits * 2;
+      partial_index = y - first_tile / 2 * splits;
     } else {
       first_tile = p.splits.pairs * 2;
       shared_tokens = false;
       splits = p.splits.single_splits;
-      split = y - p.splits.pairs * p.splits.pair_splits;
-      partial_first = 2 * split;
+      partial_index = y - p.splits.pairs * p.splits.pair_splits;
     }
     const int tiles = (length + kSpanTile - 1) / kSpanTile;
-    box_begin = int((long long)tiles * split / splits) * kBoxes;
+    box_begin = int((long long)tiles * partial_index / splits) * kBoxes;
     end = length;
-    box_end = min(int((long long)tiles * (split + 1) / splits) * kBoxes, (end + kSpanBox - 1) / kSpanBox);
+    box_end = min(int((long long)tiles * (partial_index + 1) / splits) * kBoxes, (end + kSpanBox - 1) / kSpanBox);
     first_position0 = first_position1 = last_position0 = last_position1 = length - 1;
   } else {
-    first_tile = (int(gridDim.y) - 1 - int(blockIdx.y)) * 2;  // the longest histories first
+    first_tile = (int(gridDim.y / blocks) - 1 - y) * 2;  // the longest histories first
+    shared_tokens = (first_tile + 1) * kSpanRows < stacked;
     auto position_of = [&](int i) { return base + min(i, stacked - 1) / group; };
     const int from = first_tile * kSpanRows;
     first_position0 = position_of(from), last_position0 = position_of(from + kSpanRows - 1);
-    first_position1 = position_of(from + kSpanRows), last_position1 = position_of(from + 2 * kSpanRows - 1);
+    first_position1 = shared_tokens ? position_of(from + kSpanRows) : first_position0;
+    last_position1 = shared_tokens ? position_of(from + 2 * kSpanRows - 1) : last_position0;
     end = max(0, last_position1 + 1);
     low = max(0, min(first_position0 - p.window + 1, end));
     sink_end = min(p.sinks, low);
     sink_boxes = (sink_end + kSpanBox - 1) / kSpanBox;
     box_end = sink_boxes + (end - low + kSpanBox - 1) / kSpanBox;
   }
-  const int items = (box_end - box_begin + kBoxes - 1) / kBoxes;  // tiles of tokens
+  {
+    // This block's share of the cluster's tiles.
+    const int tiles = (box_end - box_begin + kBoxes - 1) / kBoxes, begin = box_begin;
+    box_begin = begin + int((long long)tiles * rank / blocks) * kBoxes;
+    box_end = min(box_end, begin + int((long long)tiles * (rank + 1) / blocks) * kBoxes);
+  }
+  const int items = (max(0, box_end - box_begin) + kBoxes - 1) / kBoxes;  // tiles of tokens
   auto start_of = [&](int box) { return box < sink_boxes ? box * kSpanBox : low + (box - sink_boxes) * kSpanBox; };
   auto stop_of = [&](int box) { return box >= box_end ? 0 : box < sink_boxes ? sink_end : end; };
   // Tiles that a half takes: all up to its last row's position, or every other.
   auto tiles_of = [&](int half) {
     if (!shared_tokens) return (items + 1 - half) / 2;
-    if ((first_tile + half) * kSpanRows >= stacked) return 0;
     if (p.together) return items;
     const int position = half ? last_position1 : last_position0;
     if (position < 0) return 0;
     const int boxes = position < low ? (min(sink_end, position + 1) + kSpanBox - 1) / kSpanBox : sink_boxes + (position - low) / kSpanBox + 1;
-    return min(items, (boxes + kBoxes - 1) / kBoxes);
+    return min(items, (max(0, boxes - box_begin) + kBoxes - 1) / kBoxes);
   };
   const int tiles0 = tiles_of(0), tiles1 = tiles_of(1);
   auto item_of = [&](int half, int t) { return shared_tokens ? t : 2 * t + half; };
@@ -201,9 +207,16 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
   const bool live = warp < 8 && index < stacked;
   const int row = live ? index / group : 0, head = kv_head * group + (live ? index - row * group : 0);
   auto partial_of_row = [&] {
-    return p.partial + ((size_t(partial_first + (shared_tokens ? 0 : half)) * p.sequences * p.rows + row0 + row) * p.heads + head) * kStepPartial;
+    return p.partial + ((size_t(partial_index) * p.sequences * p.rows + row0 + row) * p.heads + head) * kStepPartial;
   };
   auto out_of_row = [&] { return p.out + (row0 + row) * p.out_stride + size_t(head) * kDim; };
+
+  // Of the row: running maximum, sum of the weights relative to it.
+  float maximum = -INFINITY, sum = 0.0f;
+  const float exponent_scale = rsqrtf(float(kDim)) * kLog2e;
+  // Results of other blocks of the cluster, or of the other half, belong to the same rows.
+  const bool join = blocks > 1 || !shared_tokens;
+  const int own_tiles = ((warp >> 2) & 1) ? tiles1 : tiles0;
 
   if (warp < 8) {
     // ---- weights: thread = query row ----
@@ -226,10 +239,8 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
     const uint32_t places = tmem + lanes + half * 256, outputs = places + 128;
     const int last = p.together ? length - 1 : base + row;
     const bool some_live = __any_sync(0xffffffffu, live);
-    const float exponent_scale = rsqrtf(float(kDim)) * kLog2e;
-    float maximum = -INFINITY, sum = 0.0f;
     const float2 scales = make_float2(exponent_scale, exponent_scale);
-    const int tiles = half ? tiles1 : tiles0;
+    const int tiles = own_tiles;
     // Boxes that every row of the half sees whole.
     const int clean_begin = sink_boxes + (max(0, (half ? last_position1 : last_position0) - p.window + 1 - low) + kSpanBox - 1) / kSpanBox;
     const int clean_end = sink_boxes + max(0, min(end, (half ? first_position1 : first_position0) + 1) - low) / kSpanBox;
@@ -355,14 +366,13 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
     }
     const bool any = tiles > 0;
     if (any) ok = ok && wait_all(&sh->finished[half], 0);
-    if (ok) {
+    if (ok && !join) {
       tcgen05_fence_after();
       float* const partial = partial_of_row();
       const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-      // Rows leave in whole lines, four at a time, by way of shared memory: queries that are done with (the half's own, or those
-      // that a single query tile leaves out). A thread that stores its own row's 16 bytes at a time touches 32 lines at once:
+      // Rows leave in whole lines, four at a time, by way of shared memory: queries of the half that are done with. A thread that stores its own row's 16 bytes at a time touches 32 lines at once:
       // 5.6 us instead of 1.5 for a block's partial results.
-      unsigned char* const staged = smem + (shared_tokens ? half * kQueryBytes : kQueryBytes + half * (kQueryBytes / 2)) + (warp & 3) * 4096;
+      unsigned char* const staged = smem + half * kQueryBytes + (warp & 3) * 4096;
       const uint64_t own_row = p.together ? reinterpret_cast<uint64_t>(partial) : reinterpret_cast<uint64_t>(out_of_row());
       const int parts = p.together ? 4 : 2;  // 128 bytes of a row each
       const uint32_t lives = __ballot_sync(0xffffffffu, live);
@@ -512,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
       for (int i = max(0, sh->issued - 1 - kStages); i < sh->issued - 1; ++i) mbarrier_wait(&sh->full[i % kStages], (i / kStages) & 1);
     }
     __syncthreads();
-    if (live) {
+    if (live && !join) {
       const uint32_t nan = 0x7fffffffu;
       float* const partial = partial_of_row();
       bf16* const out = out_of_row();
@@ -524,6 +534,65 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
     }
   }
   tcgen05_fence_after();
+  if (join) {
+    // Every row's sums, maximum and sum into shared memory (all copies and products are done with it), then a warp a row: its
+    // parts relative to their common maximum, in the order of the blocks.
+    unsigned char* const area = first_keys;  // [half][row][128] FP32, a row's 16-byte pieces turned by the row
+    float2* const stats = reinterpret_cast<float2*>(area + 2 * kSpanRows * kDim * 4);
+    const int place = half * kSpanRows + row_of_tile;
+    if (warp < 8) {
+      const uint32_t outputs = tmem + (uint32_t((warp & 3) * 32) << 16) + half * 256 + 128;
+#pragma unroll 1
+      for (int part = 0; part < 4; ++part) {
+        uint32_t v[32];
+        if (own_tiles > 0) {
+          tmem_request32(outputs + part * 32, v);
+          tmem_loaded32(v);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          *reinterpret_cast<uint4*>(area + place * (kDim * 4) + (((part * 8 + j) ^ (row_of_tile & 31)) << 4)) =
+              own_tiles > 0 ? make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]) : make_uint4(0, 0, 0, 0);
+      }
+      stats[place] = sh->abort ? make_float2(0.0f, __uint_as_float(0x7fffffffu)) : make_float2(maximum * exponent_scale, sum);
+    }
+    if (blocks > 1) cluster_sync();
+    else __syncthreads();
+    const int rows_here = shared_tokens ? 2 * kSpanRows : kSpanRows, sources = int(blocks) * (shared_tokens ? 1 : 2);
+    for (int r = int(rank) * (kThreads / 32) + warp; r < rows_here; r += int(blocks) * (kThreads / 32)) {
+      const int i = first_tile * kSpanRows + r;
+      if (i >= stacked) break;  // whole warps
+      const int source_place = [&](int source) { return shared_tokens ? r : (source & 1) * kSpanRows + r; }(lane);
+      auto block_of = [&](int source) { return uint32_t(shared_tokens ? source : source >> 1); };
+      float2 mine = make_float2(-INFINITY, 0.0f);
+      if (lane < sources) mine = remote_float2(stats + source_place, block_of(lane));
+      const float top = warp_max(mine.x);
+      const float factor = mine.y == 0.0f ? 0.0f : power_of_two(mine.x - top);  // nothing visible there counts nothing
+      const float total = warp_sum(mine.y == 0.0f ? 0.0f : mine.y * factor);
+      float4 out4 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+      for (int source = 0; source < sources; ++source) {
+        const float weight = __shfl_sync(0xffffffffu, factor, source);
+        const int from = shared_tokens ? r : (source & 1) * kSpanRows + r;
+        const float4 v = remote_float4(area + from * (kDim * 4) + ((lane ^ (r & 31)) << 4), block_of(source));
+        if (weight == 0.0f) continue;
+        out4.x = fmaf(v.x, weight, out4.x), out4.y = fmaf(v.y, weight, out4.y);
+        out4.z = fmaf(v.z, weight, out4.z), out4.w = fmaf(v.w, weight, out4.w);
+      }
+      const int to_row = i / group, to_head = kv_head * group + i - to_row * group;
+      if (p.together) {
+        float* const to = p.partial + ((size_t(partial_index) * p.sequences * p.rows + row0 + to_row) * p.heads + to_head) * kStepPartial;
+        reinterpret_cast<float4*>(to)[lane] = out4;
+        if (lane == 0) *reinterpret_cast<float2*>(to + kDim) = make_float2(top, total);
+      } else {
+        const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+        uint2 packed = make_uint2(0u, 0u);
+        if (inverse != 0.0f) packed = make_uint2(pack_bf16(out4.x * inverse, out4.y * inverse), pack_bf16(out4.z * inverse, out4.w * inverse));
+        reinterpret_cast<uint2*>(p.out + (row0 + to_row) * p.out_stride + size_t(to_head) * kDim)[lane] = packed;
+      }
+    }
+    if (blocks > 1) cluster_sync();  // no block leaves while another reads its shared memory
+  }
   if (warp == 11) {
     __syncwarp();
     tmem_dealloc(tmem, 512);
@@ -546,8 +615,19 @@ void launch_span_attention(const SpanAttentionParams& given, cudaStream_t stream
   p.copied_queries = p.q_stride < (1ll << 31) && all_rows < (1ll << 31) &&
                      encode_query_map(&p.q_map, p.q, int(all_rows), int(p.q_stride), group, p.kv_heads, kDim);
   const size_t query_tiles = (size_t(p.rows) * group + kSpanRows - 1) / kSpanRows;
-  const dim3 grid(unsigned(p.kv_heads), p.together ? unsigned(p.splits.blocks()) : unsigned((query_tiles + 1) / 2), unsigned(p.sequences));
-  launch(span_attention_kernel, grid, dim3(kThreads), kSpanSharedBytes, stream, false, p);
+  const unsigned clusters = p.together ? unsigned(p.splits.clusters()) : unsigned((query_tiles + 1) / 2);
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(unsigned(p.kv_heads), clusters * unsigned(p.cluster), unsigned(p.sequences));
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = kSpanSharedBytes;
+  config.stream = stream;
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = cluster.val.clusterDim.z = 1;
+  cluster.val.clusterDim.y = unsigned(p.cluster);
+  config.attrs = &cluster;
+  config.numAttrs = 1;
+  check_cuda(cudaLaunchKernelEx(&config, span_attention_kernel, p), "cudaLaunchKernelEx");
 }
 
 }  // namespace ei

@@ -22,6 +22,7 @@ struct SpanAttentionParams {
   // partial[splits.partials()][rows][heads][kStepPartial], not normalised.
   bool together;
   SpanSplits splits;
+  int cluster;  // blocks that share the tokens of two query tiles (of a stretch), joined through distributed shared memory
   float* partial;
 };
 void launch_span_attention(const SpanAttentionParams& p, cudaStream_t stream);

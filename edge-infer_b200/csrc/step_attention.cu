@@ -17,6 +17,7 @@
 // own. What a box brings beyond a stretch (other tokens, rows never written) is masked in the scores and cleared in V.
 #include "step_attention.cuh"
 
+#include "cluster.cuh"
 #include "span_choice.hpp"
 #include "step_choice.hpp"
 
@@ -55,46 +56,6 @@ __device__ __forceinline__ int tile_offset(int token, int chunk) {
 __device__ __forceinline__ int query_offset(int row, int chunk) {
   return (chunk >> 3) * (kStepRows * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
 }
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-// Every block of the cluster has started: only then may its shared memory be written.
-__device__ __forceinline__ void cluster_started() {
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void cluster_wait_started() {
-  __syncwarp();
-  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void cluster_sync() {
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t remote_address(const void* own, uint32_t rank) {
-  uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_address(own)), "r"(rank));
-  return a;
-}
-__device__ __forceinline__ void remote_store(const void* own, uint32_t rank, float2 v) {
-  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(remote_address(own, rank)), "f"(v.x), "f"(v.y) : "memory");
-}
-__device__ __forceinline__ float4 remote_float4(const void* own, uint32_t rank) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(remote_address(own, rank))
-               : "memory");
-  return v;
-}
-
 template <int kWarps, int kRowTiles, bool kWeights>
 __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attention_kernel(const __grid_constant__ StepAttentionParams p) {
   constexpr int kThreads = kWarps * 32;
@@ -625,7 +586,7 @@ void launch_step_attention(const StepAttentionParams& p, size_t tokens, cudaStre
   const StepCapacity& capacity = configure_step_kernels();
   const int group = p.heads / p.kv_heads;
   const bool two = size_t(p.rows) * group > 16;
-  const StepShape shape = step_shape(size_t(p.kv_heads) * p.sequences * p.groups, tokens, capacity);
+  const StepShape shape = step_shape(size_t(p.kv_heads) * p.sequences * p.groups, tokens, two, capacity);
   cudaLaunchAttribute attributes[2]{};
   cudaLaunchConfig_t config = step_config(shape, two, unsigned(p.kv_heads), unsigned(p.sequences), unsigned(p.groups), attributes);
   config.stream = stream;

@@ -22,8 +22,9 @@ struct StepCapacity {
 
 // `units` = sequences x KV heads x groups of rows, `tokens` = most tokens a unit may read: as many warps at work as there are
 // while all clusters run at once and no warp is without a tile; of equal shapes the one of fewer, larger blocks, whose clusters
-// are smaller (8 units of 30000 tokens, 16 blocks of four warps or 8 of eight: 28.7 and 26.7 us).
-inline StepShape step_shape(size_t units, size_t tokens, const StepCapacity& capacity) {
+// are smaller (8 units of 30000 tokens, 16 blocks of four warps or 8 of eight: 28.7 and 26.7 us). With more than 16 stacked rows
+// a warp's arithmetic counts, and the smaller blocks, which lie on more SMs, are ahead (16 units of 4096 tokens: 15.6 and 16.6).
+inline StepShape step_shape(size_t units, size_t tokens, bool two_row_tiles, const StepCapacity& capacity) {
   const size_t tiles = (tokens + kStepTile - 1) / kStepTile;
   StepShape best{1, 4};
   for (const int warps : {4, 8})
@@ -31,9 +32,15 @@ inline StepShape step_shape(size_t units, size_t tokens, const StepCapacity& cap
       const int splits = 1 << power;
       const int fit = (warps == 4 ? capacity.four : capacity.eight)[power];
       if (units > size_t(fit) || size_t(splits) * warps > std::max<size_t>(tiles, 4)) continue;
-      if (splits * warps >= best.splits * best.warps) best = {splits, warps};
+      const bool better = two_row_tiles ? splits * warps > best.splits * best.warps : splits * warps >= best.splits * best.warps;
+      if (better) best = {splits, warps};
     }
   return best;
+}
+
+// What the few-row kernel takes for many rows, in microseconds: 32 stacked rows times 32 tokens of a unit, all SMs at work.
+inline float step_microseconds(size_t units, size_t tokens) {
+  return 9.0f + 0.0021f * float(units) * float((tokens + kStepTile - 1) / kStepTile);
 }
 
 }  // namespace ei

@@ -75,31 +75,47 @@ def test_step_shape(tmp_path):
     """Powers of two, at most 16, all clusters at once where a unit is split at all, no warp of a split unit without a tile."""
     four, eight = [296, 148, 71, 33, 14], [148, 74, 33, 15, 7]
     choose = run_choice(tmp_path, "step_choice.hpp", f'ei::StepCapacity c{{{{{str(four)[1:-1]}}}, {{{str(eight)[1:-1]}}}}}; '
-                                                     'auto s = ei::step_shape(atoll(a[1]), atoll(a[2]), c); '
+                                                     'auto s = ei::step_shape(atoll(a[1]), atoll(a[2]), a[3][0] == 49, c); '
                                                      'std::printf("%d %d", s.splits, s.warps);')
     for units in (1, 4, 8, 40, 149, 296, 512):
         for tokens in (0, 1, 31, 300, 5000, 200000):
-            splits, warps = choose(units, tokens)
-            assert splits in (1, 2, 4, 8, 16) and warps in (4, 8)
-            fit = (four if warps == 4 else eight)[splits.bit_length() - 1]
-            assert (splits, warps) == (1, 4) or (units <= fit and splits * warps <= max(4, (tokens + 31) // 32))
-    assert choose(8, 0) == [1, 4] and choose(512, 100000) == [1, 4] and choose(7, 200000) == [16, 8] and choose(8, 200000) == [8, 8]
+            for two in (0, 1):
+                splits, warps = choose(units, tokens, two)
+                assert splits in (1, 2, 4, 8, 16) and warps in (4, 8)
+                fit = (four if warps == 4 else eight)[splits.bit_length() - 1]
+                assert (splits, warps) == (1, 4) or (units <= fit and splits * warps <= max(4, (tokens + 31) // 32))
+    assert choose(8, 0, 0) == [1, 4] and choose(512, 100000, 0) == [1, 4] and choose(7, 200000, 0) == [16, 8]
+    assert choose(8, 200000, 0) == [8, 8] and choose(8, 200000, 1) == [16, 4]
 
 
 def test_span_splits(tmp_path):
-    """Blocks fit the chip, rows have no more partial results than are joined, every stretch has tokens."""
-    choose = run_choice(tmp_path, "span_choice.hpp", 'auto s = ei::span_splits(atoll(a[1]), atoll(a[2]), atoi(a[3]), 148); '
-                                                     'std::printf("%d %d %d %d %d", s.pairs, s.pair_splits, s.single_splits, s.blocks(), '
+    """Rows have no more partial results than are joined, blocks have tokens, and where a prefix is cut all clusters run at once."""
+    choose = run_choice(tmp_path, "span_choice.hpp", 'auto s = ei::span_splits(atoll(a[1]), atoll(a[2]), atoi(a[3])); '
+                                                     'std::printf("%d %d %d %d %d", s.cluster, s.pairs, s.pair_splits, s.single_splits, '
                                                      's.partials());')
+    fit = {1: 148, 2: 74, 4: 33}
     for query_tiles in (1, 2, 3, 5, 8, 50, 400):
         for tokens in (1, 63, 64, 65, 1000, 30011, 200000):
             for kv_heads in (1, 4, 8):
-                pairs, pair_splits, single_splits, blocks, partials = choose(query_tiles, tokens, kv_heads)
+                cluster, pairs, pair_splits, single_splits, partials = choose(query_tiles, tokens, kv_heads)
                 tiles = (tokens + 63) // 64
                 assert pairs == query_tiles // 2 and (single_splits > 0) == (query_tiles % 2 == 1)
-                assert 1 <= partials <= 32 and blocks == pairs * pair_splits + single_splits
-                assert blocks * kv_heads <= 148 or (pair_splits == 1 and single_splits <= 1)
+                assert 1 <= partials <= 32 and partials == max(pair_splits if pairs else 0, single_splits)
+                assert (pairs * pair_splits + single_splits) * kv_heads <= fit[cluster] or (pair_splits == 1 and single_splits <= 1)
                 assert pair_splits <= tiles and single_splits <= tiles
+
+
+def test_span_window(tmp_path):
+    """Clusters of up to eight blocks where few blocks would leave the chip idle, none where it is full."""
+    choose = run_choice(tmp_path, "span_choice.hpp", 'auto s = ei::span_window(atoll(a[1]), atoll(a[2]), atoll(a[3]), atoll(a[4])); '
+                                                     'std::printf("%d %d", s.cluster, int(s.microseconds));')
+    assert choose(1, 8, 8192, 2200)[0] == 1
+    assert choose(1, 8, 256, 8192)[0] == 8
+    for sequences in (1, 3, 64):
+        for stacked in (64, 128, 129, 256, 5000):
+            for tokens in (1, 64, 1000, 30000):
+                cluster, time = choose(sequences, 8, stacked, tokens)
+                assert cluster in (1, 2, 4, 8) and time > 0
 
 
 # ---- refusals: addresses are never looked at ------------------------------------------------------------------------------
