@@ -15,9 +15,8 @@ using namespace ei;
 namespace {
 
 constexpr size_t kHeadWidth = 128;
-// From so many stacked rows of a prefix (rows of all sequences x query heads of a KV head) on the tensor-core kernel of many rows
-// takes over.
-constexpr size_t kSpanPrefixRows = 64;
+// Up to so many stacked rows (rows x query heads of a KV head) the few-row kernel is bound by the bytes alone.
+constexpr size_t kFewRows = 16;
 constexpr size_t kMostTokens = size_t(1) << 30;  // of a cache: positions and windows stay clear of 2^31
 
 // The context's device has to be the current one: launches, tensor maps and kernel attributes go there. Asked for last, so
@@ -132,6 +131,12 @@ SpanAttentionParams span_of(const StepAttentionParams& p, const CacheStrides& ke
   encode_cache_map(&s.k_tile_map, keys, size_t(p.capacity), size_t(p.kv_heads), size_t(p.sequences), kSpanTile, 2);
   encode_cache_map(&s.v_tile_map, values, size_t(p.capacity), size_t(p.kv_heads), size_t(p.sequences), kSpanTile, 2);
   return s;
+}
+// Which kernel takes a prefix for all sequences' stacked rows, by its estimate, and how it cuts it.
+bool prefix_on_tensor_cores(size_t stacked, size_t prefix, size_t kv_heads, SpanSplits* splits) {
+  if (stacked <= kFewRows) return false;
+  *splits = span_splits((stacked + kSpanRows - 1) / kSpanRows, prefix, int(kv_heads));
+  return splits->microseconds < step_microseconds(kv_heads * ((stacked + kStepRows - 1) / kStepRows), prefix);
 }
 size_t most_tokens(const StepAttentionParams& p) { return size_t(p.lengths ? p.capacity : p.length); }
 
@@ -253,9 +258,9 @@ ei_status ei_attention_window_bf16(const ei_context* ctx, ei_view3 q, ei_view4 k
     p.sinks = int(std::min(sinks, kMostTokens));
     expect_current_device(ctx);
     const size_t group = size_t(p.heads / p.kv_heads), stacked = size_t(p.rows) * group;
-    // Whichever kernel is the faster by its estimate; the tensor-core kernel's query tile is half empty below 64 stacked rows.
+    // Whichever kernel is the faster by its estimate; the tensor-core kernel's query tiles have 128 rows.
     auto seen_by = [&](size_t rows) { return std::min(most_tokens(p), size_t(p.window) + size_t(p.sinks) + rows); };
-    if (stacked >= 64) {
+    if (stacked > kFewRows) {
       const SpanWindow span = span_window(size_t(p.sequences), size_t(p.kv_heads), stacked, seen_by((2 * kSpanRows + group - 1) / group));
       const size_t units = size_t(p.sequences) * size_t(p.kv_heads) * size_t(p.groups);
       if (span.microseconds < step_microseconds(units, seen_by((kStepRows + group - 1) / group))) {
@@ -273,10 +278,8 @@ ei_status ei_attention_window_bf16(const ei_context* ctx, ei_view3 q, ei_view4 k
 
 size_t ei_attention_shared_prefix_scratch_bytes(size_t q_rows, size_t query_heads, size_t kv_heads, size_t prefix_length) {
   if (!prefix_length || !kv_heads) return 0;
-  const size_t stacked = q_rows * (query_heads / kv_heads);
-  size_t partials = 1;
-  if (stacked >= kSpanPrefixRows)
-    partials = size_t(span_splits((stacked + kSpanRows - 1) / kSpanRows, prefix_length, int(kv_heads)).partials());
+  SpanSplits splits;
+  const size_t partials = prefix_on_tensor_cores(q_rows * (query_heads / kv_heads), prefix_length, kv_heads, &splits) ? size_t(splits.partials()) : 1;
   return partials * q_rows * query_heads * kStepPartial * sizeof(float);
 }
 
@@ -312,10 +315,10 @@ ei_status ei_attention_shared_prefix_bf16(const ei_context* ctx, ei_view3 q, ei_
       own.joined = first.partial;
       own.joined_border = 0;
       own.joined_counts[1] = 1;
-      const size_t stacked = q.shape[0] * (q.shape[1] / k.shape[2]);
-      if (stacked >= kSpanPrefixRows) {
+      SpanSplits splits;
+      if (prefix_on_tensor_cores(q.shape[0] * (q.shape[1] / k.shape[2]), prefix, k.shape[2], &splits)) {
         SpanAttentionParams span = span_of(first, first_keys, first_values);
-        span.splits = span_splits((stacked + kSpanRows - 1) / kSpanRows, prefix, first.kv_heads);
+        span.splits = splits;
         span.partial = first.partial;
         own.joined_border = span.splits.pairs * 2 * kSpanRows;
         own.joined_counts[0] = span.splits.pair_splits;

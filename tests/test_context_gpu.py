@@ -102,6 +102,14 @@ WINDOW_CASES = [
     ([700, 90], 700, 300, 8, 8, 257, 0, "tokens"),           # prompts, one of them padded on the left
     ([8200], 8200, 1, 8, 8, 8000, 4, "tokens"),
     ([513], 513, 513, 4, 2, 1 << 40, 0, "tokens"),           # plain causal attention
+    # Many-row kernel: clusters of eight, four, two blocks; odd last query tiles; queries that no box copies (groups of 7, 3)
+    ([4100], 4100, 16, 32, 8, 4000, 4, "tokens"),
+    ([4096], 4100, 64, 32, 8, 4096, 0, "heads"),
+    ([2000, 1999], 2000, 100, 28, 4, 1900, 33, "tokens"),
+    ([4000], 4001, 260, 12, 4, 3900, 64, "wide"),
+    ([1300, 60, 0], 1300, 700, 16, 8, 1000, 5, "tokens"),
+    ([3000], 3000, 129, 8, 8, 2900, 100, "tokens"),
+    ([2000, 1500, 900, 20], 2000, 32, 32, 8, 2000, 0, "tokens"),
 ]
 
 
@@ -246,6 +254,9 @@ PREFIX_CASES = [
     (5000, [70] * 7, 70, 16, 16, 8),
     (130, [256] * 3, 256, 250, 4, 4),                        # prompts behind a prefix
     (0, [40, 41], 41, 2, 8, 2),                              # no prefix
+    (30011, [50] * 8, 64, 9, 16, 8),                         # 144 stacked rows: a pair of query tiles
+    (9001, [33, 9, 2], 33, 40, 28, 4),                       # 840: three pairs and an odd tile
+    (8192, [12] * 16, 16, 1, 32, 8),                         # 64
 ]
 
 
