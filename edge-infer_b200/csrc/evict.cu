@@ -5,7 +5,8 @@
 // a histogram each of the keys that share the digits before), scores above it stay, of those equal to it the ones with the
 // lowest positions. Bound: the scores once, the kept rows in and out. The selection is a chain of some microseconds however few
 // tokens there are, so that the blocks which share a head's rows each repeat it (from their own copy of the keys in shared
-// memory) instead of waiting for one another, and then move a part of the rows each.
+// memory) instead of waiting for one another, and then move a part of the rows each. 64 caches of 2304 tokens and 8 heads to 2048:
+// 176 us = 6.07 TB/s; one of 8191 to 1024: 13.7 us (46 with the place-th key found two bits a step by counting all keys).
 #include "context_kernels.cuh"
 
 #include <algorithm>

@@ -9,7 +9,8 @@
 // members of every pair are its own: vectors j and j + rotary / 16 of the rotated part (whole neighbours' pairs lie in any
 // vector), two adjacent ones of the rest. So a head is width / 16 lanes, the norm a few shuffles, and nothing passes through
 // shared memory. A thread takes the same place of kHeads heads of a row, whose loads are under way together; the table's 64 bytes
-// for that place are read once for them.
+// for that place are read once for them. 2048 rows of 32 + 8 heads of 128: 12.0 us = 3.5 TB/s, two waves of blocks that each wait
+// for the position, then for the table; 64 rows: 2.4 us, a launch.
 #include "context_kernels.cuh"
 
 #include <algorithm>

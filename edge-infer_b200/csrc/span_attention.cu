@@ -1,26 +1,33 @@
 // Attention of many query rows over caches on tcgen05: prompts with a sliding window and first tokens that stay visible, and
 // the rows of all sequences over a prefix that they share.
 //
-// A block owns two query tiles of 128 stacked rows (row x query head of one KV head) and walks its tokens in tiles of 128. Per
-// tile and query tile: S = Q K^T into tensor memory, a thread per row takes its 128 scores out, makes the weights relative to
-// its running maximum and puts them back as BF16 over the scores, from where they are the A operand of O += P V (V as it stands
-// in the cache is that product's N-major B operand). While one query tile's weights are made, the tensor cores work for the
-// other: 512 columns of tensor memory are the two tiles' scores and outputs. The bound is the chain's slower side, 2 x 128 x 128
-// exponentials at 16 a cycle and four products of 128 x 128 x 128 at 8192 multiply-adds a cycle: 2048 cycles either way.
+// A block has two halves, each with a query tile of 128 stacked rows (row x query head of one KV head), and walks its tokens in
+// tiles of 64. Per tile and half: S = Q K^T into tensor memory, a thread per row takes its 64 scores out, makes the weights
+// relative to its running maximum and puts them back as BF16 over the scores, from where they are the A operand of O += P V (V
+// as it stands in the cache is that product's N-major B operand). Scores have two places, so that a tile's are computed while
+// the last one's weights are made: 2 x (64 + 64 + 128) columns are all of the tensor memory.
 //
 // A running maximum may lag the true one by 2^8 (weights up to 256 are as exact in BF16 as those up to 1), so that the
 // outputs are hardly ever taken out of tensor memory to be rescaled; the sum is of the rounded weights, so that those used
-// add up to one exactly and a row that one token dominates comes out as that token's values.
+// add up to one exactly.
 //
-// Tokens are a list of boxes of 32, first those of the sinks, then those of the window of the block's rows; four make a tile, so
-// that a few sinks do not cost a tile of their own. What a box holds beyond its stretch is masked in the scores and cleared
-// in V. A prefix is cut into stretches over the blocks (span_choice.hpp); an odd last query tile has both halves of its
-// blocks, which then take every other tile of tokens.
+// Tokens are a list of boxes of 32, first those of the sinks, then those of the window of the block's rows; two make a tile, so
+// that a few sinks cost no tile of their own. What a box holds beyond its stretch is masked in the scores and cleared in V.
+// An odd last query tile has both halves of its block, which then take every other tile of tokens. Where the blocks are
+// fewer than the SMs, those of a cluster share the tokens of the same rows and join their sums through distributed shared
+// memory; a prefix is also cut into stretches that leave partial results (span_choice.hpp).
+//
+// What bounds it: the softmax warps' own chain. A tile takes a pair of halves some 2200 cycles, of which the exponentials are
+// 1024 (16 a cycle), the products 1280; by leaving parts out in copies, everything but the softmax takes 1200. Two warps a
+// scheduler share the exponentials: alone a warp needs 820 cycles for its 64, beside the other 1200. Sixteen softmax warps, two a
+// row by columns or by turns, came out the same; so did tiles of 128 tokens with one place for the scores, whose halves fall
+// into step and then wait for their products together. 2048 rows of 32 / 8 heads behind 6144 tokens, window 2048: 97 us = 709
+// TFLOP/s (289 us by the few-row kernel); 256 blocks are 1.73 waves, which costs 13 %, and a block some 9 us to start and to leave.
 //
 // Roles of the twelve warps: 0-3 and 4-7 the weights of one half each, 8 the copies, 9 and 10 the MMAs of one half each, 11 the
-// tensor memory. K and V tiles of 16 KB go through a ring of eight buffers. Every wait is bounded: a role whose wait runs out
-// raises `abort`, which every other wait polls; when all roles have left, the copies and MMAs in flight are waited for
-// (bounded), the block's rows come out as NaN and the tensor memory is freed.
+// tensor memory. A stage of the ring of four holds a tile's V and the K of the half's next scores. Every wait is bounded: a role
+// whose wait runs out raises `abort`, which every other wait polls; when all roles have left, the copies and MMAs in flight are
+// waited for (bounded), the block's rows come out as NaN and the tensor memory is freed.
 #include "span_attention.cuh"
 
 #include "cluster.cuh"

@@ -5,13 +5,19 @@
 //
 // A unit is 32 stacked query rows (row x query head of one KV head) of one sequence; 16 where no unit has more. The path is
 // bound by the bytes of K and V, so each is fetched once per unit and every warp streams on its own: a warp walks every
-// fourth tile of 32 tokens of its block with a private ring of three 8 KB buffers filled by TMA (K and V in turn: a tile's V
-// and the next tile's K travel while the scores are made) on its own mbarriers, so that the loop has no barrier of the block
-// and no empty barriers. Two blocks of 96 KB fit on an SM: eight warps, some 128 KB under way. Scores and products are
-// mma.sync (16 rows are all that a decode step has; a tcgen05 tile would be 128), weights are rounded to BF16 for the second
-// product only and their sum is of the rounded ones, so that the weights used add up to one exactly.
+// fourth (or eighth) tile of 32 tokens of its block with a private ring of three 8 KB buffers filled by TMA (K and V in turn: a
+// tile's V and the next tile's K travel while the scores are made) on its own mbarriers, so that the loop has no barrier of the
+// block and no empty barriers. Two blocks of four warps or one of eight fit an SM, some 128 KB under way. Scores and products
+// are mma.sync (16 rows are all that a decode step has; a tcgen05 tile would be 128), weights are rounded to BF16 for the
+// second product only and their sum is of the rounded ones, so that the weights used add up to one exactly (where weights
+// are reported, in FP32, the sum is of the unrounded ones).
 // The blocks of a unit form a cluster (up to 16): they join (sums, maximum, sum) through distributed shared memory, each
-// finishing a part of the rows, so that there is no scratch, no second launch and a fixed order of every addition.
+// finishing a part of the rows, so that there is no scratch, no second launch and a fixed order of every addition. What a block
+// says of itself it writes to all blocks ahead of the cluster's barrier: read from one another behind it, block by block, that
+// took 2.7 us of a single token's 10.
+// 64 caches of 256 to 8192 tokens, window 4096, 32 / 8 heads: 128 us = 6.5 TB/s, the measured copy rate. One token over 1028 tokens
+// of one cache: 7.6 us, a chain of launch, length, first copies, tile, join; over 30000 tokens 25 us = 4.9 TB/s. With weights
+// reported, 64 caches of 2304: 101 us (84.5 without).
 //
 // Only tokens that some row of the unit sees are read: tiles start at the window's first token, sinks are a stretch of their
 // own. What a box brings beyond a stretch (other tokens, rows never written) is masked in the scores and cleared in V.

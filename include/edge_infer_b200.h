@@ -175,8 +175,11 @@ ei_status ei_attention_prefill_static_bf16(const ei_context* ctx, ei_view3 q, ei
  * position (a sequence shorter than its rows: padding on the left) comes out as zeros, and so does every row of a sequence
  * whose length lies outside 0 .. capacity, which counts as empty. Keys and values that no row of the call may see are never
  * used, whatever they hold. Scores, weights' sums and products are FP32, weights are rounded to BF16 for the product with the
- * values, outputs once. The context's device has to be the current one; device pointers must belong to it. Nothing is
- * allocated; results do not change from call to call. */
+ * values, outputs once. `out` may be the queries' own view, else it lies apart from every input. The context's device has to be
+ * the current one; device pointers must belong to it. Nothing is allocated; results do not change from call to call; scratch is
+ * used until the call's work is done, so calls that may overlap need scratch of their own. A first call on a device sets kernels
+ * up: make it before a stream capture. Should a copy not arrive within its bounded wait (some half a second), the rows that
+ * needed it come out as NaN. */
 
 /* Rotation tables for contexts longer than a model was trained on. EI_ROPE_LINEAR: every angle is divided by `factor`.
  * EI_ROPE_YARN: frequencies that turn more than `fast` times over `original_positions` stay, those below `slow` turns are

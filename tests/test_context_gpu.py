@@ -110,6 +110,7 @@ WINDOW_CASES = [
     ([1300, 60, 0], 1300, 700, 16, 8, 1000, 5, "tokens"),
     ([3000], 3000, 129, 8, 8, 2900, 100, "tokens"),
     ([2000, 1500, 900, 20], 2000, 32, 32, 8, 2000, 0, "tokens"),
+    ([2048 - 40 * i for i in range(24)], 2048, 32, 32, 8, 2048, 0, "tokens"),  # no cluster, both halves at one query tile
 ]
 
 
@@ -186,6 +187,24 @@ def test_attention_window_nan_in_sight_stays_in_its_rows(cuda, package, ctx):
     ops.attention_window(ctx, q, k, v, out, 64, 0, length=90)
     wrong = out.isnan().all(-1)
     assert wrong[1, 2] and int(wrong.sum()) == 1 and int(out.isnan().sum()) == 128
+
+
+@pytest.mark.parametrize("rows,n", [(3, 700), (300, 700)])
+def test_attention_replaces_its_queries(cuda, package, ctx, rows, n):
+    """The outputs may take the queries' place."""
+    torch, ops = cuda, package.operators
+    q, k, v = normal(torch, 1, 2 * rows, 12, 128), normal(torch, 2, 2, n, 4, 128), normal(torch, 3, 2, n, 4, 128)
+    pk, pv = normal(torch, 4, 900, 4, 128), normal(torch, 5, 900, 4, 128)
+    out = torch.empty_like(q)
+    ops.attention_window(ctx, q, k, v, out, 200, 3, length=n)
+    mine = q.clone()
+    ops.attention_window(ctx, mine, k, v, mine, 200, 3, length=n)
+    assert torch.equal(mine, out)
+    scratch = torch.empty(ops.attention_shared_prefix_scratch_bytes(2 * rows, 12, 4, 900), dtype=torch.uint8, device="cuda")
+    ops.attention_shared_prefix(ctx, q, pk, pv, k, v, out, scratch, length=n)
+    mine = q.clone()
+    ops.attention_shared_prefix(ctx, mine, pk, pv, k, v, mine, scratch, length=n)
+    assert torch.equal(mine, out)
 
 
 def test_attention_window_in_a_graph_follows_the_lengths(cuda, package):
