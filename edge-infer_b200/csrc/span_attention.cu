@@ -9,7 +9,8 @@
 //
 // A running maximum may lag the true one by 2^8 (weights up to 256 are as exact in BF16 as those up to 1), so that the
 // outputs are hardly ever taken out of tensor memory to be rescaled; the sum is of the rounded weights, so that those used
-// add up to one exactly.
+// add up to one exactly. (Outputs are 0.0021 of their size off 64 bits, 0.0019 with the true maximum, whose weight is exactly 1,
+// and 0.0017 rounded from 32-bit arithmetic; the true maximum costs 20 %.)
 //
 // Tokens are a list of boxes of 32, first those of the sinks, then those of the window of the block's rows; two make a tile, so
 // that a few sinks cost no tile of their own. What a box holds beyond its stretch is masked in the scores and cleared in V.
