@@ -475,29 +475,33 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
     }
   }
   if (kWeights) {
-    // This block's tokens: the sum over the rows, in their order. A thread has four neighbours and the four a block's width on,
-    // of four rows under way: behind a saturated memory a trip to the L2 takes 2 us.
+    // This block's tokens: the sum over the rows, in their order. A thread has kQuads times four neighbours, of four rows, under way:
+    // behind a saturated memory a trip to the L2 takes 2 us.
+    constexpr int kQuads = 4;
     const float* scores = p.scores ? p.scores + sequence * p.scores_sequence + kv_head * p.scores_head : nullptr;
     float* scores_out = p.scores_out + sequence * p.out_sequence + kv_head * p.out_head;
     const bool whole = ((reinterpret_cast<uintptr_t>(scores) | reinterpret_cast<uintptr_t>(scores_out)) & 15) == 0;
     const int stop = min(last_tile * kStepTile, end);
-    for (int t0 = first_tile * kStepTile + 4 * int(threadIdx.x); t0 < stop; t0 += 8 * kThreads) {
-      float sum[8] = {}, old[8] = {};
+    for (int t0 = first_tile * kStepTile + 4 * int(threadIdx.x); t0 < stop; t0 += 4 * kQuads * kThreads) {
+      float sum[kQuads][4] = {}, old[kQuads][4] = {};
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int t = t0 + (u >> 2) * 4 * kThreads + (u & 3);
-        if (scores && t < stop) {
-          if (!whole) old[u] = scores[t];
-          else if ((u & 3) == 0 && t + 3 < stop) *reinterpret_cast<float4*>(old + u) = *reinterpret_cast<const float4*>(scores + t);
-          else if (t - (u & 3) + 3 >= stop) old[u] = scores[t];
+      for (int u = 0; u < kQuads; ++u) {
+        const int t = t0 + u * 4 * kThreads;
+        if (!scores) continue;
+        if (whole && t + 3 < stop) {
+          *reinterpret_cast<float4*>(old[u]) = *reinterpret_cast<const float4*>(scores + t);
+        } else {
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (t + x < stop) old[u][x] = scores[t + x];
         }
       }
       for (int i0 = 0; i0 < have; i0 += 4) {
-        float4 score[4][2];  // whole tiles of them are there
+        float4 score[4][kQuads];  // whole tiles of them are there
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
+          for (int u = 0; u < kQuads; ++u) {
             const int t = t0 + u * 4 * kThreads;
             if (i0 + i < have && t < stop) score[i][u] = *reinterpret_cast<const float4*>(raw + size_t(i0 + i) * p.raw_stride + t);
           }
@@ -507,23 +511,24 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
           const float inverse = sh->inverse[i0 + i], top = sh->top[i0 + i];
           if (inverse == 0.0f) continue;
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            sum[4 * u] = fmaf(power_of_two(score[i][u].x - top), inverse, sum[4 * u]);
-            sum[4 * u + 1] = fmaf(power_of_two(score[i][u].y - top), inverse, sum[4 * u + 1]);
-            sum[4 * u + 2] = fmaf(power_of_two(score[i][u].z - top), inverse, sum[4 * u + 2]);
-            sum[4 * u + 3] = fmaf(power_of_two(score[i][u].w - top), inverse, sum[4 * u + 3]);
+          for (int u = 0; u < kQuads; ++u) {
+            sum[u][0] = fmaf(power_of_two(score[i][u].x - top), inverse, sum[u][0]);
+            sum[u][1] = fmaf(power_of_two(score[i][u].y - top), inverse, sum[u][1]);
+            sum[u][2] = fmaf(power_of_two(score[i][u].z - top), inverse, sum[u][2]);
+            sum[u][3] = fmaf(power_of_two(score[i][u].w - top), inverse, sum[u][3]);
           }
         }
       }
 #pragma unroll
-      for (int u = 0; u < 8; u += 4) {
-        const int t = t0 + (u >> 2) * 4 * kThreads;
+      for (int u = 0; u < kQuads; ++u) {
+        const int t = t0 + u * 4 * kThreads;
         if (whole && t + 3 < stop) {
-          *reinterpret_cast<float4*>(scores_out + t) = make_float4(old[u] + sum[u], old[u + 1] + sum[u + 1], old[u + 2] + sum[u + 2], old[u + 3] + sum[u + 3]);
+          *reinterpret_cast<float4*>(scores_out + t) =
+              make_float4(old[u][0] + sum[u][0], old[u][1] + sum[u][1], old[u][2] + sum[u][2], old[u][3] + sum[u][3]);
         } else {
 #pragma unroll
           for (int x = 0; x < 4; ++x)
-            if (t + x < stop) scores_out[t + x] = old[u + x] + sum[u + x];
+            if (t + x < stop) scores_out[t + x] = old[u][x] + sum[u][x];
         }
       }
     }
