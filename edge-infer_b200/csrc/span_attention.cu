@@ -52,6 +52,7 @@ constexpr float kSlack = 8.0f;  // powers of two
 constexpr size_t kStateBytes = 512;
 // Queries, first K of each half, ring, state.
 constexpr size_t kSpanSharedBytes = size_t(2) * kQueryBytes + 2 * kBufferBytes + size_t(kStages) * kStageBytes + 1024 + kStateBytes;
+static_assert(kBoxes == 2, "a tile's boxes are looked at one by one");
 static_assert(kSpanSharedBytes <= 227 * 1024, "a block's buffers fit an SM");
 
 struct SpanShared {
@@ -297,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
         if (moved) rescale = power_of_two((previous - reference) * exponent_scale);
         moved_some = __any_sync(0xffffffffu, moved);
       }
-      if (!clean) {
+      if (!clean && (stop_of(box0) - start_of(box0) < kSpanBox || stop_of(box0 + 1) - start_of(box0 + 1) < kSpanBox)) {
         // V's rows that are no token of the list are cleared: nothing there may pass through a zero weight. (Both halves'
         // warps do it before they hand over their weights, with the same zeros.)
         ok = wait_all(&sh->full[item % kStages], (item / kStages) & 1);

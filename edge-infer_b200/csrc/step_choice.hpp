@@ -38,13 +38,14 @@ inline StepShape step_shape(size_t units, size_t tokens, bool two_row_tiles, con
   return best;
 }
 
-// What the few-row kernel takes for units of more than 16 stacked rows, in microseconds: 2.1 ns for 32 rows times 32 tokens with
-// 1184 warps at work, as many as fit a B200; few units do not get as many.
+// What the few-row kernel takes for units of more than 16 stacked rows, in microseconds: 9 for a block's start and join, in as many
+// waves as there are, and 2.1 ns for 32 rows times 32 tokens with 1184 warps at work, as many as fit a B200; few units do not
+// get as many.
 inline float step_microseconds(size_t units, size_t tokens) {
   size_t warps = units > 14 ? 32 : 64;  // of a unit
   while (warps > 4 && warps * units > 1184) warps /= 2;
   const float busy = std::min(1.0f, float(warps * units) / 1184.0f);
-  return 9.0f + 0.0021f * float(units) * float((tokens + kStepTile - 1) / kStepTile) / busy;
+  return 9.0f * std::max(1.0f, float(units) / 296.0f) + 0.0021f * float(units) * float((tokens + kStepTile - 1) / kStepTile) / busy;
 }
 
 }  // namespace ei
