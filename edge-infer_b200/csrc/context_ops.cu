@@ -140,7 +140,7 @@ bool prefix_on_tensor_cores(size_t stacked, size_t prefix, size_t kv_heads, Span
 }
 size_t most_tokens(const StepAttentionParams& p) { return size_t(p.lengths ? p.capacity : p.length); }
 
-size_t raw_rows(size_t rows, size_t group) { return std::min<size_t>(kStepRows, rows * group); }
+size_t raw_rows(size_t rows, size_t group) { return std::min<size_t>(kStepWeightGroups * kStepRows, rows * group); }
 size_t raw_stride(size_t capacity) { return (capacity + kStepTile - 1) / kStepTile * kStepTile; }
 
 }  // namespace
@@ -336,7 +336,8 @@ ei_status ei_attention_shared_prefix_bf16(const ei_context* ctx, ei_view3 q, ei_
 
 size_t ei_attention_accumulate_scratch_bytes(size_t sequences, size_t rows, size_t query_heads, size_t kv_heads, size_t capacity) {
   if (!kv_heads) return 0;
-  return sequences * kv_heads * raw_rows(rows, query_heads / kv_heads) * raw_stride(capacity) * sizeof(float);
+  const size_t stored = sequences * kv_heads * raw_rows(rows, query_heads / kv_heads);
+  return stored * (raw_stride(capacity) * sizeof(float) + sizeof(float2));
 }
 
 ei_status ei_attention_accumulate_bf16(const ei_context* ctx, ei_view3 q, ei_view4 k, ei_view4 v, ei_view3 out, const int32_t* lengths,
@@ -362,11 +363,13 @@ ei_status ei_attention_accumulate_bf16(const ei_context* ctx, ei_view3 q, ei_vie
     p.scores_sequence = scores.stride[0], p.scores_head = scores.stride[1];
     p.scores_out = static_cast<float*>(scores_out.data);
     p.out_sequence = scores_out.stride[0], p.out_head = scores_out.stride[1];
-    // 32 stacked rows a launch, each adding to what the one before it left, so that the order of the additions is fixed.
+    // Up to eight groups of 32 stacked rows at a time, each time adding to what the one before left, in a fixed order.
     const int groups = p.groups;
-    p.groups = 1;
-    for (p.first_group = 0; p.first_group < groups; ++p.first_group) {
+    if (groups > 1) p.row_stats = reinterpret_cast<float2*>(p.raw + size_t(p.sequences) * p.kv_heads * p.raw_rows * p.raw_stride);
+    for (p.first_group = 0; p.first_group < groups; p.first_group += kStepWeightGroups) {
+      p.groups = std::min(kStepWeightGroups, groups - p.first_group);
       launch_step_attention(p, most_tokens(p), stream, false);
+      if (p.row_stats) launch_step_weights(p, most_tokens(p), stream);
       p.scores = p.scores_out;
       p.scores_sequence = p.out_sequence, p.scores_head = p.out_head;
     }

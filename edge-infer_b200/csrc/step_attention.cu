@@ -161,7 +161,8 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
       limit[rt][half] = i < have ? (p.together ? length - 1 : base + row_of(i)) : -1;
     }
   const float exponent_scale = rsqrtf(float(kDim)) * kLog2e;
-  float* const raw = kWeights ? p.raw + (size_t(sequence) * p.kv_heads + kv_head) * p.raw_rows * p.raw_stride : nullptr;
+  float* const raw =
+      kWeights ? p.raw + ((size_t(sequence) * p.kv_heads + kv_head) * p.raw_rows + size_t(blockIdx.z) * kStepRows) * p.raw_stride : nullptr;
 
   float o[kRowTiles][16][4];
   float m[kRowTiles][2], l[kRowTiles][2];
@@ -422,7 +423,10 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
     for (uint32_t r = 0; r < splits; ++r) sum += sh->blocks[r][i].y;
 #pragma unroll 4
     for (int j = 0; j < count; ++j) sum += others[j][i].y;
-    sh->inverse[i] = count < 0 || sum == 0.0f ? 0.0f : p.partial ? sum : 1.0f / sum;
+    const float inverse = count < 0 || sum == 0.0f ? 0.0f : p.partial ? sum : 1.0f / sum;
+    sh->inverse[i] = inverse;
+    if (kWeights && p.row_stats && rank == 0 && i < have)
+      p.row_stats[(size_t(sequence) * p.kv_heads + kv_head) * p.raw_rows + size_t(blockIdx.z) * kStepRows + i] = make_float2(sh->top[i], inverse);
   }
   __syncthreads();
   {
@@ -474,7 +478,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
       }
     }
   }
-  if (kWeights) {
+  if (kWeights && !p.row_stats) {
     // This block's tokens: the sum over the rows, in their order. A thread has kQuads times four neighbours, of four rows, under way:
     // behind a saturated memory a trip to the L2 takes 2 us.
     constexpr int kQuads = 4;
@@ -534,6 +538,53 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
     }
   }
   if (splits > 1) cluster_sync();  // no block leaves while another reads its shared memory
+}
+
+// Weights of more than one unit's rows: block (128 tokens, KV head, sequence), a warp takes every eighth row, the warps' sums are
+// added in their order.
+constexpr int kWeightWarps = 8;
+__global__ void __launch_bounds__(kWeightWarps * 32) step_weights_kernel(const __grid_constant__ StepAttentionParams p, int rows) {
+  __shared__ float4 sums[kWeightWarps][32];
+  const int kv_head = blockIdx.y, sequence = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  grid_dependency_wait();
+  int length = p.lengths ? p.lengths[sequence] : p.length;
+  if (length < 0 || length > p.capacity) length = 0;
+  const int first = blockIdx.x * 128, t = first + lane * 4;
+  if (first >= length) return;
+  const size_t unit = (size_t(sequence) * p.kv_heads + kv_head) * p.raw_rows;
+  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  constexpr int kAtOnce = 8;
+  for (int i0 = warp; i0 < rows; i0 += kWeightWarps * kAtOnce) {
+    float4 score[kAtOnce];
+    float2 stats[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int i = i0 + u * kWeightWarps;
+      stats[u] = make_float2(0.0f, 0.0f);
+      if (i < rows && t < length) {  // whole tiles of scores are there
+        stats[u] = p.row_stats[unit + i];
+        score[u] = *reinterpret_cast<const float4*>(p.raw + (unit + i) * p.raw_stride + t);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      if (stats[u].y == 0.0f) continue;
+      sum.x = fmaf(power_of_two(score[u].x - stats[u].x), stats[u].y, sum.x);
+      sum.y = fmaf(power_of_two(score[u].y - stats[u].x), stats[u].y, sum.y);
+      sum.z = fmaf(power_of_two(score[u].z - stats[u].x), stats[u].y, sum.z);
+      sum.w = fmaf(power_of_two(score[u].w - stats[u].x), stats[u].y, sum.w);
+    }
+  }
+  sums[warp][lane] = sum;
+  __syncthreads();
+  if (threadIdx.x < 128 && first + int(threadIdx.x) < length) {
+    float total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWeightWarps; ++w) total += reinterpret_cast<const float*>(sums[w])[threadIdx.x];
+    const int token = first + int(threadIdx.x);
+    const float old = p.scores ? p.scores[sequence * p.scores_sequence + kv_head * p.scores_head + token] : 0.0f;
+    p.scores_out[sequence * p.out_sequence + kv_head * p.out_head + token] = old + total;
+  }
 }
 
 template <int kWarps>
@@ -605,6 +656,12 @@ void launch_step_attention(const StepAttentionParams& p, size_t tokens, cudaStre
   attributes[1].val.programmaticStreamSerializationAllowed = 1;
   if (pdl) config.numAttrs = 2;
   check_cuda(cudaLaunchKernelEx(&config, step_kernel(shape.warps, two, p.raw != nullptr), p), "cudaLaunchKernelEx");
+}
+
+void launch_step_weights(const StepAttentionParams& p, size_t tokens, cudaStream_t stream) {
+  const int rows = std::min(p.groups * kStepRows, p.rows * (p.heads / p.kv_heads) - p.first_group * kStepRows);
+  launch(step_weights_kernel, dim3(unsigned((tokens + 127) / 128), unsigned(p.kv_heads), unsigned(p.sequences)), dim3(kWeightWarps * 32), 0, stream, true,
+         p, rows);
 }
 
 }  // namespace ei

@@ -36,16 +36,21 @@ struct StepAttentionParams {
   int joined_border, joined_counts[2];
   float* partial;             // leave (sums, maximum, sum) here in that layout instead of normalised rows in `out`
   // Weights: scores_out[s][j][t] = scores[s][j][t] + the weights of token t, summed over this launch's rows and the group's
-  // heads; every token of the sequence is written. raw: [sequences][kv_heads][raw_rows][raw_stride] FP32.
+  // heads; every token of the sequence is written. raw: [sequences][kv_heads][raw_rows][raw_stride] FP32. Rows of one unit (one
+  // group) are added up by its own blocks; of more, row_stats [sequences][kv_heads][raw_rows] receives each row's maximum and
+  // inverse sum, and launch_step_weights adds up.
   const float* scores;
   float* scores_out;
   size_t scores_sequence, scores_head, out_sequence, out_head;
   float* raw;
-  size_t raw_rows, raw_stride;  // a unit's rows; its tokens, whole tiles
+  size_t raw_rows, raw_stride;  // the launch's stacked rows; tokens, whole tiles
+  float2* row_stats;
 };
 constexpr int kStepRows = 32;  // stacked query rows (row x query head of one KV head) of a unit
 inline int step_groups(int rows, int group) { return int((size_t(rows) * group + kStepRows - 1) / kStepRows); }
 // k_map, v_map, first_group and groups are the caller's; tokens: the most a unit may read.
 void launch_step_attention(const StepAttentionParams& p, size_t tokens, cudaStream_t stream, bool pdl);
+constexpr int kStepWeightGroups = 8;  // that may share a launch with weights (their scores take scratch)
+void launch_step_weights(const StepAttentionParams& p, size_t tokens, cudaStream_t stream);
 
 }  // namespace ei

@@ -216,7 +216,7 @@ ei_status ei_attention_shared_prefix_bf16(const ei_context* ctx, ei_view3 q, ei_
 /* Causal attention that adds up what every cached token received: scores_out[s][j][t] = scores[s][j][t] + the softmax weights
  * of token t, over the call's rows and the query heads of KV head j, for every token t of sequence s; FP32
  * [sequences, kv_heads, capacity]. Places behind a sequence's length are left as they were. scores_out may be `scores` itself;
- * scores with null data count as zeros. For steps of a few rows: 32 of rows * (heads / kv_heads) share a launch. */
+ * scores with null data count as zeros. Meant for steps and observation windows: 256 of rows * (heads / kv_heads) share a pass. */
 size_t ei_attention_accumulate_scratch_bytes(size_t sequences, size_t rows, size_t query_heads, size_t kv_heads, size_t capacity);
 ei_status ei_attention_accumulate_bf16(const ei_context* ctx, ei_view3 q, ei_view4 k, ei_view4 v, ei_view3 out,
                                        const int32_t* lengths, size_t length, ei_view3 scores, ei_view3 scores_out, void* scratch,

@@ -195,7 +195,7 @@ def test_more_attention_refusals(call):
     refused(call, call.lib.ei_attention_window_bf16(C.byref(call.ctx), *a, 0, 4), says="window")
     scores, ctx = call.view(5, 2, 2, 70), C.byref(call.ctx)
     need = call.lib.ei_attention_accumulate_scratch_bytes(2, 3, 8, 2, 70)
-    assert need == 2 * 2 * 12 * 96 * 4
+    assert need == 2 * 2 * 12 * (96 * 4 + 8)
     accumulate = call.lib.ei_attention_accumulate_bf16
     refused(call, accumulate(ctx, *a, scores, scores, 1 << 30, need - 1), says="scratch")
     refused(call, accumulate(ctx, *a, scores, scores, (1 << 30) + 4, need), says="scratch")

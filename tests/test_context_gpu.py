@@ -351,6 +351,9 @@ ACCUMULATE_CASES = [
     ([2000], 2001, 1, 16, 8, False),
     ([900, 45], 901, 32, 16, 4, True),               # an observation window of 128 stacked rows
     ([6000], 6000, 2, 32, 8, False),
+    ([700, 129, 100], 701, 130, 12, 4, True),        # 390 stacked rows: two passes; padded on the left
+    ([300], 300, 100, 16, 4, False),                 # 400 without old scores
+    ([128, 0], 128, 16, 28, 4, True),                # 112
 ]
 
 
