@@ -111,6 +111,10 @@ WINDOW_CASES = [
     ([3000], 3000, 129, 8, 8, 2900, 100, "tokens"),
     ([2000, 1500, 900, 20], 2000, 32, 32, 8, 2000, 0, "tokens"),
     ([2048 - 40 * i for i in range(24)], 2048, 32, 32, 8, 2048, 0, "tokens"),  # no cluster, both halves at one query tile
+    ([500, 33], 500, 16, 64, 1, 300, 4, "tokens"),           # 64, 128 and 256 query heads over one
+    ([2500], 2500, 7, 128, 1, 2400, 4, "heads"),
+    ([700], 700, 5, 256, 1, 600, 1, "tokens"),
+    ([40] * 300, 64, 1, 8, 2, 30, 2, "tokens"),              # many sequences
 ]
 
 
