@@ -14,7 +14,6 @@
 namespace ei {
 namespace {
 
-constexpr int kDim = 128;
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMoves = 4;          // tokens a warp has under way
 constexpr int kCachedKeys = 40960;  // keys that a block holds itself (160 KB); further ones are made from the scores again

@@ -9,7 +9,7 @@
 // members of every pair are its own: vectors j and j + rotary / 16 of the rotated part (whole neighbours' pairs lie in any
 // vector), two adjacent ones of the rest. So a head is width / 16 lanes, the norm a few shuffles, and nothing passes through
 // shared memory. A thread takes the same place of kHeads heads of a row, whose loads are under way together; the table's 64 bytes
-// for that place are read once for them. 2048 rows of 32 + 8 heads of 128: 12.0 us = 3.5 TB/s, two waves of blocks that each wait
+// for that place are read once for them. 2048 rows of 32 + 8 heads of 128: 11.8 us = 3.6 TB/s, two waves of blocks that each wait
 // for the position, then for the table; 64 rows: 2.4 us, a launch.
 #include "context_kernels.cuh"
 
@@ -29,9 +29,10 @@ __device__ __forceinline__ uint4 pack(const float* x) {
   return make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
 }
 
-// Block (row, chunk of heads); `lanes` (a power of two >= width / 16) threads a head.
-template <bool kInterleaved>
-__global__ void __launch_bounds__(kMostThreads) qk_norm_rope_kernel(const QkRopeParams p, int lanes) {
+// Block (row, chunk of heads); kLanes (a power of two >= width / 16) threads a head.
+template <bool kInterleaved, int kLanes>
+__global__ void __launch_bounds__(kMostThreads) qk_norm_rope_kernel(const __grid_constant__ QkRopeParams p) {
+  constexpr int lanes = kLanes;
   const int row = blockIdx.x;
   const int slot = threadIdx.x / lanes, slots = blockDim.x / lanes, j = threadIdx.x & (lanes - 1);
   const bool active = j < p.width / 16;
@@ -79,6 +80,7 @@ __global__ void __launch_bounds__(kMostThreads) qk_norm_rope_kernel(const QkRope
     float squares = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) squares = fmaf(x[i], x[i], squares);
+#pragma unroll
     for (int o = lanes >> 1; o > 0; o >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, o);
     if (!active || head >= stop) continue;
     if (weight) {
@@ -109,18 +111,32 @@ __global__ void __launch_bounds__(kMostThreads) qk_norm_rope_kernel(const QkRope
   }
 }
 
+using RopeKernel = void (*)(QkRopeParams);
+template <bool kInterleaved>
+RopeKernel rope_kernel_of(int lanes) {
+  switch (lanes) {
+    case 1: return qk_norm_rope_kernel<kInterleaved, 1>;
+    case 2: return qk_norm_rope_kernel<kInterleaved, 2>;
+    case 4: return qk_norm_rope_kernel<kInterleaved, 4>;
+    case 8: return qk_norm_rope_kernel<kInterleaved, 8>;
+    case 16: return qk_norm_rope_kernel<kInterleaved, 16>;
+    default: return qk_norm_rope_kernel<kInterleaved, 32>;
+  }
+}
+RopeKernel rope_kernel(bool interleaved, int lanes) { return interleaved ? rope_kernel_of<true>(lanes) : rope_kernel_of<false>(lanes); }
+
 }  // namespace
 
 void launch_qk_norm_rope(const QkRopeParams& p, cudaStream_t stream) {
   int lanes = 1;
   while (lanes < p.width / 16) lanes *= 2;
-  // A row's heads make a block where they can. (2048 rows of 32 + 8 heads: 11.9 us; a block that walks rows with the next one's loads
+  // A row's heads make a block where they can. (2048 rows of 32 + 8 heads: 11.8 us; a block that walks rows with the next one's loads
   // under way needs twice the registers and takes 14.8, four heads a thread 14.1, one 13.9.)
   const int all = p.heads + p.kv_heads;
   const int threads = std::min(kMostThreads, ((all + kHeads - 1) / kHeads * lanes + 31) / 32 * 32);
   const int chunk = threads / lanes * kHeads;
   const dim3 grid(unsigned(p.rows), unsigned((all + chunk - 1) / chunk));
-  launch(p.interleaved ? qk_norm_rope_kernel<true> : qk_norm_rope_kernel<false>, grid, dim3(unsigned(threads)), 0, stream, false, p, lanes);
+  launch(rope_kernel(p.interleaved, lanes), grid, dim3(unsigned(threads)), 0, stream, false, p);
 }
 
 }  // namespace ei

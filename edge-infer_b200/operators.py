@@ -138,7 +138,10 @@ def _native():
     if _native_calls is None:
         import torch
         _lib()
-        from . import _calls
+        try:
+            from . import _calls
+        except ImportError as error:
+            raise ImportError(f"{abi.HERE / '_calls.so'} is not built. Run `python edge-infer_b200/build.py`.") from error
         _calls.configure(torch.bfloat16, torch.float32, torch.int32)
         _native_calls = _calls
     return _native_calls
