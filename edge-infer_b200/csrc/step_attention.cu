@@ -659,6 +659,7 @@ void launch_step_attention(const StepAttentionParams& p, size_t tokens, cudaStre
 }
 
 void launch_step_weights(const StepAttentionParams& p, size_t tokens, cudaStream_t stream) {
+  if (tokens == 0) return;  // no token to add to, and no launch without blocks
   const int rows = std::min(p.groups * kStepRows, p.rows * (p.heads / p.kv_heads) - p.first_group * kStepRows);
   launch(step_weights_kernel, dim3(unsigned((tokens + 127) / 128), unsigned(p.kv_heads), unsigned(p.sequences)), dim3(kWeightWarps * 32), 0, stream, true,
          p, rows);
