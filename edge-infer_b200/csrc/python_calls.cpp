@@ -114,6 +114,16 @@ bool begin(PyObject* const* args, Py_ssize_t given, Py_ssize_t wanted, const ei_
   return *ctx != nullptr;
 }
 
+// The C call runs without the interpreter's lock, as calls through ctypes do: a launch waits while the device's queue is full, and
+// what empties the queue may need the interpreter. The caller holds the tensors and the context meanwhile.
+template <typename Call>
+PyObject* status_of(Call call) {
+  PyThreadState* const thread = PyEval_SaveThread();
+  const ei_status status = call();
+  PyEval_RestoreThread(thread);
+  return PyLong_FromLong(status);
+}
+
 PyObject* configure(PyObject*, PyObject* const* args, Py_ssize_t given) {
   if (given != 3) return PyErr_Format(PyExc_TypeError, "expected 3 types");
   PyObject** const types[3] = {&type_bf16, &type_f32, &type_i32};
@@ -140,7 +150,9 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t given) {
   const double epsilon = PyFloat_AsDouble(a[10]);
   const int interleaved = PyObject_IsTrue(a[11]);
   if (PyErr_Occurred()) return nullptr;
-  return PyLong_FromLong(ei_qk_norm_rope_bf16(ctx, q, k, table, positions, offset, q_weight, k_weight, float(epsilon), interleaved, q_out, k_out));
+  return status_of([&] {
+    return ei_qk_norm_rope_bf16(ctx, q, k, table, positions, offset, q_weight, k_weight, float(epsilon), interleaved, q_out, k_out);
+  });
 }
 
 // (ctx, q, k, v, output, window, sinks, lengths, length)
@@ -154,7 +166,7 @@ PyObject* attention_window(PyObject*, PyObject* const* a, Py_ssize_t given) {
       !view(a[4], ctx, type_bf16, &out) || !as_size(a[5], &window) || !as_size(a[6], &sinks) ||
       !values(a[7], ctx, k.shape[0], "lengths", &lengths) || !as_size(a[8], &length))
     return nullptr;
-  return PyLong_FromLong(ei_attention_window_bf16(ctx, q, k, v, out, lengths, length, window, sinks));
+  return status_of([&] { return ei_attention_window_bf16(ctx, q, k, v, out, lengths, length, window, sinks); });
 }
 
 // (ctx, q, prefix_k, prefix_v, k, v, output, scratch, lengths, length)
@@ -170,7 +182,9 @@ PyObject* attention_shared_prefix(PyObject*, PyObject* const* a, Py_ssize_t give
       !view(a[6], ctx, type_bf16, &out) || !scratch_of(a[7], ctx, &scratch, &scratch_bytes) ||
       !values(a[8], ctx, k.shape[0], "lengths", &lengths) || !as_size(a[9], &length))
     return nullptr;
-  return PyLong_FromLong(ei_attention_shared_prefix_bf16(ctx, q, prefix_k, prefix_v, k, v, out, lengths, length, scratch, scratch_bytes));
+  return status_of([&] {
+    return ei_attention_shared_prefix_bf16(ctx, q, prefix_k, prefix_v, k, v, out, lengths, length, scratch, scratch_bytes);
+  });
 }
 
 // (ctx, q, k, v, output, scores, scores_out, scratch, lengths, length)
@@ -186,7 +200,9 @@ PyObject* attention_accumulate(PyObject*, PyObject* const* a, Py_ssize_t given) 
       !view(a[6], ctx, type_f32, &scores_out) || !scratch_of(a[7], ctx, &scratch, &scratch_bytes) ||
       !values(a[8], ctx, k.shape[0], "lengths", &lengths) || !as_size(a[9], &length))
     return nullptr;
-  return PyLong_FromLong(ei_attention_accumulate_bf16(ctx, q, k, v, out, lengths, length, scores, scores_out, scratch, scratch_bytes));
+  return status_of([&] {
+    return ei_attention_accumulate_bf16(ctx, q, k, v, out, lengths, length, scores, scores_out, scratch, scratch_bytes);
+  });
 }
 
 // (ctx, k, v, scores, k_out, v_out, scores_out, kept, lengths_out, sinks, recent, lengths, length)
@@ -201,7 +217,9 @@ PyObject* evict_kv(PyObject*, PyObject* const* a, Py_ssize_t given) {
       !view(a[7], ctx, type_i32, &kept) || !values(a[8], ctx, k.shape[0], "lengths_out", &lengths_out) || !as_size(a[9], &sinks) ||
       !as_size(a[10], &recent) || !values(a[11], ctx, k.shape[0], "lengths", &lengths) || !as_size(a[12], &length))
     return nullptr;
-  return PyLong_FromLong(ei_evict_kv_bf16(ctx, k, v, scores, lengths, length, sinks, recent, k_out, v_out, scores_out, kept, lengths_out));
+  return status_of([&] {
+    return ei_evict_kv_bf16(ctx, k, v, scores, lengths, length, sinks, recent, k_out, v_out, scores_out, kept, lengths_out);
+  });
 }
 
 #define CALL(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr}
