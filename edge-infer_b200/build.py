@@ -3,8 +3,9 @@
     python edge-infer_b200/build.py            # incremental
     python edge-infer_b200/build.py --force
 
-Output: edge-infer_b200/libedge_infer_b200.so and _calls.so, the Python calls that take torch tensors apart natively (both
-git-ignored; they travel with the tree).
+Output: edge-infer_b200/libedge_infer_b200.so and _calls.so, the Python calls that take torch
+tensors apart natively (both git-ignored; they travel with the tree). Where Python's headers are not installed only the library
+is built: hosts that link it need no more, and the operators that go through the native calls say what is missing.
 """
 from __future__ import annotations
 
@@ -37,6 +38,23 @@ def _newest_dependency() -> float:
     return max(p.stat().st_mtime for p in paths)
 
 
+def _python_headers() -> Path | None:
+    include = Path(sysconfig.get_paths()["include"])
+    return include if (include / "Python.h").exists() else None
+
+
+def _build_calls() -> None:
+    include = _python_headers()
+    if include is None:
+        print(f"{sysconfig.get_paths()['include']} has no Python.h: {CALLS.name} is not built", file=sys.stderr)
+        return
+    calls = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared", "-I" + str(include),
+             str(CSRC / "python_calls.cpp"), "-o", str(CALLS), "-L" + str(HERE), "-ledge_infer_b200", "-Wl,-rpath,$ORIGIN"]
+    result = subprocess.run(calls, capture_output=True, text=True)
+    if result.returncode:
+        raise RuntimeError(f"compilation of the Python calls failed:\n{result.stdout}\n{result.stderr}")
+
+
 def _compile(source: str, verbose: bool) -> None:
     out = OBJ / (source + ".o")
     cmd = [NVCC, *FLAGS, "-c", str(CSRC / source), "-o", str(out)]
@@ -53,7 +71,8 @@ def _compile(source: str, verbose: bool) -> None:
 def build(force: bool = False, verbose: bool = False) -> Path:
     """Compiles every CUDA source for sm_100a and links the shared library."""
     newest = _newest_dependency()
-    if not force and all(p.exists() and p.stat().st_mtime >= newest for p in (LIB, CALLS)):
+    wanted = (LIB, CALLS) if _python_headers() else (LIB,)
+    if not force and all(p.exists() and p.stat().st_mtime >= newest for p in wanted):
         return LIB
     OBJ.mkdir(exist_ok=True)
     stale = [s for s in SOURCES
@@ -66,11 +85,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     result = subprocess.run(link, capture_output=True, text=True)
     if result.returncode:
         raise RuntimeError(f"link failed:\n{result.stdout}\n{result.stderr}")
-    calls = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared", "-I" + sysconfig.get_paths()["include"],
-             str(CSRC / "python_calls.cpp"), "-o", str(CALLS), "-L" + str(HERE), "-ledge_infer_b200", "-Wl,-rpath,$ORIGIN"]
-    result = subprocess.run(calls, capture_output=True, text=True)
-    if result.returncode:
-        raise RuntimeError(f"compilation of the Python calls failed:\n{result.stdout}\n{result.stderr}")
+    _build_calls()
     return LIB
 
 
