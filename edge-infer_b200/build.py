@@ -3,7 +3,7 @@
     python edge-infer_b200/build.py            # incremental
     python edge-infer_b200/build.py --force
 
-Output: edge-infer_b200/libedge_infer_b200.so and _calls.so, the Python calls that take torch
+Output: edge-infer_b200/libedge_infer_b200.so and _calls with the interpreter's suffix, the Python calls that take torch
 tensors apart natively (both git-ignored; they travel with the tree). Where Python's headers are not installed only the library
 is built: hosts that link it need no more, and the operators that go through the native calls say what is missing.
 """
@@ -20,7 +20,7 @@ HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 OBJ = HERE / "build"
 LIB = HERE / "libedge_infer_b200.so"
-CALLS = HERE / "_calls.so"
+CALLS = HERE / ("_calls" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))  # another interpreter's is not loaded
 SOURCES = ["abi_ops.cu", "smallm_gemm.cu", "prompt_gemm.cu", "elementwise.cu", "attention.cu", "sampling.cu", "runtime.cu",
            "layered.cu", "layered_kernels.cu", "lightning.cu", "sized_attention.cu",
            "parallel_block.cu", "outer_state.cu", "latent_attention.cu", "delta_prompt.cu",
@@ -53,6 +53,8 @@ def _build_calls() -> None:
     result = subprocess.run(calls, capture_output=True, text=True)
     if result.returncode:
         raise RuntimeError(f"compilation of the Python calls failed:\n{result.stdout}\n{result.stderr}")
+    if CALLS.name != "_calls.so":
+        (HERE / "_calls.so").unlink(missing_ok=True)  # of any interpreter: an earlier build's name
 
 
 def _compile(source: str, verbose: bool) -> None:

@@ -141,8 +141,8 @@ def _native():
         try:
             from . import _calls
         except ImportError as error:
-            raise ImportError(f"{abi.HERE / '_calls.so'} is not built. Run `python edge-infer_b200/build.py` where Python's "
-                              "headers are installed.") from error
+            raise ImportError(f"{abi.HERE / '_calls'} is not built for this interpreter. Run `python edge-infer_b200/build.py` where "
+                              "Python's headers are installed.") from error
         _calls.configure(torch.bfloat16, torch.float32, torch.int32)
         _native_calls = _calls
     return _native_calls

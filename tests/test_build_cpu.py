@@ -41,3 +41,14 @@ def test_the_library_needs_no_python_headers(builder, tmp_path, monkeypatch, cap
     builder.commands.clear()
     builder.build()
     assert builder.commands == []
+
+
+def test_python_calls_are_built_for_one_interpreter(builder):
+    """Their file's name carries the interpreter's suffix, and a build leaves none that any interpreter would load."""
+    (builder.HERE / "_calls.so").write_bytes(b"")
+    builder.build()
+    assert (builder.HERE / ("_calls" + sysconfig.get_config_var("EXT_SUFFIX"))).exists()
+    assert sysconfig.get_config_var("EXT_SUFFIX") == ".so" or not (builder.HERE / "_calls.so").exists()
+    builder.commands.clear()
+    builder.build()
+    assert builder.commands == []
