@@ -5,9 +5,11 @@
 #include "context_kernels.cuh"
 #include "span_attention.cuh"
 #include "step_choice.hpp"
+#include "view_overlap.hpp"
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 #include <vector>
 
 using namespace ei;
@@ -39,6 +41,13 @@ bool overlap(const A& a, size_t a_size, const B& b, size_t b_size) {
   const uintptr_t a0 = reinterpret_cast<uintptr_t>(a.data), b0 = reinterpret_cast<uintptr_t>(b.data);
   return a0 < b0 + extent_of(b) * b_size && b0 < a0 + extent_of(a) * a_size;
 }
+
+// `out` is written while others read or write the rest.
+void expect_apart(const Region& out, std::initializer_list<Region> others, const char* what) {
+  for (const Region& other : others)
+    if (may_meet(out, other)) reject(what);
+}
+Region region_of_rows(const ei_view3& v) { return region_of(v, sizeof(bf16), 2); }
 
 // [rows, heads, width]: heads of a row adjacent, rows 16-byte aligned and disjoint.
 void expect_rows(const ei_view3& v, const char* name) {
@@ -207,11 +216,6 @@ ei_status ei_qk_norm_rope_bf16(const ei_context* ctx, ei_view3 q, ei_view3 k, ei
     const size_t rows = q.shape[0], width = q.shape[2];
     if (k.shape[0] != rows || k.shape[2] != width) reject("queries and keys must share rows and head width");
     if (width % 16 || width > 512) reject("the head width must be a multiple of 16 up to 512");
-    // In place, or apart.
-    for (const auto& pair : {std::make_pair(&q, &q_out), std::make_pair(&k, &k_out)}) {
-      const bool same = pair.first->data == pair.second->data && row_stride(*pair.first) == row_stride(*pair.second);
-      if (!same && overlap(*pair.first, 2, *pair.second, 2)) reject("rotated heads must replace their inputs or lie apart from them");
-    }
     expect_packed(table, "RoPE table");
     const size_t rotary = table.shape[1];
     if (rotary % 16 || rotary > width) reject("the rotated width must be a multiple of 16 within the head");
@@ -224,6 +228,18 @@ ei_status ei_qk_norm_rope_bf16(const ei_context* ctx, ei_view3 q, ei_view3 k, ei
       if (weight->shape[0] != width || weight->stride[0] != 1 || !aligned16(weight->data))
         reject("a norm weight must have one packed, 16-byte aligned value per value of a head");
     }
+    // In place, or apart: a thread reads its own values before it writes them, others' at any time.
+    const char* apart = "rotated heads must replace their inputs or lie apart from them and from all else";
+    for (const ei_view3* to : {&q_out, &k_out}) {
+      const ei_view3 &from = to == &q_out ? q : k, &other = to == &q_out ? k : q;
+      const Region out = region_of_rows(*to);
+      if (from.data != to->data || row_stride(from) != row_stride(*to)) expect_apart(out, {region_of_rows(from)}, apart);
+      expect_apart(out,
+                   {region_of_rows(other), region_of(table.data, table.shape[0] * rotary * sizeof(float)), region_of(positions, rows * sizeof(int32_t)),
+                    region_of(q_weight.data, width * sizeof(bf16)), region_of(k_weight.data, width * sizeof(bf16))},
+                   apart);
+    }
+    expect_apart(region_of_rows(q_out), {region_of_rows(k_out)}, apart);
     if ((q_weight.data || k_weight.data) && !(std::isfinite(epsilon) && epsilon >= 0.0f)) reject("the norm's epsilon must not be negative");
     if (q.shape[1] + k.shape[1] > size_t(1) << 20) reject("too many heads");
     expect_current_device(ctx);

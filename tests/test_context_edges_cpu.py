@@ -1,0 +1,67 @@
+"""CPU checks of what the operators for long contexts refuse: outputs that meet other arguments in memory."""
+import ctypes as C
+import itertools
+
+import pytest
+
+from test_context_cpu import Call, call, refused, run_choice  # noqa: F401
+
+
+def accepted(call, status):
+    """Nothing about the arguments is wrong: what is left to refuse is the context, of a device that no machine has."""
+    with pytest.raises((RuntimeError, ValueError)) as caught:
+        call.abi.check(status)
+    assert isinstance(caught.value, RuntimeError) or "another CUDA device" in str(caught.value), str(caught.value)
+
+
+@pytest.fixture
+def elsewhere(call):  # noqa: F811
+    call.ctx.device = 1 << 20
+    return call
+
+
+def test_views_that_may_meet(tmp_path):
+    """Against the sets of bytes of small views: two that meet are always found, those that lie apart in the ways that buffers
+    are shared in earnest are told apart."""
+    meet = run_choice(tmp_path, "view_overlap.hpp", 'auto r = [&](int i) { ei::Region g{(uintptr_t)atoll(a[i]), (size_t)atoll(a[i + 1]), 2, '
+                      '{(size_t)atoll(a[i + 2]), (size_t)atoll(a[i + 4])}, {(size_t)atoll(a[i + 3]), (size_t)atoll(a[i + 5])}}; return g; };'
+                      'std::printf("%d", int(ei::may_meet(r(1), r(7))));')
+
+    def touched(at, item, n0, s0, n1, s1):
+        return {at + i * s0 + j * s1 + x for i in range(n0) for j in range(n1) for x in range(item)}
+
+    shapes = [(4, 3, 16, 1, 4), (4, 3, 16, 2, 4), (8, 2, 48, 3, 16), (6, 1, 7, 4, 16), (4, 2, 20, 3, 8)]
+    for (one, two), shift in itertools.product(itertools.product(shapes, shapes), (0, 3, 4, 8, 30, 200)):
+        a, b = (64, *one), (64 + shift, *two)
+        met = meet(*a, *b)[0]
+        assert met == meet(*b, *a)[0]
+        assert met or not touched(*a) & touched(*b)
+        assert not met or min(touched(*b)) <= max(touched(*a))
+    # Keys and values side by side for every token; halves of every row; one row behind the other.
+    assert meet(64, 8, 5, 160, 10, 16, 72, 8, 5, 160, 10, 16) == [0]
+    assert meet(64, 8, 5, 160, 10, 16, 71, 8, 5, 160, 10, 16) == [1]
+    assert meet(64, 80, 5, 160, 1, 1, 144, 80, 5, 160, 1, 1) == [0]
+    assert meet(64, 16, 1, 16, 1, 16, 80, 16, 1, 16, 1, 16) == [0]
+    assert meet(64, 1, 2 ** 40, 2 ** 40, 2 ** 40, 2 ** 40, 80, 16, 1, 16, 1, 16) == [1]
+
+
+def test_rotated_heads_that_meet_other_arguments(elsewhere):
+    call, fn, none = elsewhere, elsewhere.lib.ei_qk_norm_rope_bf16, elsewhere.abi.View1()
+
+    def go(q=call.view(1, 5, 4, 64), k=call.view(2, 5, 2, 64), table=call.view(3, 99, 64), positions=None, qw=none, q_out=call.view(4, 5, 4, 64),
+           k_out=call.view(5, 5, 2, 64)):
+        return fn(C.byref(call.ctx), q, k, table, positions, 0, qw, none, 1e-6, 0, q_out, k_out)
+
+    accepted(call, go())
+    accepted(call, go(q_out=call.view(1, 5, 4, 64), k_out=call.view(2, 5, 2, 64)))
+    # Slices of one projection's rows, in place and apart.
+    fused = lambda first, heads: call.view(1, 5, heads, 64, stride=(14 * 64, 64, 1), offset=first * 128)
+    accepted(call, go(q=fused(0, 4), k=fused(4, 2), q_out=fused(0, 4), k_out=fused(4, 2)))
+    accepted(call, go(q=fused(0, 4), k=fused(4, 2), q_out=fused(8, 4), k_out=fused(12, 2)))
+    for fault in (dict(q_out=call.view(2, 5, 4, 64)), dict(k_out=call.view(1, 5, 2, 64, offset=256)),
+                  dict(q_out=call.view(4, 5, 4, 64), k_out=call.view(4, 5, 2, 64, offset=512)),
+                  dict(q_out=call.view(1, 5, 4, 64), k_out=call.view(1, 5, 2, 64)),
+                  dict(q=fused(0, 4), k=fused(4, 2), q_out=fused(1, 4)), dict(q=fused(0, 4), k=fused(4, 2), k_out=fused(3, 2)),
+                  dict(q_out=call.view(3, 5, 4, 64, offset=64)), dict(k_out=call.view(3, 5, 2, 64, offset=99 * 256 - 16)),
+                  dict(qw=call.view(4, 64, offset=128)), dict(positions=call.view(5, 5).data + 1264)):
+        refused(call, go(**fault), says="lie apart")
