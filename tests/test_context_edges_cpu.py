@@ -42,7 +42,9 @@ def test_views_that_may_meet(tmp_path):
     assert meet(64, 8, 5, 160, 10, 16, 71, 8, 5, 160, 10, 16) == [1]
     assert meet(64, 80, 5, 160, 1, 1, 144, 80, 5, 160, 1, 1) == [0]
     assert meet(64, 16, 1, 16, 1, 16, 80, 16, 1, 16, 1, 16) == [0]
-    assert meet(64, 1, 2 ** 40, 2 ** 40, 2 ** 40, 2 ** 40, 80, 16, 1, 16, 1, 16) == [1]
+    # A reach beyond 64 bits.
+    assert meet(64, 1, 2 ** 40, 2 ** 40, 2 ** 40, 2 ** 40, 80, 16, 1, 16, 1, 16) == [0]
+    assert meet(64, 17, 2 ** 40, 2 ** 40, 2 ** 40, 2 ** 40, 80, 16, 1, 16, 1, 16) == [1]
 
 
 def test_rotated_heads_that_meet_other_arguments(elsewhere):
