@@ -48,6 +48,9 @@ void expect_apart(const Region& out, std::initializer_list<Region> others, const
     if (may_meet(out, other)) reject(what);
 }
 Region region_of_rows(const ei_view3& v) { return region_of(v, sizeof(bf16), 2); }
+Region region_of_cache(const ei_view4& v) { return region_of(v, sizeof(bf16), 1); }
+Region region_of_scores(const ei_view3& v) { return region_of(v, sizeof(float), 1); }
+Region region_of_lengths(const int32_t* lengths, size_t sequences) { return region_of(lengths, sequences * sizeof(int32_t)); }
 
 // [rows, heads, width]: heads of a row adjacent, rows 16-byte aligned and disjoint.
 void expect_rows(const ei_view3& v, const char* name) {
@@ -109,6 +112,11 @@ StepAttentionParams attention_of(const ei_view3& q, const ei_view4& k, const ei_
   if (rows > kMostTokens / group || (rows * group + kStepRows - 1) / kStepRows > 65535) reject("too many query rows");
   if (q.shape[0] > (size_t(1) << 31) / q.shape[1]) reject("too many query rows");
   if (!lengths && length > k.shape[1]) reject("the length exceeds the caches' capacity");
+  // A row's queries are read by the blocks that write it and, as part of their boxes, by others that do not use them.
+  if (q.data != out.data || row_stride(q) != row_stride(out))
+    expect_apart(region_of_rows(out), {region_of_rows(q)}, "attention outputs must be the queries' own view or lie apart from them");
+  expect_apart(region_of_rows(out), {region_of_cache(k), region_of_cache(v), region_of_lengths(lengths, k.shape[0])},
+               "attention outputs must lie apart from keys, values and lengths");
   StepAttentionParams p{};
   p.q = static_cast<const bf16*>(q.data);
   p.q_stride = row_stride(q);
@@ -316,6 +324,12 @@ ei_status ei_attention_shared_prefix_bf16(const ei_context* ctx, ei_view3 q, ei_
           scratch_bytes < ei_attention_shared_prefix_scratch_bytes(q.shape[0], q.shape[1], k.shape[2], prefix))
         reject("shared prefix attention needs 16-byte aligned scratch of the size it names");
       if ((q.shape[0] * (q.shape[1] / k.shape[2]) + kStepRows - 1) / kStepRows > 65535) reject("too many query rows");
+      const Region first_k = region_of(prefix_k, sizeof(bf16), 1), first_v = region_of(prefix_v, sizeof(bf16), 1);
+      expect_apart(region_of_rows(out), {first_k, first_v}, "attention outputs must lie apart from the prefix");
+      expect_apart(region_of(scratch, ei_attention_shared_prefix_scratch_bytes(q.shape[0], q.shape[1], k.shape[2], prefix)),
+                   {first_k, first_v, region_of_rows(q), region_of_cache(k), region_of_cache(v), region_of_lengths(lengths, k.shape[0]),
+                    region_of_rows(out)},
+                   "scratch must lie apart from all else");
     }
     expect_current_device(ctx);
     encode_maps(&own, keys, values);
@@ -365,11 +379,19 @@ ei_status ei_attention_accumulate_bf16(const ei_context* ctx, ei_view3 q, ei_vie
     if (scores.data) expect_scores(scores, k.shape[0], k.shape[2], k.shape[1], "accumulated weights");
     expect_scores(scores_out, k.shape[0], k.shape[2], k.shape[1], "new accumulated weights");
     const bool same = scores.data == scores_out.data && scores.stride[0] == scores_out.stride[0] && scores.stride[1] == scores_out.stride[1];
-    if (scores.data && !same && overlap(scores, 4, scores_out, 4)) reject("new accumulated weights must replace the old ones or lie apart from them");
+    const Region old_weights = region_of_scores(scores), new_weights = region_of_scores(scores_out);
+    if (!same) expect_apart(new_weights, {old_weights}, "new accumulated weights must replace the old ones or lie apart from them");
+    expect_apart(new_weights, {region_of_rows(q), region_of_cache(k), region_of_cache(v), region_of_lengths(lengths, k.shape[0])},
+                 "new accumulated weights must lie apart from queries, keys, values and lengths");
+    expect_apart(region_of_rows(out), {old_weights, new_weights}, "attention outputs must lie apart from accumulated weights");
     const size_t group = q.shape[1] / k.shape[2];
-    if (!scratch || !aligned16(scratch) ||
-        scratch_bytes < ei_attention_accumulate_scratch_bytes(k.shape[0], size_t(p.rows), q.shape[1], k.shape[2], k.shape[1]))
+    const size_t needed = ei_attention_accumulate_scratch_bytes(k.shape[0], size_t(p.rows), q.shape[1], k.shape[2], k.shape[1]);
+    if (!scratch || !aligned16(scratch) || scratch_bytes < needed)
       reject("attention with accumulated weights needs 16-byte aligned scratch of the size it names");
+    expect_apart(region_of(scratch, needed),
+                 {region_of_rows(q), region_of_cache(k), region_of_cache(v), region_of_lengths(lengths, k.shape[0]), region_of_rows(out),
+                  old_weights, new_weights},
+                 "scratch must lie apart from all else");
     expect_current_device(ctx);
     encode_maps(&p, keys, values);
     p.raw = static_cast<float*>(scratch);

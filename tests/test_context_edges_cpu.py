@@ -67,3 +67,41 @@ def test_rotated_heads_that_meet_other_arguments(elsewhere):
                   dict(q_out=call.view(3, 5, 4, 64, offset=64)), dict(k_out=call.view(3, 5, 2, 64, offset=99 * 256 - 16)),
                   dict(qw=call.view(4, 64, offset=128)), dict(positions=call.view(5, 5).data + 1264)):
         refused(call, go(**fault), says="lie apart")
+
+
+def test_attention_outputs_that_meet_other_arguments(elsewhere):
+    """Every attention, with everything apart, with outputs in the queries' place, and with one argument over another."""
+    call, lib, ctx = elsewhere, elsewhere.lib, C.byref(elsewhere.ctx)
+    view = call.view
+    prefix_bytes = lib.ei_attention_shared_prefix_scratch_bytes(6, 8, 2, 33)
+    scratch_bytes = lib.ei_attention_accumulate_scratch_bytes(2, 3, 8, 2, 70)
+
+    def every(q=view(1, 6, 8, 128), k=view(2, 2, 70, 2, 128), v=view(3, 2, 70, 2, 128), out=view(4, 6, 8, 128), lengths=1 << 33,
+              scores=view(5, 2, 2, 70), scores_out=view(6, 2, 2, 70), pk=view(7, 33, 2, 128), pv=view(8, 33, 2, 128), scratch=view(9, 1).data):
+        first = (q, k, v, out, lengths, 0)
+        return {"window": lambda: lib.ei_attention_window_bf16(ctx, *first, 16, 0),
+                "prefix": lambda: lib.ei_attention_shared_prefix_bf16(ctx, q, pk, pv, k, v, out, lengths, 0, scratch, prefix_bytes),
+                "accumulate": lambda: lib.ei_attention_accumulate_bf16(ctx, *first, scores, scores_out, scratch, scratch_bytes)}
+
+    side = lambda place: view(2, 2, 70, 2, 128, stride=(70 * 512, 512, 128, 1), offset=512 * place)  # keys and values of a token adjacent
+    wide = lambda first: view(4, 6, 8, 128, stride=(2048, 128, 1), offset=2048 * first)
+    for fine in (dict(), dict(out=view(1, 6, 8, 128)), dict(k=side(0), v=side(1)), dict(v=view(2, 2, 70, 2, 128)), dict(q=wide(0), out=wide(1)),
+                 dict(scores=view(6, 2, 2, 70)), dict(pk=view(2, 33, 2, 128)), dict(scores=call.abi.View3())):
+        for go in every(**fine).values():
+            accepted(call, go())
+    everywhere, some = ("window", "prefix", "accumulate"), ("prefix", "accumulate")
+    row, token = 2048, 512  # bytes
+    for names, fault in [(everywhere, dict(out=view(1, 6, 8, 128, offset=row))), (everywhere, dict(out=view(1, 6, 8, 128, stride=(2048, 128, 1)))),
+                         (everywhere, dict(q=wide(0), out=view(4, 6, 8, 128, stride=(2048, 128, 1), offset=2032))),
+                         (everywhere, dict(out=view(2, 6, 8, 128, offset=140 * token - 16))), (everywhere, dict(out=view(3, 6, 8, 128))),
+                         (everywhere, dict(lengths=view(4, 1).data + 6 * row - 4)), (("prefix",), dict(out=view(7, 6, 8, 128))),
+                         (("prefix",), dict(out=view(8, 6, 8, 128))), (some, dict(scratch=view(4, 1).data)), (some, dict(scratch=view(1, 1).data)),
+                         (some, dict(scratch=view(2, 1).data)), (some, dict(scratch=view(3, 1).data)), (some, dict(lengths=view(9, 1).data)),
+                         (("prefix",), dict(scratch=view(7, 1).data)), (("prefix",), dict(scratch=view(8, 1).data)),
+                         (("accumulate",), dict(scratch=view(5, 1).data)), (("accumulate",), dict(scratch=view(6, 1).data)),
+                         (("accumulate",), dict(out=view(5, 6, 8, 128))), (("accumulate",), dict(out=view(6, 6, 8, 128))),
+                         (("accumulate",), dict(scores_out=view(1, 2, 2, 70))), (("accumulate",), dict(scores_out=view(2, 2, 2, 70))),
+                         (("accumulate",), dict(scores_out=view(3, 2, 2, 70))), (("accumulate",), dict(scores=view(6, 2, 2, 70, stride=(150, 70, 1)))),
+                         (("accumulate",), dict(lengths=view(6, 1).data))]:
+        for name in names:
+            refused(call, every(**fault)[name](), says="lie apart")
