@@ -29,19 +29,6 @@ void expect_current_device(const ei_context* ctx) {
   if (device != ctx->device) reject("the execution context belongs to another CUDA device than the current one");
 }
 
-// Elements from a view's first to its last.
-template <typename View>
-size_t extent_of(const View& v) {
-  size_t last = 0;
-  for (int axis = 0; axis < rank_of(v); ++axis) last += (v.shape[axis] - 1) * v.stride[axis];
-  return last + 1;
-}
-template <typename A, typename B>
-bool overlap(const A& a, size_t a_size, const B& b, size_t b_size) {
-  const uintptr_t a0 = reinterpret_cast<uintptr_t>(a.data), b0 = reinterpret_cast<uintptr_t>(b.data);
-  return a0 < b0 + extent_of(b) * b_size && b0 < a0 + extent_of(a) * a_size;
-}
-
 // `out` is written while others read or write the rest.
 void expect_apart(const Region& out, std::initializer_list<Region> others, const char* what) {
   for (const Region& other : others)
@@ -432,11 +419,13 @@ ei_status ei_evict_kv_bf16(const ei_context* ctx, ei_view4 k, ei_view4 v, ei_vie
     if (sinks > budget || recent > budget - sinks) reject("first and latest tokens must fit the budget");
     if (!lengths && length > k.shape[1]) reject("the length exceeds the caches' capacity");
     if (!lengths_out || lengths_out == lengths) reject("new lengths need storage of their own");
-    for (const ei_view4* from : {&k, &v})
-      for (const ei_view4* to : {&k_out, &v_out})
-        if (overlap(*from, 2, *to, 2)) reject("kept keys and values must lie apart from the cached ones");
-    if (overlap(k_out, 2, v_out, 2) && k_out.data == v_out.data) reject("kept keys and values must not share storage");
-    if (overlap(scores, 4, scores_out, 4)) reject("kept weights must lie apart from the accumulated ones");
+    const Region from[] = {region_of_cache(k), region_of_cache(v), region_of_scores(scores), region_of_lengths(lengths, sequences)};
+    const Region to[] = {region_of_cache(k_out), region_of_cache(v_out), region_of_scores(scores_out), region_of_scores(kept),
+                         region_of_lengths(lengths_out, sequences)};
+    for (const Region& out : to)
+      expect_apart(out, {from[0], from[1], from[2], from[3]}, "kept keys, values, weights, positions and lengths must lie apart from all inputs");
+    for (int i = 0; i < 5; ++i)
+      for (int j = 0; j < i; ++j) expect_apart(to[i], {to[j]}, "kept keys, values, weights, positions and lengths must not share storage, but lie apart");
     p.k_out = const_cast<bf16*>(k_to.data), p.k_out_token = k_to.token, p.k_out_head = k_to.head, p.k_out_sequence = k_to.sequence;
     p.v_out = const_cast<bf16*>(v_to.data), p.v_out_token = v_to.token, p.v_out_head = v_to.head, p.v_out_sequence = v_to.sequence;
     p.scores = static_cast<const float*>(scores.data);

@@ -105,3 +105,28 @@ def test_attention_outputs_that_meet_other_arguments(elsewhere):
                          (("accumulate",), dict(lengths=view(6, 1).data))]:
         for name in names:
             refused(call, every(**fault)[name](), says="lie apart")
+
+
+def test_evicted_outputs_that_meet_other_arguments(elsewhere):
+    call, view = elsewhere, elsewhere.view
+
+    def go(k=view(1, 2, 90, 4, 128), v=view(2, 2, 90, 4, 128), scores=view(3, 2, 4, 90), lengths=view(8, 1).data, k_out=view(4, 2, 32, 4, 128),
+           v_out=view(5, 2, 32, 4, 128), scores_out=view(6, 2, 4, 32), kept=view(7, 2, 4, 32), lengths_out=view(9, 1).data):
+        return call.lib.ei_evict_kv_bf16(C.byref(call.ctx), k, v, scores, lengths, 0, 4, 8, k_out, v_out, scores_out, kept, lengths_out)
+
+    side = lambda at, tokens, place: view(at, 2, tokens, 4, 128, stride=(tokens * 1024, 1024, 128, 1), offset=1024 * place)
+    both = lambda place: view(6, 2, 4, 32, stride=(256, 64, 1), offset=128 * place)  # weights and positions of a head adjacent
+    for fine in (dict(), dict(k=side(1, 90, 0), v=side(1, 90, 1), k_out=side(4, 32, 0), v_out=side(4, 32, 1)),
+                 dict(scores_out=both(0), kept=both(1)), dict(lengths=view(9, 1).data + 8),
+                 dict(k=view(1, 2, 90, 4, 128, stride=(200 * 512, 512, 128, 1)), k_out=view(1, 2, 32, 4, 128, stride=(200 * 512, 512, 128, 1), offset=90 * 1024))):
+        accepted(call, go(**fine))
+    outputs = dict(k_out=lambda *a, **o: view(a[0], 2, 32, 4, 128, **o), v_out=lambda *a, **o: view(a[0], 2, 32, 4, 128, **o),
+                   scores_out=lambda *a, **o: view(a[0], 2, 4, 32, **o), kept=lambda *a, **o: view(a[0], 2, 4, 32, **o),
+                   lengths_out=lambda *a, **o: view(a[0], 1, **o).data)
+    own = dict(k_out=4, v_out=5, scores_out=6, kept=7, lengths_out=9)
+    for name, make in outputs.items():
+        for place in (1, 2, 3, 8, *(at for other, at in own.items() if other != name)):
+            refused(call, go(**{name: make(place)}), says="new lengths" if (name, place) == ("lengths_out", 8) else "lie apart")
+    refused(call, go(v_out=side(4, 32, 1)), says="lie apart")
+    refused(call, go(lengths_out=view(8, 1).data + 4), says="lie apart")
+    refused(call, go(lengths_out=view(8, 1).data - 4), says="lie apart")
