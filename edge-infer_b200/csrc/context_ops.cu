@@ -78,6 +78,8 @@ void expect_scores(const ei_view3& v, size_t sequences, size_t kv_heads, size_t 
     reject(std::string(name) + " must be [sequences, kv_heads, tokens]");
   if ((tokens > 1 && v.stride[2] != 1) || (kv_heads > 1 && v.stride[1] < tokens) || (sequences > 1 && v.stride[0] < tokens))
     reject(std::string(name) + " must be packed along its tokens, rows apart");
+  if ((kv_heads > 1 && v.stride[1] > (size_t(1) << 40)) || (sequences > 1 && v.stride[0] > (size_t(1) << 40)))
+    reject(std::string(name) + " has rows too far apart");
   if (reinterpret_cast<uintptr_t>(v.data) & 3) reject(std::string(name) + " must be 4-byte aligned");
 }
 
@@ -366,6 +368,7 @@ ei_status ei_attention_accumulate_bf16(const ei_context* ctx, ei_view3 q, ei_vie
     if (scores.data) expect_scores(scores, k.shape[0], k.shape[2], k.shape[1], "accumulated weights");
     expect_scores(scores_out, k.shape[0], k.shape[2], k.shape[1], "new accumulated weights");
     const bool same = scores.data == scores_out.data && scores.stride[0] == scores_out.stride[0] && scores.stride[1] == scores_out.stride[1];
+    if (may_fold(region_of_scores(scores_out))) reject("new accumulated weights must have storage for every token of every head");
     const Region old_weights = region_of_scores(scores), new_weights = region_of_scores(scores_out);
     if (!same) expect_apart(new_weights, {old_weights}, "new accumulated weights must replace the old ones or lie apart from them");
     expect_apart(new_weights, {region_of_rows(q), region_of_cache(k), region_of_cache(v), region_of_lengths(lengths, k.shape[0])},
@@ -424,6 +427,8 @@ ei_status ei_evict_kv_bf16(const ei_context* ctx, ei_view4 k, ei_view4 v, ei_vie
                          region_of_lengths(lengths_out, sequences)};
     for (const Region& out : to)
       expect_apart(out, {from[0], from[1], from[2], from[3]}, "kept keys, values, weights, positions and lengths must lie apart from all inputs");
+    for (int i = 0; i < 4; ++i)
+      if (may_fold(to[i])) reject("kept keys, values, weights and positions must have storage for every token of every head");
     for (int i = 0; i < 5; ++i)
       for (int j = 0; j < i; ++j) expect_apart(to[i], {to[j]}, "kept keys, values, weights, positions and lengths must not share storage, but lie apart");
     p.k_out = const_cast<bf16*>(k_to.data), p.k_out_token = k_to.token, p.k_out_head = k_to.head, p.k_out_sequence = k_to.sequence;

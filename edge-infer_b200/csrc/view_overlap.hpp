@@ -56,4 +56,21 @@ inline bool may_meet(const Region& a, const Region& b) {
   return true;
 }
 
+// False only where no two items meet because every axis steps over all that shorter steps reach.
+inline bool may_fold(const Region& r) {
+  unsigned __int128 reach = r.item;
+  bool taken[4] = {};
+  for (int i = 0; i < r.rank; ++i) {
+    int shortest = -1;
+    for (int axis = 0; axis < r.rank; ++axis)
+      if (!taken[axis] && (shortest < 0 || r.step[axis] < r.step[shortest])) shortest = axis;
+    taken[shortest] = true;
+    // An axis of one is not stepped along: where it comes in the order does not matter.
+    if (r.count[shortest] <= 1) continue;
+    if (r.step[shortest] < reach) return true;
+    reach += (unsigned __int128)(r.count[shortest] - 1) * r.step[shortest];
+  }
+  return false;
+}
+
 }  // namespace ei

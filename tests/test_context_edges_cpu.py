@@ -130,3 +130,42 @@ def test_evicted_outputs_that_meet_other_arguments(elsewhere):
     refused(call, go(v_out=side(4, 32, 1)), says="lie apart")
     refused(call, go(lengths_out=view(8, 1).data + 4), says="lie apart")
     refused(call, go(lengths_out=view(8, 1).data - 4), says="lie apart")
+
+
+def test_views_that_may_fold(tmp_path):
+    fold = run_choice(tmp_path, "view_overlap.hpp", 'ei::Region g{64, (size_t)atoll(a[1]), 3, {}, {}}; for (int i = 0; i < 3; ++i) '
+                      'g.count[i] = atoll(a[2 + 2 * i]), g.step[i] = atoll(a[3 + 2 * i]); std::printf("%d", int(ei::may_fold(g)));')
+    for item, axes in itertools.product((1, 4), itertools.product([(1, 0), (2, 4), (3, 4), (2, 12), (3, 8), (2, 0), (4, 48)], repeat=3)):
+        flat = [x for axis in axes for x in axis]
+        every = [sum(i * step for i, (_, step) in zip(at, axes)) + x for at in itertools.product(*(range(n) for n, _ in axes)) for x in range(item)]
+        folded = fold(item, *flat)[0]
+        assert folded or len(set(every)) == len(every)
+    # Packed in any order of the axes, and with gaps.
+    for order in itertools.permutations([(2, 256), (3, 512), (5, 2000)]):
+        assert fold(256, *(x for axis in order for x in axis)) == [0]
+    assert fold(256, 2, 2 ** 63, 3, 2 ** 63, 1, 0) == [1]
+
+
+def test_outputs_that_meet_themselves(elsewhere):
+    """Heads or sequences of an output that share tokens' storage: two writers of one place."""
+    call, view, ctx = elsewhere, elsewhere.view, C.byref(elsewhere.ctx)
+    size = call.lib.ei_attention_accumulate_scratch_bytes(2, 3, 8, 2, 70)
+
+    def accumulate(scores_out):
+        return call.lib.ei_attention_accumulate_bf16(ctx, view(1, 6, 8, 128), view(2, 2, 70, 2, 128), view(3, 2, 70, 2, 128), view(4, 6, 8, 128), None, 70,
+                                                     call.abi.View3(), scores_out, view(6, 1).data, size)
+
+    accepted(call, accumulate(view(5, 2, 2, 70, stride=(72, 200, 1))))
+    refused(call, accumulate(view(5, 2, 2, 70, stride=(70, 70, 1))), says="storage for every")
+    refused(call, accumulate(view(5, 2, 2, 70, stride=(100, 140, 1))), says="storage for every")
+
+    refused(call, accumulate(view(5, 2, 2, 70, stride=(2 ** 62, 70, 1))), says="too far apart")
+
+    def evict(k_out=view(4, 2, 32, 4, 128), v_out=view(5, 2, 32, 4, 128), scores_out=view(6, 2, 4, 32), kept=view(7, 2, 4, 32)):
+        return call.lib.ei_evict_kv_bf16(ctx, view(1, 2, 90, 4, 128), view(2, 2, 90, 4, 128), view(3, 2, 4, 90), None, 90, 4, 8, k_out, v_out,
+                                         scores_out, kept, view(9, 1).data)
+
+    accepted(call, evict(k_out=view(4, 2, 32, 4, 128, stride=(32 * 128, 128, 64 * 128, 1))))
+    for fault in (dict(k_out=view(4, 2, 32, 4, 128, stride=(32 * 512, 128, 128, 1))), dict(v_out=view(5, 2, 32, 4, 128, stride=(512, 512, 128, 1))),
+                  dict(scores_out=view(6, 2, 4, 32, stride=(32, 32, 1))), dict(kept=view(7, 2, 4, 32, stride=(64, 32, 1)))):
+        refused(call, evict(**fault), says="storage for every")
