@@ -37,6 +37,10 @@ void expect_apart(const Region& out, std::initializer_list<Region> others, const
 Region region_of_rows(const ei_view3& v) { return region_of(v, sizeof(bf16), 2); }
 Region region_of_cache(const ei_view4& v) { return region_of(v, sizeof(bf16), 1); }
 Region region_of_scores(const ei_view3& v) { return region_of(v, sizeof(float), 1); }
+// Values in device memory that the kernels read or write one by one; null is the caller's to look at.
+void expect_integers(const int32_t* values, const char* name) {
+  if (reinterpret_cast<uintptr_t>(values) & 3) reject(std::string(name) + " must be 4-byte aligned");
+}
 Region region_of_lengths(const int32_t* lengths, size_t sequences) { return region_of(lengths, sequences * sizeof(int32_t)); }
 
 // [rows, heads, width]: heads of a row adjacent, rows 16-byte aligned and disjoint.
@@ -101,6 +105,7 @@ StepAttentionParams attention_of(const ei_view3& q, const ei_view4& k, const ei_
   if (rows > kMostTokens / group || (rows * group + kStepRows - 1) / kStepRows > 65535) reject("too many query rows");
   if (q.shape[0] > (size_t(1) << 31) / q.shape[1]) reject("too many query rows");
   if (!lengths && length > k.shape[1]) reject("the length exceeds the caches' capacity");
+  expect_integers(lengths, "lengths");
   // A row's queries are read by the blocks that write it and, as part of their boxes, by others that do not use them.
   if (q.data != out.data || row_stride(q) != row_stride(out))
     expect_apart(region_of_rows(out), {region_of_rows(q)}, "attention outputs must be the queries' own view or lie apart from them");
@@ -218,6 +223,7 @@ ei_status ei_qk_norm_rope_bf16(const ei_context* ctx, ei_view3 q, ei_view3 k, ei
     if (rotary % 16 || rotary > width) reject("the rotated width must be a multiple of 16 within the head");
     if (!aligned16(table.data)) reject("the RoPE table must be 16-byte aligned");
     const int table_rows = kernel_extent(table.shape[0], "RoPE positions");
+    expect_integers(positions, "positions");
     if (!positions && (offset > table.shape[0] || rows > table.shape[0] - offset))
       throw std::out_of_range("RoPE positions exceed the table");
     for (const ei_view1* weight : {&q_weight, &k_weight}) {
@@ -421,6 +427,8 @@ ei_status ei_evict_kv_bf16(const ei_context* ctx, ei_view4 k, ei_view4 v, ei_vie
     expect_scores(kept, sequences, kv_heads, budget, "kept positions");
     if (sinks > budget || recent > budget - sinks) reject("first and latest tokens must fit the budget");
     if (!lengths && length > k.shape[1]) reject("the length exceeds the caches' capacity");
+    expect_integers(lengths, "lengths");
+    expect_integers(lengths_out, "new lengths");
     if (!lengths_out || lengths_out == lengths) reject("new lengths need storage of their own");
     const Region from[] = {region_of_cache(k), region_of_cache(v), region_of_scores(scores), region_of_lengths(lengths, sequences)};
     const Region to[] = {region_of_cache(k_out), region_of_cache(v_out), region_of_scores(scores_out), region_of_scores(kept),

@@ -169,3 +169,19 @@ def test_outputs_that_meet_themselves(elsewhere):
     for fault in (dict(k_out=view(4, 2, 32, 4, 128, stride=(32 * 512, 128, 128, 1))), dict(v_out=view(5, 2, 32, 4, 128, stride=(512, 512, 128, 1))),
                   dict(scores_out=view(6, 2, 4, 32, stride=(32, 32, 1))), dict(kept=view(7, 2, 4, 32, stride=(64, 32, 1)))):
         refused(call, evict(**fault), says="storage for every")
+
+
+def test_integers_in_device_memory_are_aligned(elsewhere):
+    """A kernel that read them from an odd address would fault."""
+    call, view, lib, ctx = elsewhere, elsewhere.view, elsewhere.lib, C.byref(elsewhere.ctx)
+    q, k, v, out, odd = view(1, 6, 8, 128), view(2, 2, 70, 2, 128), view(3, 2, 70, 2, 128), view(4, 6, 8, 128), view(9, 1).data + 2
+    prefix, scores, none = view(5, 33, 2, 128), view(6, 2, 2, 70), call.abi.View1()
+    refused(call, lib.ei_attention_window_bf16(ctx, q, k, v, out, odd, 0, 16, 0), says="aligned")
+    refused(call, lib.ei_attention_shared_prefix_bf16(ctx, q, prefix, prefix, k, v, out, odd, 0, 1 << 30, 1 << 26), says="aligned")
+    refused(call, lib.ei_attention_accumulate_bf16(ctx, q, k, v, out, odd, 0, scores, scores, 1 << 30, 1 << 26), says="aligned")
+    keys = view(1, 5, 2, 64)
+    refused(call, lib.ei_qk_norm_rope_bf16(ctx, keys, keys, view(3, 99, 64), odd, 0, none, none, 1e-6, 0, view(4, 5, 2, 64), view(5, 5, 2, 64)),
+            says="aligned")
+    for lengths, lengths_out in ((odd, 1 << 33), (None, odd)):
+        refused(call, lib.ei_evict_kv_bf16(ctx, k, v, scores, lengths, 70, 4, 8, view(10, 2, 32, 2, 128), view(11, 2, 32, 2, 128), view(12, 2, 2, 32),
+                                           view(13, 2, 2, 32), lengths_out), says="aligned")
