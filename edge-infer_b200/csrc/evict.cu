@@ -8,6 +8,7 @@
 // memory) instead of waiting for one another, and then move a part of the rows each. 64 caches of 2304 tokens and 8 heads to 2048:
 // 176 us = 6.07 TB/s; one of 8191 to 1024: 13.7 us (46 with the place-th key found two bits a step by counting all keys).
 #include "context_kernels.cuh"
+#include "per_device.hpp"
 
 #include <algorithm>
 
@@ -189,14 +190,14 @@ void launch_evict(const EvictParams& p, int multiprocessors, cudaStream_t stream
   parts = std::max(parts, (p.budget + 8191) / 8192);
   const int part_rows = (p.budget + parts - 1) / parts;
   const size_t shared = sizeof(EvictShared) + size_t(part_rows) * 4 + size_t(cached) * 4;
-  static thread_local int configured_device = -1;
+  static PerDevice<bool> devices;
   int device = 0;
   EI_CUDA(cudaGetDevice(&device));
-  if (configured_device != device) {
+  devices.get(device, [] {
     EI_CUDA(cudaFuncSetAttribute(evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  int(sizeof(EvictShared) + (8192 + kCachedKeys) * 4)));
-    configured_device = device;
-  }
+    return true;
+  });
   launch(evict_kernel, dim3(unsigned((p.budget + part_rows - 1) / part_rows), unsigned(p.kv_heads), unsigned(p.sequences)), dim3(kThreads),
          shared, stream, false, p, cached, part_rows);
 }

@@ -32,6 +32,7 @@
 #include "span_attention.cuh"
 
 #include "cluster.cuh"
+#include "per_device.hpp"
 #include "prompt_attention.cuh"
 
 #include <algorithm>
@@ -611,13 +612,13 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
 }  // namespace
 
 void launch_span_attention(const SpanAttentionParams& given, cudaStream_t stream) {
-  static thread_local int configured_device = -1;
+  static PerDevice<bool> devices;
   int device = 0;
   EI_CUDA(cudaGetDevice(&device));
-  if (configured_device != device) {
+  devices.get(device, [] {
     EI_CUDA(cudaFuncSetAttribute(span_attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSpanSharedBytes)));
-    configured_device = device;
-  }
+    return true;
+  });
   SpanAttentionParams p = given;
   const int group = p.heads / p.kv_heads;
   const long long all_rows = (long long)p.rows * p.sequences;

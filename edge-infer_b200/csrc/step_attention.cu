@@ -24,6 +24,7 @@
 #include "step_attention.cuh"
 
 #include "cluster.cuh"
+#include "per_device.hpp"
 #include "span_choice.hpp"
 #include "step_choice.hpp"
 
@@ -610,26 +611,26 @@ cudaLaunchConfig_t step_config(const StepShape& shape, bool two, unsigned heads,
 
 // Sets the kernels up on the current device and says how many clusters it runs at once.
 const StepCapacity& configure_step_kernels() {
-  static thread_local int configured_device = -1;
-  static thread_local StepCapacity capacity;
+  static PerDevice<StepCapacity> devices;
   int device = 0;
   EI_CUDA(cudaGetDevice(&device));
-  if (configured_device == device) return capacity;
-  for (const int warps : {4, 8}) {
-    for (const bool two : {false, true})
-      for (const bool weights : {false, true}) {
-        EI_CUDA(cudaFuncSetAttribute(step_kernel(warps, two, weights), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     int(step_shared(warps, two ? 2 : 1))));
-        EI_CUDA(cudaFuncSetAttribute(step_kernel(warps, two, weights), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  return devices.get(device, [] {
+    StepCapacity capacity;
+    for (const int warps : {4, 8}) {
+      for (const bool two : {false, true})
+        for (const bool weights : {false, true}) {
+          EI_CUDA(cudaFuncSetAttribute(step_kernel(warps, two, weights), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       int(step_shared(warps, two ? 2 : 1))));
+          EI_CUDA(cudaFuncSetAttribute(step_kernel(warps, two, weights), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        }
+      for (int power = 0; power < 5; ++power) {
+        cudaLaunchAttribute cluster{};
+        const cudaLaunchConfig_t config = step_config({1 << power, warps}, true, 64, 1, 1, &cluster);
+        EI_CUDA(cudaOccupancyMaxActiveClusters(&(warps == 4 ? capacity.four : capacity.eight)[power], step_kernel(warps, true, true), &config));
       }
-    for (int power = 0; power < 5; ++power) {
-      cudaLaunchAttribute cluster{};
-      const cudaLaunchConfig_t config = step_config({1 << power, warps}, true, 64, 1, 1, &cluster);
-      EI_CUDA(cudaOccupancyMaxActiveClusters(&(warps == 4 ? capacity.four : capacity.eight)[power], step_kernel(warps, true, true), &config));
     }
-  }
-  configured_device = device;
-  return capacity;
+    return capacity;
+  });
 }
 
 }  // namespace

@@ -1,10 +1,11 @@
 """CPU checks of what the operators for long contexts refuse: outputs that meet other arguments in memory."""
 import ctypes as C
 import itertools
+import subprocess
 
 import pytest
 
-from test_context_cpu import Call, call, refused, run_choice  # noqa: F401
+from test_context_cpu import ROOT, call, refused, run_choice  # noqa: F401
 
 
 def accepted(call, status):
@@ -185,3 +186,40 @@ def test_integers_in_device_memory_are_aligned(elsewhere):
     for lengths, lengths_out in ((odd, 1 << 33), (None, odd)):
         refused(call, lib.ei_evict_kv_bf16(ctx, k, v, scores, lengths, 70, 4, 8, view(10, 2, 32, 2, 128), view(11, 2, 32, 2, 128), view(12, 2, 2, 32),
                                            view(13, 2, 2, 32), lengths_out), says="aligned")
+
+
+def test_set_up_once_per_device(tmp_path):
+    """Threads that take devices in turn set each of them up once; a set-up that fails is tried again."""
+    source = tmp_path / "devices.cpp"
+    source.write_text('''#include "per_device.hpp"
+#include <atomic>
+#include <cstdio>
+#include <stdexcept>
+#include <thread>
+#include <vector>
+int main() {
+  static ei::PerDevice<int> devices;
+  std::atomic<int> made{0}, wrong{0};
+  int failed = 0;
+  try { devices.get(9, []() -> int { throw std::runtime_error("no"); }); } catch (const std::runtime_error&) { ++failed; }
+  std::vector<std::thread> threads;
+  for (int t = 0; t < 8; ++t)
+    threads.emplace_back([&] {
+      for (int i = 0; i < 1000; ++i) {
+        const int device = i % 2 ? 3 : 9;
+        if (devices.get(device, [&] { ++made; return 10 * device; }) != 10 * device) ++wrong;
+      }
+    });
+  for (auto& t : threads) t.join();
+  std::printf("%d %d %d", failed, made.load(), wrong.load());
+}
+''')
+    program = tmp_path / "devices"
+    subprocess.run(["g++", "-std=c++17", "-pthread", "-I", str(ROOT / "edge-infer_b200" / "csrc"), "-o", str(program), str(source)], check=True)
+    assert subprocess.run([str(program)], check=True, capture_output=True, text=True).stdout == "1 2 0"
+
+
+def test_kernels_for_long_contexts_are_set_up_per_device_not_per_thread():
+    for name in ("step_attention.cu", "span_attention.cu", "evict.cu"):
+        text = (ROOT / "edge-infer_b200" / "csrc" / name).read_text()
+        assert "thread_local" not in text and "PerDevice" in text
