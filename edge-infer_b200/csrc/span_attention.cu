@@ -195,7 +195,10 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem = sh->tmem_base;
-  if (p.together) grid_launch_dependents();  // launched in plain stream order: all that came before has completed
+  if (p.together) {  // launched in plain stream order: the wait is over at once
+    grid_dependency_wait();
+    grid_launch_dependents();
+  }
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (mbarrier_test_wait(bar, parity)) return true;
     for (uint32_t polls = 0; polls < kTmaWaitLimit; ++polls) {

@@ -131,7 +131,10 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
     for (int i = 0; i < kBuffers; ++i) request(i);
   }
   __syncwarp();
-  if (p.partial) grid_launch_dependents();  // this kernel follows nothing early; what joins its results waits for them
+  if (p.partial) {  // launched in plain stream order: the wait is over at once
+    grid_dependency_wait();
+    grid_launch_dependents();
+  }
 
   if (kRowTiles > 1) {
     for (int i = threadIdx.x; i < kStepRows * 16; i += kThreads) {

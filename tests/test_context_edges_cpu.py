@@ -223,3 +223,12 @@ def test_kernels_for_long_contexts_are_set_up_per_device_not_per_thread():
     for name in ("step_attention.cu", "span_attention.cu", "evict.cu"):
         text = (ROOT / "edge-infer_b200" / "csrc" / name).read_text()
         assert "thread_local" not in text and "PerDevice" in text
+
+
+def test_kernels_trigger_their_dependents_behind_their_own_wait():
+    """The rule of common.cuh, kernel by kernel: what a successor runs before its wait relies on it."""
+    for path in sorted((ROOT / "edge-infer_b200" / "csrc").glob("*.cu*")):
+        for kernel in path.read_text().split("__global__")[1:]:
+            trigger = kernel.find("grid_launch_dependents();")
+            if trigger >= 0:
+                assert 0 <= kernel.find("grid_dependency_wait();") < trigger, (path.name, kernel[:80])
