@@ -87,6 +87,15 @@ void expect_scores(const ei_view3& v, size_t sequences, size_t kv_heads, size_t 
   if (reinterpret_cast<uintptr_t>(v.data) & 3) reject(std::string(name) + " must be 4-byte aligned");
 }
 
+// Test hook: poll limit for the next attention that this thread calls (0: none is armed).
+thread_local uint32_t injected_polls = 0;
+void take_injected(StepAttentionParams* p) {
+  if (!injected_polls) return;
+  p->wait_limit = injected_polls;
+  p->fault_tx = 16;
+  injected_polls = 0;
+}
+
 // What every attention of this file checks and fills in: queries [sequences * rows, heads, 128] over caches.
 StepAttentionParams attention_of(const ei_view3& q, const ei_view4& k, const ei_view4& v, const ei_view3& out, const int32_t* lengths,
                                  size_t length, CacheStrides* keys, CacheStrides* values) {
@@ -136,6 +145,7 @@ SpanAttentionParams span_of(const StepAttentionParams& p, const CacheStrides& ke
   SpanAttentionParams s{};
   s.q = p.q, s.q_stride = p.q_stride, s.out = p.out, s.out_stride = p.out_stride;
   s.rows = p.rows, s.heads = p.heads, s.kv_heads = p.kv_heads, s.sequences = p.sequences, s.capacity = p.capacity;
+  s.wait_limit = p.wait_limit, s.fault_tx = p.fault_tx;
   s.lengths = p.lengths, s.length = p.length, s.window = p.window, s.sinks = p.sinks, s.together = p.together;
   encode_cache_map(&s.k_map, keys, size_t(p.capacity), size_t(p.kv_heads), size_t(p.sequences), kSpanBox, 1);
   encode_cache_map(&s.v_map, values, size_t(p.capacity), size_t(p.kv_heads), size_t(p.sequences), kSpanBox, 1);
@@ -276,6 +286,7 @@ ei_status ei_attention_window_bf16(const ei_context* ctx, ei_view3 q, ei_view4 k
     p.window = int(std::min(window, kMostTokens));
     p.sinks = int(std::min(sinks, kMostTokens));
     expect_current_device(ctx);
+    take_injected(&p);
     const size_t group = size_t(p.heads / p.kv_heads), stacked = size_t(p.rows) * group;
     // Whichever kernel is the faster by its estimate; the tensor-core kernel's query tiles have 128 rows.
     auto seen_by = [&](size_t rows) { return std::min(most_tokens(p), size_t(p.window) + size_t(p.sinks) + rows); };
@@ -293,6 +304,10 @@ ei_status ei_attention_window_bf16(const ei_context* ctx, ei_view3 q, ei_view4 k
     const size_t seen = seen_by(kStepRows);
     launch_step_attention(p, seen, stream, false);
   });
+}
+
+ei_status ei_context_inject_wait_timeout(uint32_t polls) {
+  return guarded([&] { injected_polls = polls; });
 }
 
 size_t ei_attention_shared_prefix_scratch_bytes(size_t q_rows, size_t query_heads, size_t kv_heads, size_t prefix_length) {
@@ -328,8 +343,10 @@ ei_status ei_attention_shared_prefix_bf16(const ei_context* ctx, ei_view3 q, ei_
     }
     expect_current_device(ctx);
     encode_maps(&own, keys, values);
+    take_injected(&own);
     if (prefix) {
       StepAttentionParams first = own;
+      own.wait_limit = own.fault_tx = 0;  // of the call's first launch alone
       first.rows = int(q.shape[0]);
       first.sequences = 1;
       first.capacity = first.length = int(prefix);
@@ -390,6 +407,7 @@ ei_status ei_attention_accumulate_bf16(const ei_context* ctx, ei_view3 q, ei_vie
                  "scratch must lie apart from all else");
     expect_current_device(ctx);
     encode_maps(&p, keys, values);
+    take_injected(&p);
     p.raw = static_cast<float*>(scratch);
     p.raw_rows = raw_rows(size_t(p.rows), group);
     p.raw_stride = raw_stride(k.shape[1]);
@@ -404,6 +422,7 @@ ei_status ei_attention_accumulate_bf16(const ei_context* ctx, ei_view3 q, ei_vie
       p.groups = std::min(kStepWeightGroups, groups - p.first_group);
       launch_step_attention(p, most_tokens(p), stream, false);
       if (p.row_stats) launch_step_weights(p, most_tokens(p), stream);
+      p.wait_limit = p.fault_tx = 0;
       p.scores = p.scores_out;
       p.scores_sequence = p.out_sequence, p.scores_head = p.out_head;
     }

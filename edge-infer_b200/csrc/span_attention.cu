@@ -199,9 +199,10 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
     grid_dependency_wait();
     grid_launch_dependents();
   }
+  const uint32_t wait_limit = p.wait_limit ? p.wait_limit : kTmaWaitLimit;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (mbarrier_test_wait(bar, parity)) return true;
-    for (uint32_t polls = 0; polls < kTmaWaitLimit; ++polls) {
+    for (uint32_t polls = 0; polls < wait_limit; ++polls) {
       if (mbarrier_try_wait(bar, parity)) return true;
       if (sh->abort) return false;
     }
@@ -451,7 +452,8 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
           sh->query_tiles |= 1 << i;
         }
       if (most > 0) {
-        mbarrier_expect_tx(&sh->first, uint32_t(min(ahead, most)) * kBufferBytes);
+        const bool faulty = sequence == 0 && rank == blocks - 1;
+        mbarrier_expect_tx(&sh->first, uint32_t(min(ahead, most)) * kBufferBytes + (faulty ? p.fault_tx : 0));
         for (int i = 0; i < min(ahead, most); ++i) copy(p.k_tile_map, p.k_map, i, first_keys + i * kBufferBytes, &sh->first);
         sh->issued = 1;
       }
@@ -527,12 +529,12 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
   __syncthreads();
   if (sh->abort) {  // no role is left to raise it: block-uniform
     if (threadIdx.x == 0) {
-      for (uint32_t polls = 0; polls < kTmaWaitLimit && !mbarrier_try_wait(&sh->done, 0); ++polls) {
+      for (uint32_t polls = 0; polls < wait_limit && !mbarrier_try_wait(&sh->done, 0); ++polls) {
       }
       for (int i = 0; i < 2; ++i)
-        if (sh->query_tiles >> i & 1) mbarrier_wait(&sh->queries[i], 0);
-      if (sh->issued > 0) mbarrier_wait(&sh->first, 0);
-      for (int i = max(0, sh->issued - 1 - kStages); i < sh->issued - 1; ++i) mbarrier_wait(&sh->full[i % kStages], (i / kStages) & 1);
+        if (sh->query_tiles >> i & 1) mbarrier_wait(&sh->queries[i], 0, wait_limit);
+      if (sh->issued > 0) mbarrier_wait(&sh->first, 0, wait_limit);
+      for (int i = max(0, sh->issued - 1 - kStages); i < sh->issued - 1; ++i) mbarrier_wait(&sh->full[i % kStages], (i / kStages) & 1, wait_limit);
     }
     __syncthreads();
     if (live && !join) {

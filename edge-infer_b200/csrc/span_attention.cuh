@@ -24,6 +24,7 @@ struct SpanAttentionParams {
   SpanSplits splits;
   int cluster;  // blocks that share the tokens of two query tiles (of a stretch), joined through distributed shared memory
   float* partial;
+  uint32_t wait_limit, fault_tx;  // as StepAttentionParams
 };
 void launch_span_attention(const SpanAttentionParams& p, cudaStream_t stream);
 

@@ -63,6 +63,12 @@ __device__ __forceinline__ int tile_offset(int token, int chunk) {
 __device__ __forceinline__ int query_offset(int row, int chunk) {
   return (chunk >> 3) * (kStepRows * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
 }
+// The larger of two, not a number if either is none.
+__device__ __forceinline__ float fmaxf_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
 template <int kWarps, int kRowTiles, bool kWeights>
 __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attention_kernel(const __grid_constant__ StepAttentionParams p) {
   constexpr int kThreads = kWarps * 32;
@@ -114,6 +120,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
   const int tiles = sink_tiles + (max(0, end - low) + kStepTile - 1) / kStepTile;
   const int first_tile = int((long long)tiles * rank / splits), last_tile = int((long long)tiles * (rank + 1) / splits);
 
+  const uint32_t wait_limit = p.wait_limit ? p.wait_limit : kTmaWaitLimit;
   unsigned char* const ring = smem + warp * kBuffers * kBuffer;
   uint64_t* const full = sh->full[warp];
   auto start_of = [&](int tile) { return tile < sink_tiles ? tile * kStepTile : low + (tile - sink_tiles) * kStepTile; };
@@ -122,7 +129,8 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
     const int tile = first_tile + warp + (item >> 1) * kWarps;
     if (tile >= last_tile) return;
     uint64_t* bar = &full[item % kBuffers];
-    mbarrier_expect_tx(bar, kBuffer);
+    const bool faulty = item == 0 && warp == 0 && sequence == 0 && rank == splits - 1;  // which has a tile if any block has
+    mbarrier_expect_tx(bar, kBuffer + (faulty ? p.fault_tx : 0));
     tma_load_5d(ring + (item % kBuffers) * kBuffer, (item & 1) ? &p.v_map : &p.k_map, 0, start_of(tile), 0, kv_head, sequence, bar);
   };
   if (lane == 0) {
@@ -182,7 +190,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
   int item = 0, buffer = 0;
   uint32_t parity = 0;
   for (int tile = first_tile + warp; tile < last_tile; tile += kWarps) {
-    ok = __all_sync(0xffffffffu, mbarrier_wait(&full[buffer], parity));
+    ok = __all_sync(0xffffffffu, mbarrier_wait(&full[buffer], parity, wait_limit));
     if (!ok) break;
     const unsigned char* ks = ring + buffer * kBuffer;
     const int first = start_of(tile);
@@ -285,7 +293,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
 
     ++item;
     if (++buffer == kBuffers) buffer = 0, parity ^= 1;
-    ok = __all_sync(0xffffffffu, mbarrier_wait(&full[buffer], parity));
+    ok = __all_sync(0xffffffffu, mbarrier_wait(&full[buffer], parity, wait_limit));
     if (!ok) break;
     unsigned char* vs = ring + buffer * kBuffer;
     if (stop - first < kStepTile) {
@@ -318,15 +326,16 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
   }
   if (!ok) {
     // A copy did not arrive within the bound. Those requested are waited for (bounded) before their buffers are used for
-    // anything else, and the unit's rows come out as NaN.
+    // anything else, and the unit's rows come out as NaN. A maximum that is no number, which no scores make, says so to the
+    // other warps and blocks.
     if (lane == 0) {
       for (int i = item; i < item + kBuffers; ++i) {
-        if (first_tile + warp + (i >> 1) * kWarps < last_tile) mbarrier_wait(&full[i % kBuffers], (i / kBuffers) & 1);
+        if (first_tile + warp + (i >> 1) * kWarps < last_tile) mbarrier_wait(&full[i % kBuffers], (i / kBuffers) & 1, wait_limit);
       }
     }
     __syncwarp();
 #pragma unroll
-    for (int rt = 0; rt < kRowTiles; ++rt) l[rt][0] = l[rt][1] = __int_as_float(0x7fffffff), m[rt][0] = m[rt][1] = 0.0f;
+    for (int rt = 0; rt < kRowTiles; ++rt) l[rt][0] = l[rt][1] = m[rt][0] = m[rt][1] = __int_as_float(0x7fffffff);
   }
   grid_dependency_wait();  // what is joined below may be the preceding kernel's
 
@@ -360,7 +369,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
     const int i = e % kUnitRows;
     float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sh->maxima[w][i]);
+    for (int w = 0; w < kWarps; ++w) top = fmaxf_nan(top, sh->maxima[w][i]);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float part = sh->sums[w][i];
@@ -402,9 +411,9 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
   if (threadIdx.x < kUnitRows) {
     const int i = threadIdx.x, count = sh->others[i];
     float top = -INFINITY;
-    for (uint32_t r = 0; r < splits; ++r) top = fmaxf(top, sh->blocks[r][i].x);
+    for (uint32_t r = 0; r < splits; ++r) top = fmaxf_nan(top, sh->blocks[r][i].x);
 #pragma unroll 4
-    for (int j = 0; j < count; ++j) top = fmaxf(top, others[j][i].x);
+    for (int j = 0; j < count; ++j) top = fmaxf_nan(top, others[j][i].x);
     sh->top[i] = top;
   }
   __syncthreads();
@@ -430,7 +439,8 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
     const float inverse = count < 0 || sum == 0.0f ? 0.0f : p.partial ? sum : 1.0f / sum;
     sh->inverse[i] = inverse;
     if (kWeights && p.row_stats && rank == 0 && i < have)
-      p.row_stats[(size_t(sequence) * p.kv_heads + kv_head) * p.raw_rows + size_t(blockIdx.z) * kStepRows + i] = make_float2(sh->top[i], inverse);
+      p.row_stats[(size_t(sequence) * p.kv_heads + kv_head) * p.raw_rows + size_t(blockIdx.z) * kStepRows + i] =
+          make_float2(sh->top[i], sh->top[i] != sh->top[i] ? 0.0f : inverse);
   }
   __syncthreads();
   {
@@ -517,7 +527,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
         for (int i = 0; i < 4; ++i) {
           if (i0 + i >= have) break;
           const float inverse = sh->inverse[i0 + i], top = sh->top[i0 + i];
-          if (inverse == 0.0f) continue;
+          if (inverse == 0.0f || top != top) continue;  // a row that gave up adds nothing
 #pragma unroll
           for (int u = 0; u < kQuads; ++u) {
             sum[u][0] = fmaf(power_of_two(score[i][u].x - top), inverse, sum[u][0]);

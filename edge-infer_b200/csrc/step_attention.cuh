@@ -45,6 +45,10 @@ struct StepAttentionParams {
   float* raw;
   size_t raw_rows, raw_stride;  // the launch's stacked rows; tokens, whole tiles
   float2* row_stats;
+  // Polls before a bounded wait gives up (0: the default), and bytes more than it brings that the first copy of each unit of the
+  // first sequence is told to expect (0 but for tests). What gives up leaves NaN rows, a NaN maximum in partial results and the
+  // accumulated weights without its rows'.
+  uint32_t wait_limit, fault_tx;
 };
 constexpr int kStepRows = 32;  // stacked query rows (row x query head of one KV head) of a unit
 inline int step_groups(int rows, int group) { return int((size_t(rows) * group + kStepRows - 1) / kStepRows); }

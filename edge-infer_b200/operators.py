@@ -176,6 +176,11 @@ def attention_window(ctx, q, k, v, output, window: int, sinks: int = 0, *, lengt
     abi.check(_native().attention_window(C.addressof(ctx), q, k, v, output, window, sinks, lengths, length))
 
 
+def inject_wait_timeout(polls: int) -> None:
+    """Test hook: a copy of this thread's next attention for long contexts does not arrive within `polls` polls."""
+    abi.check(_lib().ei_context_inject_wait_timeout(polls))
+
+
 def attention_shared_prefix_scratch_bytes(q_rows: int, query_heads: int, kv_heads: int, prefix_length: int) -> int:
     return _lib().ei_attention_shared_prefix_scratch_bytes(q_rows, query_heads, kv_heads, prefix_length)
 

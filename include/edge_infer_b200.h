@@ -179,7 +179,7 @@ ei_status ei_attention_prefill_static_bf16(const ei_context* ctx, ei_view3 q, ei
  * the current one; device pointers must belong to it. Nothing is allocated; results do not change from call to call; scratch is
  * used until the call's work is done, so calls that may overlap need scratch of their own. A first call on a device sets kernels
  * up: make it before a stream capture. Should a copy not arrive within its bounded wait (some half a second), the rows that
- * needed it come out as NaN. */
+ * needed it come out as NaN and add nothing to accumulated weights. */
 
 /* Rotation tables for contexts longer than a model was trained on. EI_ROPE_LINEAR: every angle is divided by `factor`.
  * EI_ROPE_YARN: frequencies that turn more than `fast` times over `original_positions` stay, those below `slow` turns are
@@ -496,6 +496,9 @@ ei_status ei_session_inject_failure(ei_session* session, int nth_launch, int com
  * own stream is drained and its history forgotten (prefill again); other sessions are untouched.
  * ref: the drain-or-poison rules of runtime/src/qwen3.cpp:127-161. No counterpart in the reference's API. */
 ei_status ei_session_inject_wait_timeout(ei_session* session, uint32_t polls);
+/* The same hook for the attentions for long contexts: in the calling thread's next one, the first K copy of each unit of rows of the
+ * first sequence is told to expect 16 bytes more than it delivers (0 disarms). What then gives up is described there. */
+ei_status ei_context_inject_wait_timeout(uint32_t polls);
 /* The same hook for the attention kernel: the first K / V tile copy of every block of this session's next
  * attention launch is told to expect 16 bytes more than it delivers. No counterpart in the reference's API. */
 ei_status ei_session_inject_attention_wait_timeout(ei_session* session, uint32_t polls);

@@ -35,3 +35,81 @@ def test_no_tokens_at_all(cuda, package, ctx, rows, heads, kv_heads):
         ops.attention_accumulate(ctx, q, k, v, out, old, scores, scratch)
         torch.cuda.synchronize()
         assert (out == 0).all() and (scores == 9).all()
+
+
+# Waits that run out. The first copy of every unit of the first sequence is told to expect 16 bytes more than it brings, with
+# a short limit: nothing faults or hangs, the unit's blocks give up and leave.
+
+# rows, tokens, sequences, heads, kv_heads: few rows in clusters, in one block, in two units a head, eight warps; the many-row
+# kernel with one query tile, with two and loaded queries, without a cluster, in clusters.
+GIVE_UP = [(1, 3000, 2, 8, 8), (1, 90, 40, 32, 8), (5, 700, 2, 28, 4), (2, 9000, 2, 8, 2), (16, 4000, 2, 32, 8), (300, 3000, 2, 28, 4),
+           (700, 2000, 3, 32, 8), (130, 6000, 2, 8, 4)]
+
+
+@pytest.mark.parametrize("case", GIVE_UP, ids=[str(i) for i in range(len(GIVE_UP))])
+def test_window_waits_that_run_out(cuda, package, ctx, case):
+    torch, ops = cuda, package.operators
+    rows, tokens, sequences, heads, kv_heads = case
+    q = normal(torch, 1, sequences * rows, heads, 128)
+    k, v = normal(torch, 2, sequences, tokens, kv_heads, 128), normal(torch, 3, sequences, tokens, kv_heads, 128)
+    want, out = torch.empty_like(q), torch.empty_like(q)
+    ops.attention_window(ctx, q, k, v, want, 1 << 20, 0, length=tokens)
+    for _ in range(2):
+        ops.inject_wait_timeout(2000)
+        ops.attention_window(ctx, q, k, v, out, 1 << 20, 0, length=tokens)
+        torch.cuda.synchronize()
+        assert out[:rows].isnan().all() and torch.equal(out[rows:], want[rows:])
+        ops.attention_window(ctx, q, k, v, out, 1 << 20, 0, length=tokens)
+        assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("rows,prefix,sequences,heads,kv_heads", [(1, 900, 2, 8, 2), (1, 8192, 64, 32, 8), (40, 9001, 3, 28, 4)])
+def test_prefix_waits_that_run_out(cuda, package, ctx, rows, prefix, sequences, heads, kv_heads):
+    torch, ops = cuda, package.operators
+    q = normal(torch, 1, sequences * rows, heads, 128)
+    pk, pv = normal(torch, 2, prefix, kv_heads, 128), normal(torch, 3, prefix, kv_heads, 128)
+    k, v = normal(torch, 4, sequences, 50, kv_heads, 128), normal(torch, 5, sequences, 50, kv_heads, 128)
+    scratch = torch.empty(ops.attention_shared_prefix_scratch_bytes(sequences * rows, heads, kv_heads, prefix), dtype=torch.uint8, device="cuda")
+    want, out = torch.empty_like(q), torch.empty_like(q)
+    ops.attention_shared_prefix(ctx, q, pk, pv, k, v, want, scratch, length=50)
+    ops.inject_wait_timeout(2000)
+    ops.attention_shared_prefix(ctx, q, pk, pv, k, v, out, scratch, length=50)
+    torch.cuda.synchronize()
+    assert out.isnan().all()
+    ops.attention_shared_prefix(ctx, q, pk, pv, k, v, out, scratch, length=50)
+    assert torch.equal(out, want) and torch.isfinite(want).all()
+
+
+@pytest.mark.parametrize("rows,tokens,heads,kv_heads", [(1, 5000, 8, 8), (9, 300, 4, 4), (16, 700, 16, 4), (130, 500, 12, 4)])
+def test_accumulated_weights_survive_waits_that_run_out(cuda, package, ctx, rows, tokens, heads, kv_heads):
+    """What the first sequence has accumulated stays, in place and apart; the others' is added to as ever. With 390 stacked rows
+    the second pass, which is not told to fail, adds what is its own."""
+    torch, ops = cuda, package.operators
+    q = normal(torch, 1, 2 * rows, heads, 128)
+    k, v = normal(torch, 2, 2, tokens, kv_heads, 128), normal(torch, 3, 2, tokens, kv_heads, 128)
+    old = torch.rand((2, kv_heads, tokens), generator=torch.Generator("cuda").manual_seed(4), device="cuda")
+    scratch = torch.empty(ops.attention_accumulate_scratch_bytes(2, rows, heads, kv_heads, tokens), dtype=torch.uint8, device="cuda")
+    want, new = torch.empty_like(q), torch.empty_like(old)
+    ops.attention_accumulate(ctx, q, k, v, want, old, new, scratch, length=tokens)
+    passes = -(-rows * (heads // kv_heads) // 256)
+    for apart in (True, False):
+        held, out = old.clone(), torch.empty_like(q)
+        scores = torch.empty_like(old) if apart else held
+        ops.inject_wait_timeout(2000)
+        ops.attention_accumulate(ctx, q, k, v, out, held, scores, scratch, length=tokens)
+        torch.cuda.synchronize()
+        assert torch.equal(scores[1], new[1]) and torch.equal(out[rows:], want[rows:])
+        assert torch.isfinite(scores).all()
+        if passes == 1:
+            assert torch.equal(scores[0], old[0]) and out[:rows].isnan().all()
+        else:
+            # Stacked rows of a KV head are row * group + head of the group: those from 256 on are as ever.
+            failed = (torch.arange(rows * (heads // kv_heads), device="cuda") < 256).view(rows, 1, -1).expand(-1, kv_heads, -1).flatten(1)
+            assert out[:rows][failed].isnan().all() and torch.equal(out[:rows][~failed], want[:rows][~failed])
+            total = (scores[0] - old[0]).double().sum(-1)
+            # As many rows' weights, which add up to one each: a weight's exponential and the one in the row's sum have arguments
+            # up to 16 with three roundings of 2^-24 apart, below 2^-17; and per place some roundings of a value up to the total.
+            left = (~failed).view(rows, kv_heads, -1).sum((0, 2))
+            assert ((total - left).abs() <= left * 2.0 ** -17 + tokens * 2.0 ** -22 * float(scores.max())).all()
+    ops.attention_accumulate(ctx, q, k, v, out, old, scores, scratch, length=tokens)
+    assert torch.equal(scores, new) and torch.equal(out, want)
