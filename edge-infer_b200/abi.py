@@ -146,6 +146,7 @@ PROTOTYPES = {
     "ei_attention_prefill_bf16": (_S, [C.POINTER(Context), View3, View3, View3, View3, _Z, _P, _Z]),
     "ei_attention_verify_bf16": (_S, [C.POINTER(Context), View3, View3, View3, View3, _P, _P, _Z]),
     "ei_attention_prefill_static_bf16": (_S, [C.POINTER(Context), View3, View3, View3, View3, _Z]),
+    "ei_context_expired_waits": (_S, [C.POINTER(Context), C.POINTER(C.c_uint64)]),
     "ei_context_inject_wait_timeout": (_S, [C.c_uint32]),
     "ei_build_rope_table_scaled": (_S, [_P, _Z, _Z, C.c_double, C.POINTER(RopeScaling)]),
     "ei_qk_norm_rope_bf16": (_S, [C.POINTER(Context), View3, View3, View2, _P, _Z, View1, View1, C.c_float, C.c_int32, View3,

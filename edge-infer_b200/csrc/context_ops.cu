@@ -306,6 +306,15 @@ ei_status ei_attention_window_bf16(const ei_context* ctx, ei_view3 q, ei_view4 k
   });
 }
 
+ei_status ei_context_expired_waits(const ei_context* ctx, uint64_t* count) {
+  return guarded([&] {
+    cudaStream_t stream = stream_of(ctx);
+    if (!count) reject("the count of expired waits needs a place");
+    expect_current_device(ctx);
+    *count = uint64_t(step_expired_waits(stream)) + span_expired_waits(stream);
+  });
+}
+
 ei_status ei_context_inject_wait_timeout(uint32_t polls) {
   return guarded([&] { injected_polls = polls; });
 }

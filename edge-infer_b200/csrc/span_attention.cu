@@ -94,6 +94,8 @@ __device__ __forceinline__ void tmem_loaded32(uint32_t* r) {
                  "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
 }
 
+__device__ uint32_t expired_waits;  // blocks that have given up since the library was loaded
+
 __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __grid_constant__ SpanAttentionParams p) {
   extern __shared__ unsigned char span_smem_raw[];
   unsigned char* const smem = span_smem_raw + ((1024u - (smem_address(span_smem_raw) & 1023u)) & 1023u);
@@ -529,6 +531,7 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
   __syncthreads();
   if (sh->abort) {  // no role is left to raise it: block-uniform
     if (threadIdx.x == 0) {
+      atomicAdd(&expired_waits, 1u);
       for (uint32_t polls = 0; polls < wait_limit && !mbarrier_try_wait(&sh->done, 0); ++polls) {
       }
       for (int i = 0; i < 2; ++i)
@@ -643,6 +646,13 @@ void launch_span_attention(const SpanAttentionParams& given, cudaStream_t stream
   config.attrs = &cluster;
   config.numAttrs = 1;
   check_cuda(cudaLaunchKernelEx(&config, span_attention_kernel, p), "cudaLaunchKernelEx");
+}
+
+uint32_t span_expired_waits(cudaStream_t stream) {
+  uint32_t count = 0;
+  EI_CUDA(cudaMemcpyFromSymbolAsync(&count, expired_waits, sizeof(count), 0, cudaMemcpyDeviceToHost, stream));
+  EI_CUDA(cudaStreamSynchronize(stream));
+  return count;
 }
 
 }  // namespace ei

@@ -27,5 +27,6 @@ struct SpanAttentionParams {
   uint32_t wait_limit, fault_tx;  // as StepAttentionParams
 };
 void launch_span_attention(const SpanAttentionParams& p, cudaStream_t stream);
+uint32_t span_expired_waits(cudaStream_t stream);  // as step_expired_waits
 
 }  // namespace ei

@@ -63,6 +63,8 @@ __device__ __forceinline__ int tile_offset(int token, int chunk) {
 __device__ __forceinline__ int query_offset(int row, int chunk) {
   return (chunk >> 3) * (kStepRows * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
 }
+__device__ uint32_t expired_waits;  // warps that have given up since the library was loaded
+
 // The larger of two, not a number if either is none.
 __device__ __forceinline__ float fmaxf_nan(float a, float b) {
   float y;
@@ -329,6 +331,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
     // anything else, and the unit's rows come out as NaN. A maximum that is no number, which no scores make, says so to the
     // other warps and blocks.
     if (lane == 0) {
+      atomicAdd(&expired_waits, 1u);
       for (int i = item; i < item + kBuffers; ++i) {
         if (first_tile + warp + (i >> 1) * kWarps < last_tile) mbarrier_wait(&full[i % kBuffers], (i / kBuffers) & 1, wait_limit);
       }
@@ -670,6 +673,13 @@ void launch_step_attention(const StepAttentionParams& p, size_t tokens, cudaStre
   attributes[1].val.programmaticStreamSerializationAllowed = 1;
   if (pdl) config.numAttrs = 2;
   check_cuda(cudaLaunchKernelEx(&config, step_kernel(shape.warps, two, p.raw != nullptr), p), "cudaLaunchKernelEx");
+}
+
+uint32_t step_expired_waits(cudaStream_t stream) {
+  uint32_t count = 0;
+  EI_CUDA(cudaMemcpyFromSymbolAsync(&count, expired_waits, sizeof(count), 0, cudaMemcpyDeviceToHost, stream));
+  EI_CUDA(cudaStreamSynchronize(stream));
+  return count;
 }
 
 void launch_step_weights(const StepAttentionParams& p, size_t tokens, cudaStream_t stream) {

@@ -55,6 +55,8 @@ inline int step_groups(int rows, int group) { return int((size_t(rows) * group +
 // k_map, v_map, first_group and groups are the caller's; tokens: the most a unit may read.
 void launch_step_attention(const StepAttentionParams& p, size_t tokens, cudaStream_t stream, bool pdl);
 constexpr int kStepWeightGroups = 8;  // that may share a launch with weights (their scores take scratch)
+// Waits that have run out in this kernel on the current device, read when the stream gets there.
+uint32_t step_expired_waits(cudaStream_t stream);
 void launch_step_weights(const StepAttentionParams& p, size_t tokens, cudaStream_t stream);
 
 }  // namespace ei

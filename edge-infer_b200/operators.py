@@ -176,6 +176,14 @@ def attention_window(ctx, q, k, v, output, window: int, sinks: int = 0, *, lengt
     abi.check(_native().attention_window(C.addressof(ctx), q, k, v, output, window, sinks, lengths, length))
 
 
+def expired_waits(ctx) -> int:
+    """How many bounded waits of the operators for long contexts have run out on the context's device so far, behind all that
+    its stream holds. While the count stays, nothing gave up; rows that did came out as NaN."""
+    count = C.c_uint64()
+    abi.check(_lib().ei_context_expired_waits(C.byref(ctx), C.byref(count)))
+    return count.value
+
+
 def inject_wait_timeout(polls: int) -> None:
     """Test hook: a copy of this thread's next attention for long contexts does not arrive within `polls` polls."""
     abi.check(_lib().ei_context_inject_wait_timeout(polls))

@@ -179,7 +179,12 @@ ei_status ei_attention_prefill_static_bf16(const ei_context* ctx, ei_view3 q, ei
  * the current one; device pointers must belong to it. Nothing is allocated; results do not change from call to call; scratch is
  * used until the call's work is done, so calls that may overlap need scratch of their own. A first call on a device sets kernels
  * up: make it before a stream capture. Should a copy not arrive within its bounded wait (some half a second), the rows that
- * needed it come out as NaN and add nothing to accumulated weights. */
+ * needed it come out as NaN and add nothing to accumulated weights; ei_context_expired_waits counts it. */
+
+/* How many bounded waits of these operators have run out on the context's device since the library was loaded, on any stream. Waits
+ * for the context's stream first (so it cannot be captured): when the count has not grown, nothing that this stream has run since
+ * gave up. */
+ei_status ei_context_expired_waits(const ei_context* ctx, uint64_t* count);
 
 /* Rotation tables for contexts longer than a model was trained on. EI_ROPE_LINEAR: every angle is divided by `factor`.
  * EI_ROPE_YARN: frequencies that turn more than `fast` times over `original_positions` stay, those below `slow` turns are

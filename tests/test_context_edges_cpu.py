@@ -232,3 +232,13 @@ def test_kernels_trigger_their_dependents_behind_their_own_wait():
             trigger = kernel.find("grid_launch_dependents();")
             if trigger >= 0:
                 assert 0 <= kernel.find("grid_dependency_wait();") < trigger, (path.name, kernel[:80])
+
+
+def test_counting_expired_waits_refuses(call):  # noqa: F811
+    count = C.c_uint64(7)
+    refused(call, call.lib.ei_context_expired_waits(None, C.byref(count)), says="context")
+    refused(call, call.lib.ei_context_expired_waits(C.byref(call.ctx), None), says="place")
+    call.ctx.device = 1 << 20
+    with pytest.raises((RuntimeError, ValueError)):
+        call.abi.check(call.lib.ei_context_expired_waits(C.byref(call.ctx), C.byref(count)))
+    assert count.value == 7

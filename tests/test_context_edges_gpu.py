@@ -113,3 +113,29 @@ def test_accumulated_weights_survive_waits_that_run_out(cuda, package, ctx, rows
             assert ((total - left).abs() <= left * 2.0 ** -17 + tokens * 2.0 ** -22 * float(scores.max())).all()
     ops.attention_accumulate(ctx, q, k, v, out, old, scores, scratch, length=tokens)
     assert torch.equal(scores, new) and torch.equal(out, want)
+
+
+def test_the_host_learns_of_waits_that_ran_out(cuda, package):
+    """By a count that grows with them and with nothing else, of both kernels, also from another thread and context."""
+    import threading
+    torch, ops = cuda, package.operators
+    stream = torch.cuda.Stream()
+    context, plain = ops.prepare_execution_context(stream.cuda_stream), ops.prepare_execution_context(0)
+    k, v = normal(torch, 2, 1, 6000, 4, 128), normal(torch, 3, 1, 6000, 4, 128)
+    before = ops.expired_waits(plain)
+    for rows in (1, 300):
+        q = normal(torch, 1, rows, 8, 128)
+        out = torch.empty_like(q)
+        torch.cuda.synchronize()
+        ops.attention_window(context, q, k, v, out, 1 << 20, 0, length=6000)
+        assert ops.expired_waits(context) == before
+        ops.inject_wait_timeout(2000)
+        ops.attention_window(context, q, k, v, out, 1 << 20, 0, length=6000)
+        after = ops.expired_waits(context)
+        assert after > before and out.isnan().all()
+        seen = []
+        other = threading.Thread(target=lambda: seen.append(ops.expired_waits(plain)))
+        other.start()
+        other.join()
+        assert seen == [after]
+        before = after
