@@ -151,9 +151,19 @@ EncodeTiled tensor_map_encoder() {
 void encode_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims,
                 const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle, const char* what) {
   const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
-  const CUresult result = tensor_map_encoder()(map, type, cuuint32_t(rank), const_cast<void*>(base), dims, strides, box,
-                                               ones, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&] {
+    return tensor_map_encoder()(map, type, cuuint32_t(rank), const_cast<void*>(base), dims, strides, box, ones,
+                                CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult result = encode();
+  if (result == CUDA_ERROR_INVALID_CONTEXT) {
+    // A thread whose first CUDA call this is: the driver, unlike the runtime, does not make the device's context current.
+    int device = 0;
+    EI_CUDA(cudaGetDevice(&device));
+    EI_CUDA(cudaSetDevice(device));
+    result = encode();
+  }
   if (result != CUDA_SUCCESS)
     throw std::runtime_error(std::string("Tensor map for ") + what + " could not be encoded: " +
                              std::to_string(int(result)));

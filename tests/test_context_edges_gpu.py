@@ -139,3 +139,32 @@ def test_the_host_learns_of_waits_that_ran_out(cuda, package):
         other.join()
         assert seen == [after]
         before = after
+
+
+@pytest.mark.parametrize("name", ["window", "window of many rows", "prefix", "accumulate"])
+def test_the_first_call_of_a_thread(cuda, package, ctx, name):
+    """The driver's calls need the device's context, which a thread has from its first call of the runtime on."""
+    import threading
+    torch, ops = cuda, package.operators
+    rows = 300 if "many" in name else 2
+    q = normal(torch, 1, 2 * rows, 8, 128)
+    k, v = normal(torch, 2, 2, 3000, 4, 128), normal(torch, 3, 2, 3000, 4, 128)
+    scratch = torch.empty(1 << 24, dtype=torch.uint8, device="cuda")
+    scores = torch.zeros((2, 4, 3000), device="cuda")
+    calls = {"prefix": lambda out: ops.attention_shared_prefix(ctx, q, k[0, :70], v[0, :70], k, v, out, scratch, length=3000),
+             "accumulate": lambda out: ops.attention_accumulate(ctx, q, k, v, out, None, scores, scratch, length=3000)}
+    call = calls.get(name, lambda out: ops.attention_window(ctx, q, k, v, out, 1 << 20, length=3000))
+    want, out, errors = torch.empty_like(q), torch.zeros_like(q), []
+    call(want)
+
+    def first():
+        try:
+            call(out)
+        except BaseException as error:  # noqa: BLE001
+            errors.append(error)
+
+    thread = threading.Thread(target=first)
+    thread.start()
+    thread.join()
+    torch.cuda.synchronize()
+    assert not errors and torch.equal(out, want)
