@@ -2,9 +2,9 @@
 // with accumulated weights, eviction. Validation before any write, no allocation, launches on the context's stream.
 #include "abi_checks.cuh"
 #include "abi_util.cuh"
+#include "attention_choice.hpp"
 #include "context_kernels.cuh"
 #include "span_attention.cuh"
-#include "step_choice.hpp"
 #include "view_overlap.hpp"
 
 #include <algorithm>
@@ -17,8 +17,6 @@ using namespace ei;
 namespace {
 
 constexpr size_t kHeadWidth = 128;
-// Up to so many stacked rows (rows x query heads of a KV head) the few-row kernel is bound by the bytes alone.
-constexpr size_t kFewRows = 16;
 constexpr size_t kMostTokens = size_t(1) << 30;  // of a cache: positions and windows stay clear of 2^31
 
 // The context's device has to be the current one: launches, tensor maps and kernel attributes go there. Asked for last, so
@@ -153,12 +151,6 @@ SpanAttentionParams span_of(const StepAttentionParams& p, const CacheStrides& ke
   encode_cache_map(&s.v_tile_map, values, size_t(p.capacity), size_t(p.kv_heads), size_t(p.sequences), kSpanTile, 2);
   return s;
 }
-// Which kernel takes a prefix for all sequences' stacked rows, by its estimate, and how it cuts it.
-bool prefix_on_tensor_cores(size_t stacked, size_t prefix, size_t kv_heads, SpanSplits* splits) {
-  if (stacked <= kFewRows) return false;
-  *splits = span_splits((stacked + kSpanRows - 1) / kSpanRows, prefix, int(kv_heads));
-  return splits->microseconds < step_microseconds(kv_heads * ((stacked + kStepRows - 1) / kStepRows), prefix);
-}
 size_t most_tokens(const StepAttentionParams& p) { return size_t(p.lengths ? p.capacity : p.length); }
 
 size_t raw_rows(size_t rows, size_t group) { return std::min<size_t>(kStepWeightGroups * kStepRows, rows * group); }
@@ -287,22 +279,16 @@ ei_status ei_attention_window_bf16(const ei_context* ctx, ei_view3 q, ei_view4 k
     p.sinks = int(std::min(sinks, kMostTokens));
     expect_current_device(ctx);
     take_injected(&p);
-    const size_t group = size_t(p.heads / p.kv_heads), stacked = size_t(p.rows) * group;
-    // Whichever kernel is the faster by its estimate; the tensor-core kernel's query tiles have 128 rows.
-    auto seen_by = [&](size_t rows) { return std::min(most_tokens(p), size_t(p.window) + size_t(p.sinks) + rows); };
-    if (stacked > kFewRows) {
-      const SpanWindow span = span_window(size_t(p.sequences), size_t(p.kv_heads), stacked, seen_by((2 * kSpanRows + group - 1) / group));
-      const size_t units = size_t(p.sequences) * size_t(p.kv_heads) * size_t(p.groups);
-      if (span.microseconds < step_microseconds(units, seen_by((kStepRows + group - 1) / group))) {
-        SpanAttentionParams s = span_of(p, keys, values);
-        s.cluster = span.cluster;
-        launch_span_attention(s, stream);
-        return;
-      }
+    const size_t group = size_t(p.heads / p.kv_heads), tokens = most_tokens(p);
+    SpanWindow choice;
+    if (window_on_tensor_cores(size_t(p.sequences), size_t(p.kv_heads), size_t(p.rows), group, tokens, size_t(p.window), size_t(p.sinks), &choice)) {
+      SpanAttentionParams span = span_of(p, keys, values);
+      span.cluster = choice.cluster;
+      launch_span_attention(span, stream);
+      return;
     }
     encode_maps(&p, keys, values);
-    const size_t seen = seen_by(kStepRows);
-    launch_step_attention(p, seen, stream, false);
+    launch_step_attention(p, window_tokens(tokens, size_t(p.window), size_t(p.sinks), kStepRows), stream, false);
   });
 }
 

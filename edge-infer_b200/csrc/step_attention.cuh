@@ -2,6 +2,7 @@
 #pragma once
 
 #include "kernels.cuh"
+#include "step_choice.hpp"
 
 namespace ei {
 
@@ -50,7 +51,6 @@ struct StepAttentionParams {
   // accumulated weights without its rows'.
   uint32_t wait_limit, fault_tx;
 };
-constexpr int kStepRows = 32;  // stacked query rows (row x query head of one KV head) of a unit
 inline int step_groups(int rows, int group) { return int((size_t(rows) * group + kStepRows - 1) / kStepRows); }
 // k_map, v_map, first_group and groups are the caller's; tokens: the most a unit may read.
 void launch_step_attention(const StepAttentionParams& p, size_t tokens, cudaStream_t stream, bool pdl);

@@ -6,6 +6,7 @@
 
 namespace ei {
 
+constexpr int kStepRows = 32;   // stacked query rows (row x query head of one KV head) of a unit
 constexpr int kStepTile = 32;   // tokens of a tile; a warp has one at a time
 constexpr int kStepMaxSplits = 16;
 

@@ -5,6 +5,7 @@ import subprocess
 
 import pytest
 
+import context_cases
 from test_context_cpu import ROOT, call, refused, run_choice  # noqa: F401
 
 
@@ -242,3 +243,20 @@ def test_counting_expired_waits_refuses(call):  # noqa: F811
     with pytest.raises((RuntimeError, ValueError)):
         call.abi.check(call.lib.ei_context_expired_waits(C.byref(call.ctx), C.byref(count)))
     assert count.value == 7
+
+
+def test_cases_run_on_the_kernels_they_are_named_for(tmp_path):
+    """The GPU tests' calls against the choice that the library makes."""
+    window = run_choice(tmp_path, "attention_choice.hpp", "ei::SpanWindow s{}; auto n = [&](int i) { return (size_t)atoll(a[i]); }; "
+                        "bool many = ei::window_on_tensor_cores(n(1), n(2), n(3), n(4), n(5), n(6), n(7), &s); "
+                        'std::printf("%d %d", int(many), many ? s.cluster : 0);')
+    for cases in (context_cases.HARD, context_cases.GIVE_UP, context_cases.GRAPH):
+        for name, c in cases.items():
+            got = window(c.sequences, c.kv_heads, c.rows, c.heads // c.kv_heads, c.tokens, c.window, c.sinks)
+            assert got == [int(c.kernel == "many"), c.cluster or 0], name
+    prefix = run_choice(tmp_path, "attention_choice.hpp", "ei::SpanSplits s{}; auto n = [&](int i) { return (size_t)atoll(a[i]); }; "
+                        'bool many = ei::prefix_on_tensor_cores(n(1), n(2), n(3), &s); std::printf("%d %d", int(many), many ? s.cluster : 0);')
+    for cases in (context_cases.PREFIX_HARD, context_cases.PREFIX_GIVE_UP):
+        for name, c in cases.items():
+            got = prefix(c.sequences * c.rows * c.heads // c.kv_heads, c.prefix, c.kv_heads)
+            assert got == [int(c.kernel == "many"), c.cluster or 0], name

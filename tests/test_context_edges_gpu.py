@@ -4,6 +4,7 @@ import math
 
 import pytest
 
+import context_cases
 from test_context_gpu import attention_reference, ctx, expect_attention, normal, window_visible  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -40,36 +41,30 @@ def test_no_tokens_at_all(cuda, package, ctx, rows, heads, kv_heads):
 # Waits that run out. The first copy of every unit of the first sequence is told to expect 16 bytes more than it brings, with
 # a short limit: nothing faults or hangs, the unit's blocks give up and leave.
 
-# rows, tokens, sequences, heads, kv_heads: few rows in clusters, in one block, in two units a head, eight warps; the many-row
-# kernel with one query tile, with two and loaded queries, without a cluster, in clusters.
-GIVE_UP = [(1, 3000, 2, 8, 8), (1, 90, 40, 32, 8), (5, 700, 2, 28, 4), (2, 9000, 2, 8, 2), (16, 4000, 2, 32, 8), (300, 3000, 2, 28, 4),
-           (700, 2000, 3, 32, 8), (130, 6000, 2, 8, 4)]
-
-
-@pytest.mark.parametrize("case", GIVE_UP, ids=[str(i) for i in range(len(GIVE_UP))])
-def test_window_waits_that_run_out(cuda, package, ctx, case):
-    torch, ops = cuda, package.operators
-    rows, tokens, sequences, heads, kv_heads = case
-    q = normal(torch, 1, sequences * rows, heads, 128)
-    k, v = normal(torch, 2, sequences, tokens, kv_heads, 128), normal(torch, 3, sequences, tokens, kv_heads, 128)
+@pytest.mark.parametrize("name", context_cases.GIVE_UP)
+def test_window_waits_that_run_out(cuda, package, ctx, name):
+    torch, ops, c = cuda, package.operators, context_cases.GIVE_UP[name]
+    q = normal(torch, 1, c.sequences * c.rows, c.heads, 128)
+    k, v = (normal(torch, seed, c.sequences, c.tokens, c.kv_heads, 128) for seed in (2, 3))
     want, out = torch.empty_like(q), torch.empty_like(q)
-    ops.attention_window(ctx, q, k, v, want, 1 << 20, 0, length=tokens)
+    ops.attention_window(ctx, q, k, v, want, c.window, c.sinks, length=c.tokens)
     for _ in range(2):
         ops.inject_wait_timeout(2000)
-        ops.attention_window(ctx, q, k, v, out, 1 << 20, 0, length=tokens)
+        ops.attention_window(ctx, q, k, v, out, c.window, c.sinks, length=c.tokens)
         torch.cuda.synchronize()
-        assert out[:rows].isnan().all() and torch.equal(out[rows:], want[rows:])
-        ops.attention_window(ctx, q, k, v, out, 1 << 20, 0, length=tokens)
+        assert out[:c.rows].isnan().all() and torch.equal(out[c.rows:], want[c.rows:])
+        ops.attention_window(ctx, q, k, v, out, c.window, c.sinks, length=c.tokens)
         assert torch.equal(out, want)
 
 
-@pytest.mark.parametrize("rows,prefix,sequences,heads,kv_heads", [(1, 900, 2, 8, 2), (1, 8192, 64, 32, 8), (40, 9001, 3, 28, 4)])
-def test_prefix_waits_that_run_out(cuda, package, ctx, rows, prefix, sequences, heads, kv_heads):
-    torch, ops = cuda, package.operators
-    q = normal(torch, 1, sequences * rows, heads, 128)
-    pk, pv = normal(torch, 2, prefix, kv_heads, 128), normal(torch, 3, prefix, kv_heads, 128)
-    k, v = normal(torch, 4, sequences, 50, kv_heads, 128), normal(torch, 5, sequences, 50, kv_heads, 128)
-    scratch = torch.empty(ops.attention_shared_prefix_scratch_bytes(sequences * rows, heads, kv_heads, prefix), dtype=torch.uint8, device="cuda")
+@pytest.mark.parametrize("name", context_cases.PREFIX_GIVE_UP)
+def test_prefix_waits_that_run_out(cuda, package, ctx, name):
+    torch, ops, c = cuda, package.operators, context_cases.PREFIX_GIVE_UP[name]
+    q = normal(torch, 1, c.sequences * c.rows, c.heads, 128)
+    pk, pv = normal(torch, 2, c.prefix, c.kv_heads, 128), normal(torch, 3, c.prefix, c.kv_heads, 128)
+    k, v = normal(torch, 4, c.sequences, 50, c.kv_heads, 128), normal(torch, 5, c.sequences, 50, c.kv_heads, 128)
+    size = ops.attention_shared_prefix_scratch_bytes(c.sequences * c.rows, c.heads, c.kv_heads, c.prefix)
+    scratch = torch.empty(size, dtype=torch.uint8, device="cuda")
     want, out = torch.empty_like(q), torch.empty_like(q)
     ops.attention_shared_prefix(ctx, q, pk, pv, k, v, want, scratch, length=50)
     ops.inject_wait_timeout(2000)
@@ -139,6 +134,318 @@ def test_the_host_learns_of_waits_that_ran_out(cuda, package):
         other.join()
         assert seen == [after]
         before = after
+
+
+# What is hard, on both kernels.
+
+HARD = pytest.mark.parametrize("name", context_cases.HARD)
+
+
+def window_call(torch, ops, context, c, q, k, v, out=None, **given):
+    out = torch.empty_like(q) if out is None else out
+    ops.attention_window(context, q, k, v, out, c.window, c.sinks, **(given or dict(length=c.tokens)))
+    return out
+
+
+def inputs_of(torch, c, scale=1.0):
+    return (normal(torch, 1, c.sequences * c.rows, c.heads, 128, scale=scale),
+            normal(torch, 2, c.sequences, c.tokens, c.kv_heads, 128, scale=scale), normal(torch, 3, c.sequences, c.tokens, c.kv_heads, 128))
+
+
+def visible_of(torch, c, n=None):
+    return window_visible(torch, c.tokens if n is None else n, c.rows, c.window, c.sinks, c.tokens)
+
+
+@HARD
+def test_random_scores_near_and_far_apart(cuda, package, ctx, name):
+    torch, ops, c = cuda, package.operators, context_cases.HARD[name]
+    for scale in (1.0, 1.5, 6.0, 40.0):
+        q, k, v = inputs_of(torch, c, scale)
+        out = window_call(torch, ops, ctx, c, q, k, v)
+        for s in {0, c.sequences - 1}:
+            mine = slice(s * c.rows, (s + 1) * c.rows)
+            want, size, _, _ = attention_reference(torch, q[mine], k[s], v[s], visible_of(torch, c))
+            expect_attention(torch, out[mine], want, size)
+
+
+PATTERNS = ["ascending", "descending", "zigzag", "steps", "equal", "last"]
+
+
+def patterned_keys(torch, pattern, tokens):
+    """First values of the keys; all others meet zeros of the queries, so that a score is one product, exact in FP32."""
+    t = torch.arange(tokens, device="cuda", dtype=torch.float64)
+    return {"ascending": t / 2, "descending": -t / 2, "zigzag": (t % 2 * 2 - 1) * 60, "steps": (t // 77) * 20, "equal": torch.full_like(t, 3.0),
+            "last": torch.where(t == tokens - 1, 300.0, -300.0)}[pattern].bfloat16()
+
+
+def expect_exact_scores(torch, out, q, k, v, visible):
+    """The reference's tolerance, but for scores that are exact: left are the exponential's argument, whose two roundings are of
+    2^-24 of the score and of its distance from the maximum, and the joining of parts, two roundings of the maxima. A score
+    beyond 16384 is at least 64 from any other (keys have eight bits) or equal to it, which no rounding takes apart."""
+    n, heads = q.shape[:2]
+    group = heads // k.shape[1]
+    for h in range(heads):
+        s = (q[:, h].double() @ k[:, h // group].double().T / math.sqrt(128)).masked_fill(~visible, -math.inf)
+        top = s.amax(-1, keepdim=True)
+        w = torch.softmax(s, -1)
+        error = 2.0 ** -21 + 2.0 ** -22 * (top.abs().clamp(max=16384.0) + torch.where(w > 2.0 ** -60, (s - top).abs(), 0.0))
+        values = v[:, h // group].double()
+        expect_attention(torch, out[:, h], w @ values, (w * (1 + error * 2.0 ** 8)) @ values.abs())
+
+
+@HARD
+@pytest.mark.parametrize("pattern", PATTERNS)
+def test_scores_in_patterns(cuda, package, ctx, name, pattern):
+    """Maxima that move every tile, never, or with the last token; equal scores."""
+    torch, ops, c = cuda, package.operators, context_cases.HARD[name]
+    _, k, v = inputs_of(torch, c)
+    q = torch.zeros(c.sequences * c.rows, c.heads, 128, dtype=torch.bfloat16, device="cuda")
+    q[..., 0] = 8.0
+    k[..., 0] = patterned_keys(torch, pattern, c.tokens)[None, :, None]
+    out = window_call(torch, ops, ctx, c, q, k, v)
+    for s in {0, c.sequences - 1}:
+        mine = slice(s * c.rows, (s + 1) * c.rows)
+        expect_exact_scores(torch, out[mine], q[mine], k[s], v[s], visible_of(torch, c))
+
+
+def clean(torch, got, want, size, wrong):
+    """Rows and heads outside `wrong` are as ever."""
+    got, want, size = got[~wrong], want[~wrong], size[~wrong]
+    expect_attention(torch, got, want, size)
+
+
+@HARD
+def test_nan_keys_in_sight_stay_in_their_rows(cuda, package, ctx, name):
+    """A key that is no number makes the rows that see it NaN, and no other: not the rows before it, those whose window has left it
+    behind, other heads' or sequences'."""
+    torch, ops, c = cuda, package.operators, context_cases.HARD[name]
+    q, k, v = inputs_of(torch, c)
+    base, visible = window_call(torch, ops, ctx, c, q, k, v), visible_of(torch, c)
+    group, s, head = c.heads // c.kv_heads, c.sequences - 1, c.kv_heads - 1
+    for token in (c.tokens - 1, c.tokens - 1 - c.rows // 2, max(c.sinks, c.tokens - c.window)):
+        bad = k.clone()
+        bad[s, token, head, 5] = math.nan
+        out = window_call(torch, ops, ctx, c, q, bad, v)
+        wrong = torch.zeros(out.shape[:2], dtype=torch.bool, device="cuda")
+        wrong[s * c.rows:, head * group:] = visible[:, token, None]
+        assert wrong.any()
+        assert out[wrong].isnan().all() and torch.equal(out[~wrong], base[~wrong])
+
+
+@HARD
+def test_infinite_keys_in_sight(cuda, package, ctx, name):
+    """A score of -inf is a weight of zero, one of +inf leaves nothing that is a number, as in the formula."""
+    torch, ops, c = cuda, package.operators, context_cases.HARD[name]
+    q, k, v = inputs_of(torch, c)
+    q[..., 9] = torch.where(q[..., 9] == 0, 1.0, q[..., 9])
+    visible = visible_of(torch, c)
+    group, token = c.heads // c.kv_heads, c.tokens - 1 - c.rows // 3
+    k[0, token, 0, 9] = math.inf
+    out = window_call(torch, ops, ctx, c, q, k, v)[:c.rows]
+    mine = q[:c.rows]
+    infinite = visible[:, token, None] & (mine[..., 9] > 0)
+    infinite[:, group:] = False
+    assert infinite.any() and out[infinite].isnan().all()
+    rest = visible.clone()
+    rest[:, token] = False
+    finite = k[0].clone()
+    finite[token, 0, 9] = 0.0
+    some, _, _, _ = attention_reference(torch, mine, finite, v[0], visible)
+    without, size, _, _ = attention_reference(torch, mine, finite, v[0], rest)
+    minus = visible[:, token, None] & (mine[..., 9] < 0)
+    minus[:, group:] = False
+    assert minus.any()
+    want, wide, _, _ = attention_reference(torch, mine, finite, v[0], visible)
+    want, wide = torch.where(minus[..., None], without, want), torch.where(minus[..., None], size, wide)
+    clean(torch, out, want, wide, infinite)
+
+
+@HARD
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_values_that_are_no_numbers_stay_in_their_column(cuda, package, ctx, name, value):
+    """Rows that see the token lose that one column; of rows of the same call that do not see it, no other column, head or
+    sequence is touched."""
+    torch, ops, c = cuda, package.operators, context_cases.HARD[name]
+    q, k, v = inputs_of(torch, c)
+    base, visible = window_call(torch, ops, ctx, c, q, k, v), visible_of(torch, c)
+    group, token = c.heads // c.kv_heads, c.tokens - 1 - c.rows // 2
+    v[0, token, 0, 33] = value
+    out = window_call(torch, ops, ctx, c, q, k, v)
+    assert not torch.isfinite(out[:c.rows, :group, 33][visible[:, token]]).any()
+    out[:c.rows, :group, 33] = base[:c.rows, :group, 33]
+    assert torch.equal(out, base)
+
+
+@HARD
+def test_outputs_in_the_queries_place_and_wide_rows(cuda, package, ctx, name):
+    """In place, as slices of wider rows, and over caches in another order: the same bits."""
+    torch, ops, c = cuda, package.operators, context_cases.HARD[name]
+    q, k, v = inputs_of(torch, c)
+    base = window_call(torch, ops, ctx, c, q, k, v)
+    mine = q.clone()
+    assert torch.equal(window_call(torch, ops, ctx, c, mine, k, v, mine), base)
+    wide = torch.full((q.shape[0], c.heads * 128 + 24), 7.0, dtype=torch.bfloat16, device="cuda")
+    rows = wide[:, 16:-8].unflatten(-1, (c.heads, 128))
+    rows.copy_(q)
+    turned = k.transpose(1, 2).contiguous().transpose(1, 2), torch.stack((v, v), 2)[:, :, 1]
+    assert torch.equal(window_call(torch, ops, ctx, c, rows, *turned, rows), base)
+    assert (wide[:, :16] == 7).all() and (wide[:, -8:] == 7).all()
+
+
+@pytest.mark.parametrize("name", context_cases.GRAPH)
+def test_graphs_follow_lengths(cuda, package, name):
+    """Captured in a thread that has never called, replayed for other lengths (none, one, one below the rows, all) and queries."""
+    import threading
+    torch, ops, c = cuda, package.operators, context_cases.GRAPH[name]
+    q, k, v = inputs_of(torch, c)
+    lengths = torch.full((c.sequences,), c.tokens, dtype=torch.int32, device="cuda")
+    out, stream, graph, errors = torch.empty_like(q), torch.cuda.Stream(), torch.cuda.CUDAGraph(), []
+    context = ops.prepare_execution_context(stream.cuda_stream)
+    with torch.cuda.stream(stream):
+        window_call(torch, ops, context, c, q, k, v, out, lengths=lengths)
+    torch.cuda.synchronize()
+
+    def capture():
+        try:
+            with torch.cuda.graph(graph, stream=stream):
+                window_call(torch, ops, context, c, q, k, v, out, lengths=lengths)
+        except BaseException as error:  # noqa: BLE001
+            errors.append(error)
+
+    thread = threading.Thread(target=capture)
+    thread.start()
+    thread.join()
+    assert not errors
+    for n in ([c.tokens, c.tokens // 2], [0, c.tokens - 1], [1, c.rows - 1], [c.rows, c.tokens + 1], [c.rows + 1, -1]):
+        lengths.copy_(torch.tensor(n, dtype=torch.int32))
+        q.copy_(normal(torch, sum(n), *q.shape))
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for s, held in enumerate(n):
+            mine = slice(s * c.rows, (s + 1) * c.rows)
+            held = held if 0 <= held <= c.tokens else 0
+            want, size, _, _ = attention_reference(torch, q[mine], k[s], v[s], visible_of(torch, c, held))
+            expect_attention(torch, out[mine], want, size)
+            assert (out[mine][:max(0, c.rows - held)] == 0).all()
+
+
+@pytest.mark.parametrize("name", context_cases.PREFIX_HARD)
+def test_shared_prefix_over_strided_caches(cuda, package, ctx, name):
+    """Own tokens in another order and with gaps, outputs as slices of wider rows, two streams and threads at once with scratch of
+    their own, in place: the same bits, and right."""
+    import threading
+    torch, ops, c = cuda, package.operators, context_cases.PREFIX_HARD[name]
+    own = 61
+    q = normal(torch, 1, c.sequences * c.rows, c.heads, 128, scale=1.5)
+    pk, pv = normal(torch, 2, c.prefix, c.kv_heads, 128, scale=1.5), normal(torch, 3, c.prefix, c.kv_heads, 128)
+    k, v = normal(torch, 4, c.sequences, own, c.kv_heads, 128, scale=1.5), normal(torch, 5, c.sequences, own, c.kv_heads, 128)
+    lengths = torch.tensor([own - s % 7 for s in range(c.sequences)], dtype=torch.int32, device="cuda")
+    size = ops.attention_shared_prefix_scratch_bytes(c.sequences * c.rows, c.heads, c.kv_heads, c.prefix)
+    results = []
+
+    def go(context, queries, keys, values, out):
+        scratch = torch.empty(size, dtype=torch.uint8, device="cuda")
+        ops.attention_shared_prefix(context, queries, pk, pv, keys, values, out, scratch, lengths=lengths)
+        results.append((out, scratch))
+
+    go(ctx, q, k, v, torch.empty_like(q))
+    wide = torch.full((q.shape[0] + 1, c.heads * 128 + 8), 7.0, dtype=torch.bfloat16, device="cuda")
+    rows = wide[:-1, 8:].unflatten(-1, (c.heads, 128))
+    both = torch.full((c.sequences, own + 3, c.kv_heads, 2, 128), math.nan, dtype=torch.bfloat16, device="cuda")
+    both[:, :own, :, 0], both[:, :own, :, 1] = k, v
+    go(ctx, q, both[:, :own, :, 0], both[:, :own, :, 1], rows)
+    mine = q.clone()
+    go(ctx, mine, k.transpose(1, 2).contiguous().transpose(1, 2), v, mine)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [torch.empty_like(q) for _ in streams]
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=lambda s=s, o=o: [go(ops.prepare_execution_context(s.cuda_stream), q, k, v, o) for _ in range(20)])
+               for s, o in zip(streams, outs)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    torch.cuda.synchronize()
+    assert len(results) == 43
+    for out, _ in results:
+        assert torch.equal(out, results[0][0])
+    assert (wide[-1] == 7).all() and (wide[:, :8] == 7).all()
+    for s in {0, c.sequences - 1}:
+        mine, n = slice(s * c.rows, (s + 1) * c.rows), int(lengths[s])
+        place = torch.arange(n - c.rows, n, device="cuda")[:, None]
+        visible = torch.cat(((place >= 0).expand(-1, c.prefix), torch.arange(own, device="cuda")[None] <= place), 1)
+        want, allowance, _, _ = attention_reference(torch, q[mine], torch.cat((pk, k[s])), torch.cat((pv, v[s])), visible)
+        expect_attention(torch, results[0][0][mine], want, allowance)
+
+
+@pytest.mark.parametrize("rows,heads,kv_heads", [(1, 16, 2), (9, 12, 4)])
+def test_accumulated_weights_over_strided_caches_and_far_scores(cuda, package, ctx, rows, heads, kv_heads):
+    """Caches in other orders and with gaps give the same bits; scores far apart give weights of one and zero."""
+    torch, ops = cuda, package.operators
+    sequences, tokens = 2, 700
+    size = ops.attention_accumulate_scratch_bytes(sequences, rows, heads, kv_heads, tokens)
+    scratch = torch.empty(size, dtype=torch.uint8, device="cuda")
+    old = torch.rand((sequences, kv_heads, tokens), generator=torch.Generator("cuda").manual_seed(9), device="cuda")
+
+    def go(q, k, v, scores):
+        out, new = torch.empty_like(q), torch.empty_like(old)
+        ops.attention_accumulate(ctx, q, k, v, out, scores, new, scratch, length=tokens)
+        return out, new
+
+    for scale in (1.0, 40.0):
+        q = normal(torch, 1, sequences * rows, heads, 128, scale=scale)
+        k, v = normal(torch, 2, sequences, tokens, kv_heads, 128, scale=scale), normal(torch, 3, sequences, tokens, kv_heads, 128)
+        out, new = go(q, k, v, old)
+        both = torch.full((sequences, tokens + 5, 2, kv_heads, 128), math.nan, dtype=torch.bfloat16, device="cuda")
+        both[:, :tokens, 0], both[:, :tokens, 1] = k, v
+        turned = torch.rand((kv_heads, sequences, tokens + 1), device="cuda")[..., :tokens].transpose(0, 1)
+        turned.copy_(old)
+        for got in (go(q, both[:, :tokens, 0], both[:, :tokens, 1], turned), go(q, k.transpose(1, 2).contiguous().transpose(1, 2), v, old)):
+            assert torch.equal(got[0], out) and torch.equal(got[1], new)
+        for s in range(sequences):
+            mine = slice(s * rows, (s + 1) * rows)
+            want, allowance, weights, slack = attention_reference(torch, q[mine], k[s], v[s], window_visible(torch, tokens, rows, 1 << 30, 0, tokens))
+            expect_attention(torch, out[mine], want, allowance)
+            total = weights + old[s].double()
+            assert ((new[s].double() - total).abs() <= slack + 2.0 ** -22 * total).all()
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("norm", [False, True])
+def test_rotation_of_what_is_no_number(cuda, package, ctx, interleaved, norm):
+    """NaN and infinities stay in their head; without a norm, in their pair."""
+    torch, ops = cuda, package.operators
+    q, k = normal(torch, 1, 6, 4, 128), normal(torch, 2, 6, 2, 128)
+    weight = 1 + normal(torch, 3, 128, scale=0.1) if norm else None
+    table = torch.from_numpy(ops.build_rope_table_scaled(100, 64, 1e4)).cuda()
+
+    def go(x):
+        out = torch.empty_like(x), torch.empty_like(k)
+        ops.qk_norm_rope(ctx, x, k, table, *out, offset=3, q_weight=weight, k_weight=weight, interleaved=interleaved)
+        return out
+
+    base, keys = go(q)
+    assert torch.isfinite(base).all()
+    for at, value in ((10, math.nan), (100, math.inf), (63, -math.inf)):
+        x = q.clone()
+        x[2, 1, at] = value
+        out, same = go(x)
+        touched = torch.zeros(128, dtype=torch.bool)
+        touched[at] = True
+        if at < 64:
+            touched[at ^ 1 if interleaved else at ^ 32] = True
+        if norm and math.isnan(value):
+            touched[:] = True
+        assert torch.equal(same, keys)
+        if norm and not math.isnan(value):  # divided by an infinite length: zeros beside it, which the rotation leaves zeros
+            assert (out[2, 1, ~touched] == 0).all() and not torch.isfinite(out[2, 1, at])
+        else:
+            assert not torch.isfinite(out[2, 1, touched]).any()
+            assert torch.equal(out[2, 1, ~touched], base[2, 1, ~touched])
+        out[2, 1] = base[2, 1]
+        assert torch.equal(out, base)
 
 
 @pytest.mark.parametrize("name", ["window", "window of many rows", "prefix", "accumulate"])
