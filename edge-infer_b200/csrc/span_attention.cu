@@ -50,6 +50,11 @@ constexpr int kStages = 4;  // each a tile's V and the K that the half's next sc
 constexpr int kStageBytes = 2 * kBufferBytes;
 constexpr int kQueryBytes = 2 * kSpanRows * 128;
 constexpr float kSlack = 8.0f;  // powers of two
+// A weight is 2^(s scale - m scale) by one multiplication and addition, with m scale rounded. That rounding is the same for a
+// row's equal scores, but from 2^31 on it soon reaches the exponents' range: the row's largest weight, 1, would be 0 or infinite.
+// Scores of that size are multiples of 128, so that any but those equal to the maximum weigh nothing at a power of two of about
+// the scale as well, and with that the products are exact.
+constexpr float kFarScore = 2147483648.0f, kFarScale = 0.125f;  // rsqrt(128) log2(e) = 0.1275
 constexpr size_t kStateBytes = 512;
 // Queries, first K of each half, ring, state.
 constexpr size_t kSpanSharedBytes = size_t(2) * kQueryBytes + 2 * kBufferBytes + size_t(kStages) * kStageBytes + 1024 + kStateBytes;
@@ -255,7 +260,6 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
     const uint32_t places = tmem + lanes + half * 256, outputs = places + 128;
     const int last = p.together ? length - 1 : base + row;
     const bool some_live = __any_sync(0xffffffffu, live);
-    const float2 scales = make_float2(exponent_scale, exponent_scale);
     const int tiles = own_tiles;
     // Boxes that every row of the half sees whole.
     const int clean_begin = sink_boxes + (max(0, (half ? last_position1 : last_position0) - p.window + 1 - low) + kSpanBox - 1) / kSpanBox;
@@ -269,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
       if (!ok) break;
       tcgen05_fence_after();
       uint32_t s[2][32];
-      float2 shifts = make_float2(0.0f, 0.0f);
+      float2 scales = make_float2(exponent_scale, exponent_scale), shifts = make_float2(0.0f, 0.0f);
       float rescale = 1.0f;
       bool moved_some = false;
       if (some_live) {
@@ -301,8 +305,10 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
         if (moved) maximum = top;
         // A row with nothing visible yet keeps -inf; 0 as the exponent's base then makes every weight 0.
         const float reference = maximum == -INFINITY ? 0.0f : maximum;
-        shifts.x = shifts.y = -reference * exponent_scale;
-        if (moved) rescale = power_of_two((previous - reference) * exponent_scale);
+        if (fabsf(reference) >= kFarScore) scales.x = scales.y = kFarScale;
+        shifts.x = shifts.y = -reference * scales.x;
+        // From one rounded base of the exponents to the next.
+        if (moved) rescale = power_of_two(__fadd_rn(__fmul_rn(previous, scales.x), shifts.x));
         moved_some = __any_sync(0xffffffffu, moved);
       }
       if (!clean && (stop_of(box0) - start_of(box0) < kSpanBox || stop_of(box0 + 1) - start_of(box0 + 1) < kSpanBox)) {

@@ -244,8 +244,16 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
             if (t >= stop || t > at || (t <= at - p.window && t >= p.sinks)) s[rt][j][x] = -INFINITY;
           }
     }
+    // Scores as powers of two, rounded once here: relative to a maximum that is one of them, the largest weight is 1 whatever its
+    // size, and the weights that are reported and their sum are made of the same numbers.
+#pragma unroll
+    for (int rt = 0; rt < kRowTiles; ++rt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s[rt][j][x] *= exponent_scale;
     if (kWeights) {
-      // Scores as powers of two, for the weights when the row's maximum and sum are known.
+      // For the weights when the row's maximum and sum are known.
 #pragma unroll
       for (int rt = 0; rt < kRowTiles; ++rt)
 #pragma unroll
@@ -255,7 +263,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
 #pragma unroll
             for (int j = 0; j < 4; ++j)
               *reinterpret_cast<float2*>(raw + size_t(i) * p.raw_stride + size_t(tile) * kStepTile + j * 8 + 2 * c) =
-                  make_float2(s[rt][j][2 * half] * exponent_scale, s[rt][j][2 * half + 1] * exponent_scale);
+                  make_float2(s[rt][j][2 * half], s[rt][j][2 * half + 1]);
           }
         }
     }
@@ -271,9 +279,9 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         // A row with nothing visible yet keeps -inf; 0 as the exponent's base then makes every weight 0.
-        const float reference = top == -INFINITY ? 0.0f : top, shift = reference * exponent_scale;
+        const float reference = top == -INFINITY ? 0.0f : top;
         if (__any_sync(0xffffffffu, top != m[rt][half])) {
-          const float rescale = power_of_two((m[rt][half] - reference) * exponent_scale);  // exactly 1 where it stayed
+          const float rescale = power_of_two(m[rt][half] - reference);  // exactly 1 where it stayed
           l[rt][half] *= rescale;
 #pragma unroll
           for (int d = 0; d < 16; ++d) {
@@ -284,8 +292,8 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float w0 = power_of_two(fmaf(s[rt][j][2 * half], exponent_scale, -shift));
-          const float w1 = power_of_two(fmaf(s[rt][j][2 * half + 1], exponent_scale, -shift));
+          const float w0 = power_of_two(s[rt][j][2 * half] - reference);
+          const float w1 = power_of_two(s[rt][j][2 * half + 1] - reference);
           const uint32_t both = pack_bf16(w0, w1);
           l[rt][half] += kWeights ? w0 + w1 : bf16_lo(both) + bf16_hi(both);
           pa[rt][j][half] = both;
@@ -349,7 +357,6 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : 2) step_attenti
     for (int half = 0; half < 2; ++half) {
       l[rt][half] += __shfl_xor_sync(0xffffffffu, l[rt][half], 1);
       l[rt][half] += __shfl_xor_sync(0xffffffffu, l[rt][half], 2);
-      m[rt][half] *= exponent_scale;
       if (c == 0) {
         sh->maxima[warp][rt * 16 + half * 8 + g] = m[rt][half];
         sh->sums[warp][rt * 16 + half * 8 + g] = l[rt][half];

@@ -168,14 +168,22 @@ def test_random_scores_near_and_far_apart(cuda, package, ctx, name):
             expect_attention(torch, out[mine], want, size)
 
 
-PATTERNS = ["ascending", "descending", "zigzag", "steps", "equal", "last"]
+PATTERNS = ["ascending", "descending", "zigzag", "steps", "equal", "last", "lowest", "1e6", "1e12", "1e30", "1e36"]
 
 
 def patterned_keys(torch, pattern, tokens):
     """First values of the keys; all others meet zeros of the queries, so that a score is one product, exact in FP32."""
     t = torch.arange(tokens, device="cuda", dtype=torch.float64)
+    if pattern[0] == "1":  # two equal ones far above the others
+        return torch.where(t % (tokens - 4) == 3, float(pattern), -float(pattern)).bfloat16()
     return {"ascending": t / 2, "descending": -t / 2, "zigzag": (t % 2 * 2 - 1) * 60, "steps": (t // 77) * 20, "equal": torch.full_like(t, 3.0),
-            "last": torch.where(t == tokens - 1, 300.0, -300.0)}[pattern].bfloat16()
+            "lowest": torch.full_like(t, torch.finfo(torch.bfloat16).min), "last": torch.where(t == tokens - 1, 300.0, -300.0)}[pattern].bfloat16()
+
+
+def exact_weights(torch, q, keys, visible):
+    """Scores and weights in 64 bits of a head's queries."""
+    s = (q.double() @ keys.double().T / math.sqrt(128)).masked_fill(~visible, -math.inf)
+    return s, torch.softmax(s, -1)
 
 
 def expect_exact_scores(torch, out, q, k, v, visible):
@@ -185,9 +193,8 @@ def expect_exact_scores(torch, out, q, k, v, visible):
     n, heads = q.shape[:2]
     group = heads // k.shape[1]
     for h in range(heads):
-        s = (q[:, h].double() @ k[:, h // group].double().T / math.sqrt(128)).masked_fill(~visible, -math.inf)
+        s, w = exact_weights(torch, q[:, h], k[:, h // group], visible)
         top = s.amax(-1, keepdim=True)
-        w = torch.softmax(s, -1)
         error = 2.0 ** -21 + 2.0 ** -22 * (top.abs().clamp(max=16384.0) + torch.where(w > 2.0 ** -60, (s - top).abs(), 0.0))
         values = v[:, h // group].double()
         expect_attention(torch, out[:, h], w @ values, (w * (1 + error * 2.0 ** 8)) @ values.abs())
@@ -196,11 +203,14 @@ def expect_exact_scores(torch, out, q, k, v, visible):
 @HARD
 @pytest.mark.parametrize("pattern", PATTERNS)
 def test_scores_in_patterns(cuda, package, ctx, name, pattern):
-    """Maxima that move every tile, never, or with the last token; equal scores."""
+    """Maxima that move every tile, never, or with the last token; equal scores; the lowest finite keys; scores as large
+    as FP32 holds, whose products with the scale are rounded by more than weights' exponents reach."""
     torch, ops, c = cuda, package.operators, context_cases.HARD[name]
     _, k, v = inputs_of(torch, c)
     q = torch.zeros(c.sequences * c.rows, c.heads, 128, dtype=torch.bfloat16, device="cuda")
-    q[..., 0] = 8.0
+    q[..., 0] = 1.0 if pattern in ("lowest", "1e36") else 8.0
+    if pattern[0] == "1":
+        q[..., 0] *= 1 + normal(torch, 8, *q.shape[:2]).abs() / 8
     k[..., 0] = patterned_keys(torch, pattern, c.tokens)[None, :, None]
     out = window_call(torch, ops, ctx, c, q, k, v)
     for s in {0, c.sequences - 1}:
@@ -380,6 +390,31 @@ def test_shared_prefix_over_strided_caches(cuda, package, ctx, name):
         expect_attention(torch, results[0][0][mine], want, allowance)
 
 
+@pytest.mark.parametrize("pattern", PATTERNS)
+@pytest.mark.parametrize("name", context_cases.PREFIX_HARD)
+def test_scores_in_patterns_behind_a_prefix(cuda, package, ctx, name, pattern):
+    """The patterns over prefix and own tokens, the largest scores on both sides of the border."""
+    torch, ops, c = cuda, package.operators, context_cases.PREFIX_HARD[name]
+    own = 310
+    q = torch.zeros(c.sequences * c.rows, c.heads, 128, dtype=torch.bfloat16, device="cuda")
+    q[..., 0] = 1.0 if pattern in ("lowest", "1e36") else 8.0
+    pk, pv = normal(torch, 2, c.prefix, c.kv_heads, 128), normal(torch, 3, c.prefix, c.kv_heads, 128)
+    k, v = normal(torch, 4, c.sequences, own, c.kv_heads, 128), normal(torch, 5, c.sequences, own, c.kv_heads, 128)
+    keys = patterned_keys(torch, pattern, c.prefix + own - 4)
+    if pattern[0] == "1":
+        keys[3], keys[c.prefix - 1], keys[c.prefix] = float(pattern), float(pattern), float(pattern)
+    keys = torch.cat((keys, keys[-4:]))
+    pk[..., 0], k[..., 0] = keys[:c.prefix, None], keys[c.prefix:][None, :, None]
+    size = ops.attention_shared_prefix_scratch_bytes(c.sequences * c.rows, c.heads, c.kv_heads, c.prefix)
+    out = torch.empty_like(q)
+    ops.attention_shared_prefix(ctx, q, pk, pv, k, v, out, torch.empty(size, dtype=torch.uint8, device="cuda"), length=own)
+    place = torch.arange(own - c.rows, own, device="cuda")[:, None]
+    visible = torch.cat(((place >= 0).expand(-1, c.prefix), torch.arange(own, device="cuda")[None] <= place), 1)
+    for s in {0, c.sequences - 1}:
+        mine = slice(s * c.rows, (s + 1) * c.rows)
+        expect_exact_scores(torch, out[mine], q[mine], torch.cat((pk, k[s])), torch.cat((pv, v[s])), visible)
+
+
 @pytest.mark.parametrize("rows,heads,kv_heads", [(1, 16, 2), (9, 12, 4)])
 def test_accumulated_weights_over_strided_caches_and_far_scores(cuda, package, ctx, rows, heads, kv_heads):
     """Caches in other orders and with gaps give the same bits; scores far apart give weights of one and zero."""
@@ -410,6 +445,30 @@ def test_accumulated_weights_over_strided_caches_and_far_scores(cuda, package, c
             expect_attention(torch, out[mine], want, allowance)
             total = weights + old[s].double()
             assert ((new[s].double() - total).abs() <= slack + 2.0 ** -22 * total).all()
+
+
+@pytest.mark.parametrize("pattern", ["lowest", "1e6", "1e12", "1e30", "1e36"])
+@pytest.mark.parametrize("rows,heads,kv_heads", [(1, 16, 2), (9, 12, 4)])
+def test_accumulated_weights_of_far_scores(cuda, package, ctx, rows, heads, kv_heads, pattern):
+    """Two equal scores above all others, or all of them equal: a half each, or one part each."""
+    torch, ops = cuda, package.operators
+    tokens = 700
+    q = torch.zeros(rows, heads, 128, dtype=torch.bfloat16, device="cuda")
+    q[..., 0] = 1 + normal(torch, 8, rows, heads).abs() / 8
+    if pattern == "lowest":
+        q[..., 0] = 1.0
+    k, v = normal(torch, 2, 1, tokens, kv_heads, 128), normal(torch, 3, 1, tokens, kv_heads, 128)
+    k[..., 0] = patterned_keys(torch, pattern, tokens)[None, :, None]
+    scratch = torch.empty(ops.attention_accumulate_scratch_bytes(1, rows, heads, kv_heads, tokens), dtype=torch.uint8, device="cuda")
+    out, new = torch.empty_like(q), torch.empty((1, kv_heads, tokens), device="cuda")
+    ops.attention_accumulate(ctx, q, k, v, out, None, new, scratch, length=tokens)
+    visible = window_visible(torch, tokens, rows, 1 << 30, 0, tokens)
+    expect_exact_scores(torch, out, q, k[0], v[0], visible)
+    group = heads // kv_heads
+    for j in range(kv_heads):
+        want = sum(exact_weights(torch, q[:, h], k[0, :, j], visible)[1].sum(0) for h in range(j * group, (j + 1) * group))
+        # A weight's exponential, its share and the additions: some roundings of 2^-24 and the exponential's 2^-22.
+        assert ((new[0, j].double() - want).abs() <= 2.0 ** -20 * want + 1e-30).all()
 
 
 @pytest.mark.parametrize("interleaved", [False, True])
