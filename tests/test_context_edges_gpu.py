@@ -5,7 +5,7 @@ import math
 import pytest
 
 import context_cases
-from test_context_gpu import attention_reference, ctx, expect_attention, normal, window_visible  # noqa: F401
+from test_context_gpu import attention_reference, ctx, evict_reference, expect_attention, normal, window_visible  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -534,3 +534,133 @@ def test_the_first_call_of_a_thread(cuda, package, ctx, name):
     thread.join()
     torch.cuda.synchronize()
     assert not errors and torch.equal(out, want)
+
+
+def test_weights_eviction_and_rotation_in_a_graph(cuda, package):
+    """One graph of a server's step behind an observation window: rotation into the cache, accumulated weights in one and in two
+    passes, eviction; replayed for other lengths, positions, queries and scores, each time as the calls one by one."""
+    torch, ops = cuda, package.operators
+    sequences, rows, heads, kv_heads, capacity, budget = 3, 70, 16, 4, 500, 128  # 280 stacked rows
+    q = normal(torch, 1, sequences * rows, heads, 128)
+    k, v = normal(torch, 3, sequences, capacity, kv_heads, 128), normal(torch, 4, sequences, capacity, kv_heads, 128)
+    table = torch.from_numpy(ops.build_rope_table_scaled(1000, 128, 1e4)).cuda()
+    positions = torch.zeros(sequences * rows, dtype=torch.int32, device="cuda")
+    lengths = torch.full((sequences,), capacity, dtype=torch.int32, device="cuda")
+    scratch = torch.empty(ops.attention_accumulate_scratch_bytes(sequences, rows, heads, kv_heads, capacity), dtype=torch.uint8, device="cuda")
+    keys = normal(torch, 5, sequences * rows, kv_heads, 128)
+
+    def buffers():
+        return dict(q=torch.zeros_like(q), k=torch.zeros_like(keys), out=torch.zeros_like(q),
+                    scores=torch.zeros((sequences, kv_heads, capacity), device="cuda"),
+                    k2=torch.zeros((sequences, budget, kv_heads, 128), dtype=torch.bfloat16, device="cuda"),
+                    v2=torch.zeros((sequences, budget, kv_heads, 128), dtype=torch.bfloat16, device="cuda"),
+                    scores2=torch.zeros((sequences, kv_heads, budget), device="cuda"),
+                    kept=torch.zeros((sequences, kv_heads, budget), dtype=torch.int32, device="cuda"),
+                    new=torch.zeros(sequences, dtype=torch.int32, device="cuda"))
+
+    def step(context, b):
+        ops.qk_norm_rope(context, q, keys, table, b["q"], b["k"], positions=positions)
+        ops.attention_accumulate(context, b["q"], k, v, b["out"], b["scores"], b["scores"], scratch, lengths=lengths)
+        ops.evict_kv(context, k, v, b["scores"], b["k2"], b["v2"], b["scores2"], b["kept"], b["new"], 4, 20, lengths=lengths)
+
+    stream, held = torch.cuda.Stream(), buffers()
+    context = ops.prepare_execution_context(stream.cuda_stream)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        step(context, held)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        step(context, held)
+    for turn, n in enumerate(([500, 300, 129], [128, 0, 60], [1, 501, -7], [333, 334, 500])):
+        lengths.copy_(torch.tensor(n, dtype=torch.int32))
+        positions.copy_(torch.randint(-2, 1002, positions.shape, generator=torch.Generator("cuda").manual_seed(turn), device="cuda", dtype=torch.int32))
+        q.copy_(normal(torch, 50 + turn, *q.shape))
+        want = buffers()
+        old = torch.rand(want["scores"].shape, generator=torch.Generator("cuda").manual_seed(90 + turn), device="cuda")
+        want["scores"].copy_(old)
+        for name in held:
+            held[name].copy_(want[name])
+        torch.cuda.synchronize()
+        step(context, want)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for name in held:
+            assert torch.equal(held[name], want[name]), name
+        for s, tokens in enumerate(n):
+            tokens = tokens if 0 <= tokens <= capacity else 0
+            assert int(held["new"][s]) == min(tokens, budget)
+            mine = slice(s * rows, (s + 1) * rows)
+            visible = window_visible(torch, tokens, rows, 1 << 30, 0, capacity)
+            exact, allowance, weights, slack = attention_reference(torch, held["q"][mine], k[s], v[s], visible)
+            expect_attention(torch, held["out"][mine], exact, allowance)
+            total = old[s].double() + weights
+            assert ((held["scores"][s].double() - total).abs() <= slack + 2.0 ** -22 * total).all()
+
+
+@pytest.mark.parametrize("lengths,capacity,budget,sinks,recent", [
+    ([70, 3, 0], 70, 100, 40, 60),                # a budget beyond the capacity, first and latest beyond it too
+    ([900, 64, 65], 150000, 64, 4, 60),           # caches far larger than what they hold; no place for any other
+    ([2000, 1999], 100000, 700, 0, 1),
+    ([41000, 100], 41000, 40, 0, 0),              # a little more than a block keeps, hardly any stay
+    ([100], 100, 1, 1, 0), ([100], 100, 1, 0, 1), ([2], 2, 1, 0, 0),
+])
+def test_eviction_at_its_edges(cuda, package, ctx, lengths, capacity, budget, sinks, recent):
+    torch, ops = cuda, package.operators
+    sequences, kv_heads = len(lengths), 2
+    generator = torch.Generator("cuda").manual_seed(5)
+    k, v = (torch.full((sequences, capacity, kv_heads, 128), math.nan, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    scores = torch.full((sequences, kv_heads, capacity), math.inf, device="cuda")  # of tokens that are not there
+    for s, n in enumerate(lengths):
+        k[s, :n], v[s, :n] = normal(torch, s, n, kv_heads, 128), normal(torch, 70 + s, n, kv_heads, 128)
+        scores[s, :, :n] = torch.randint(0, 9, (kv_heads, n), generator=generator, device="cuda") * 2.0 ** -149  # the smallest numbers
+    k_out, v_out = (torch.full((sequences, budget, kv_heads, 128), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    scores_out = torch.full((sequences, kv_heads, budget), 9.0, device="cuda")
+    kept, new = torch.zeros((sequences, kv_heads, budget), dtype=torch.int32, device="cuda"), torch.zeros(sequences, dtype=torch.int32, device="cuda")
+    ops.evict_kv(ctx, k, v, scores, k_out, v_out, scores_out, kept, new, sinks, recent, lengths=torch.tensor(lengths, dtype=torch.int32, device="cuda"))
+    assert new.tolist() == [min(n, budget) for n in lengths]
+    for s, n in enumerate(lengths):
+        host = scores[s].cpu().tolist()
+        for h in range(kv_heads):
+            want = evict_reference(torch, host[h], n, budget, sinks, recent)
+            assert kept[s, h].tolist() == want + [-1] * (budget - len(want))
+            index = torch.tensor(want, dtype=torch.long, device="cuda")
+            assert torch.equal(k_out[s, :len(want), h], k[s, index, h]) and torch.equal(v_out[s, :len(want), h], v[s, index, h])
+            assert torch.equal(scores_out[s, h, :len(want)], scores[s, h, index])
+        assert (k_out[s, len(want):] == 7).all() and (scores_out[s, :, len(want):] == 9).all()
+
+
+def test_offsets_beyond_32_bits(cuda, package, ctx):
+    """The last of five sequences starts beyond 2^32 elements: many rows, accumulated weights, eviction."""
+    torch, ops = cuda, package.operators
+    sequences, capacity, kv_heads, heads, n = 5, 65536 * 2, 8, 16, 3000
+    k = torch.zeros((sequences * 8, capacity, kv_heads, 128), dtype=torch.bfloat16, device="cuda")[::8]
+    assert k.stride(0) * 4 + 128 > 2 ** 32
+    v = k.clone()
+    k[-1, :n], v[-1, :n] = normal(torch, 1, n, kv_heads, 128), normal(torch, 2, n, kv_heads, 128)
+    lengths = torch.tensor([0] * 4 + [n], dtype=torch.int32, device="cuda")
+    q = normal(torch, 3, sequences * 300, heads, 128)
+    out = torch.empty_like(q)
+    ops.attention_window(ctx, q, k, v, out, 2500, 4, lengths=lengths)
+    want, size, _, _ = attention_reference(torch, q[-300:], k[-1, :n], v[-1, :n], window_visible(torch, n, 300, 2500, 4, n))
+    expect_attention(torch, out[-300:], want, size)
+    assert (out[:-300] == 0).all()
+    q, wide = q[:sequences * 2], torch.zeros((sequences * 1024, kv_heads, capacity), device="cuda")[::1024]
+    assert wide.stride(0) * 4 >= 2 ** 32
+    scratch = torch.empty(ops.attention_accumulate_scratch_bytes(sequences, 2, heads, kv_heads, capacity), dtype=torch.uint8, device="cuda")
+    ops.attention_accumulate(ctx, q, k, v, torch.empty_like(q), wide, wide, scratch, lengths=lengths)
+    _, _, weights, slack = attention_reference(torch, q[-2:], k[-1, :n], v[-1, :n], window_visible(torch, n, 2, 1 << 30, 0, n))
+    assert ((wide[-1, :, :n].double() - weights).abs() <= slack + 2.0 ** -22 * weights).all()
+    assert not wide[:4].any() and not wide[-1, :, n:].any()
+    k_out, v_out = (torch.zeros((sequences, 64, kv_heads, 128), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    scores_out, kept = torch.zeros((sequences, kv_heads, 64), device="cuda"), torch.zeros((sequences, kv_heads, 64), dtype=torch.int32, device="cuda")
+    new = torch.zeros(sequences, dtype=torch.int32, device="cuda")
+    ops.evict_kv(ctx, k, v, wide, k_out, v_out, scores_out, kept, new, 4, 8, lengths=lengths)
+    assert new.tolist() == [0] * 4 + [64]
+    host = wide[-1, :, :n].cpu().tolist()
+    for h in range(kv_heads):
+        want = evict_reference(torch, host[h], n, 64, 4, 8)
+        assert kept[-1, h].tolist() == want
+        index = torch.tensor(want, device="cuda")
+        assert torch.equal(k_out[-1, :, h], k[-1, index, h]) and torch.equal(v_out[-1, :, h], v[-1, index, h])
