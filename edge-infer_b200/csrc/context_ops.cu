@@ -53,8 +53,8 @@ void expect_rows(const ei_view3& v, const char* name) {
 }
 long long row_stride(const ei_view3& v) { return v.shape[0] > 1 ? (long long)v.stride[0] : (long long)(v.shape[1] * v.shape[2]); }
 
-// [sequences, capacity, kv_heads, 128] of any strides that are whole 16 bytes and let no two head rows meet in the simple
-// sense that each axis steps over at least a head row.
+// [sequences, capacity, kv_heads, 128] of any strides that are whole 16 bytes and step over at least a head row each. (Inputs may
+// show one storage twice; outputs are looked at by may_fold as well.)
 CacheStrides expect_cache(const ei_view4& v, const char* name) {
   if (v.data == nullptr || elements(v) == 0) reject(std::string(name) + " have no storage or are empty");
   if (v.shape[3] != kHeadWidth || v.stride[3] != 1) reject(std::string(name) + " must have packed heads of 128 values");

@@ -7,10 +7,11 @@
 // as it stands in the cache is that product's N-major B operand). Scores have two places, so that a tile's are computed while
 // the last one's weights are made: 2 x (64 + 64 + 128) columns are all of the tensor memory.
 //
-// A running maximum may lag the true one by 2^8 (weights up to 256 are as exact in BF16 as those up to 1), so that the
-// outputs are hardly ever taken out of tensor memory to be rescaled; the sum is of the rounded weights, so that those used
-// add up to one exactly. (Outputs are 0.0021 of their size off 64 bits, 0.0019 with the true maximum, whose weight is exactly 1,
-// and 0.0017 rounded from 32-bit arithmetic; the true maximum costs 20 %.)
+// A running maximum may lag the true one by 2^8 (weights up to 256 are as exact in BF16 as those up to 1), as is published for
+// attention on tensor memory, so that the outputs are hardly ever taken out to be rescaled; the sum is of the rounded weights, so
+// that those used add up to one exactly and a row that one token dominates is that token's values. (Outputs are 0.0021 of their
+// size off 64 bits, 0.0019 with the true maximum, whose weight is exactly 1, and 0.0017 rounded from 32-bit arithmetic; the true
+// maximum costs 20 %. The prompts of uniform decoders, whose sum is of unrounded weights, follow the true one.)
 //
 // Tokens are a list of boxes of 32, first those of the sinks, then those of the window of the block's rows; two make a tile, so
 // that a few sinks cost no tile of their own. What a box holds beyond its stretch is masked in the scores and cleared in V.
@@ -22,13 +23,13 @@
 // 1024 (16 a cycle), the products 1280; by leaving parts out in copies, everything but the softmax takes 1200. Two warps a
 // scheduler share the exponentials: alone a warp needs 820 cycles for its 64, beside the other 1200. Sixteen softmax warps, two a
 // row by columns or by turns, came out the same; so did tiles of 128 tokens with one place for the scores, whose halves fall
-// into step and then wait for their products together. 2048 rows of 32 / 8 heads behind 6144 tokens, window 2048: 97 us = 709
-// TFLOP/s (289 us by the few-row kernel); 256 blocks are 1.73 waves, which costs 13 %, and a block some 9 us to start and to leave.
+// into step and then wait for their products together. 2048 rows of 32 / 8 heads behind 6144 tokens, window 2048: 97 to 100 us = 690
+// to 709 TFLOP/s (289 us by the few-row kernel); 256 blocks are 1.73 waves, which costs 13 %, and a block some 9 us to start and to leave.
 //
 // Roles of the twelve warps: 0-3 and 4-7 the weights of one half each, 8 the copies, 9 and 10 the MMAs of one half each, 11 the
 // tensor memory. A stage of the ring of four holds a tile's V and the K of the half's next scores. Every wait is bounded: a role
 // whose wait runs out raises `abort`, which every other wait polls; when all roles have left, the copies and MMAs in flight are
-// waited for (bounded), the block's rows come out as NaN and the tensor memory is freed.
+// waited for (bounded), the block's rows come out as NaN and the tensor memory is freed. The host can ask how often that happened.
 #include "span_attention.cuh"
 
 #include "cluster.cuh"

@@ -15,12 +15,16 @@
 // finishing a part of the rows, so that there is no scratch, no second launch and a fixed order of every addition. What a block
 // says of itself it writes to all blocks ahead of the cluster's barrier: read from one another behind it, block by block, that
 // took 2.7 us of a single token's 10.
-// 64 caches of 256 to 8192 tokens, window 4096, 32 / 8 heads: 128 us = 6.5 TB/s, the measured copy rate. One token over 1028 tokens
+// 64 caches of 256 to 8192 tokens, window 4096, 32 / 8 heads: 129 to 134 us on different B200s = 6.2 to 6.4 TB/s, 94 to 98 % of the
+// measured copy rate. One token over 1028 tokens
 // of one cache: 7.6 us, a chain of launch, length, first copies, tile, join; over 30000 tokens 25 us = 4.9 TB/s. With weights
-// reported, 64 caches of 2304: 101 us (84.5 without).
+// reported, 64 caches of 2304: 100 to 103 us (84.5 without).
 //
 // Only tokens that some row of the unit sees are read: tiles start at the window's first token, sinks are a stretch of their
 // own. What a box brings beyond a stretch (other tokens, rows never written) is masked in the scores and cleared in V.
+//
+// Every wait is bounded. A warp whose wait runs out waits (bounded) for its copies in flight and joins with NaN: its unit's rows come
+// out as NaN and add nothing to reported weights, and the host can ask how often that happened.
 #include "step_attention.cuh"
 
 #include "cluster.cuh"

@@ -174,11 +174,14 @@ ei_status ei_attention_prefill_static_bf16(const ei_context* ctx, ei_view3 q, ei
  * null: `length` for every sequence. Row r of a sequence of n tokens stands at position n - rows + r. A row of negative
  * position (a sequence shorter than its rows: padding on the left) comes out as zeros, and so does every row of a sequence
  * whose length lies outside 0 .. capacity, which counts as empty. Keys and values that no row of the call may see are never
- * used, whatever they hold. Scores, weights' sums and products are FP32, weights are rounded to BF16 for the product with the
- * values, outputs once. `out` may be the queries' own view, else it lies apart from every input. The context's device has to be
- * the current one; device pointers must belong to it. Nothing is allocated; results do not change from call to call; scratch is
- * used until the call's work is done, so calls that may overlap need scratch of their own. A first call on a device sets kernels
- * up: make it before a stream capture. Should a copy not arrive within its bounded wait (some half a second), the rows that
+ * used, whatever they hold. A value that is no number and that some row sees takes its column (of its sequence and KV head) of
+ * that row, and may take the same column of the call's rows that do not see it; a key takes the rows that see it. Scores, weights'
+ * sums and products are FP32, weights are rounded to BF16 for the product with the values, outputs once. `out` may be the queries'
+ * own view, else it lies apart from every input; views that may meet where they must not, or integers off their 4-byte alignment,
+ * are refused. The context's device has to be the current one; device pointers must belong to it. Nothing is allocated; results do
+ * not change from call to call; scratch is used until the call's work is done, so calls that may overlap need scratch of their
+ * own. The process's first call of an operator on a device sets its kernels up: make it, with the sizes that will be captured,
+ * before a stream capture. Should a copy not arrive within its bounded wait (some half a second), the rows that
  * needed it come out as NaN and add nothing to accumulated weights; ei_context_expired_waits counts it. */
 
 /* How many bounded waits of these operators have run out on the context's device since the library was loaded, on any stream. Waits
