@@ -110,7 +110,10 @@ __global__ void __launch_bounds__(kThreads, 1) span_attention_kernel(const __gri
   SpanShared* const sh = reinterpret_cast<SpanShared*>(ring + kStages * kStageBytes);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 9 * 32) prefetch_map(&p.k_tile_map), prefetch_map(&p.v_tile_map), prefetch_map(&p.q_map);
+  if (threadIdx.x == 9 * 32) {
+    prefetch_map(&p.k_tile_map), prefetch_map(&p.v_tile_map);
+    if (p.copied_queries) prefetch_map(&p.q_map);  // encoded only then
+  }
   const int kv_head = blockIdx.x, sequence = blockIdx.z;
   const int group = p.heads / p.kv_heads, stacked = p.rows * group;
 

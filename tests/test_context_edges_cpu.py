@@ -260,3 +260,9 @@ def test_cases_run_on_the_kernels_they_are_named_for(tmp_path):
         for name, c in cases.items():
             got = prefix(c.sequences * c.rows * c.heads // c.kv_heads, c.prefix, c.kv_heads)
             assert got == [int(c.kernel == "many"), c.cluster or 0], name
+
+
+def test_only_an_encoded_query_map_is_prefetched():
+    """Groups that no box copies leave the map as it is."""
+    text = (ROOT / "edge-infer_b200" / "csrc" / "span_attention.cu").read_text()
+    assert text.count("prefetch_map(&p.q_map)") == text.count("if (p.copied_queries) prefetch_map(&p.q_map)") == 1
