@@ -17,7 +17,9 @@ namespace {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMoves = 4;          // tokens a warp has under way
-constexpr int kCachedKeys = 40960;  // keys that a block holds itself (160 KB); further ones are made from the scores again
+// Keys that a block holds itself (160 KB); further ones are made from the scores again. The room goes by the capacity, the lengths
+// being on the device: at a capacity of 40960 one block fits an SM, and 64 caches of 2304 tokens take 246 us instead of 182.
+constexpr int kCachedKeys = 40960;
 
 constexpr int kBins = 2048;
 
