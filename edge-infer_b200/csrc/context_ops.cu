@@ -297,6 +297,9 @@ ei_status ei_context_expired_waits(const ei_context* ctx, uint64_t* count) {
     cudaStream_t stream = stream_of(ctx);
     if (!count) reject("the count of expired waits needs a place");
     expect_current_device(ctx);
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    EI_CUDA(cudaStreamIsCapturing(stream, &capturing));
+    if (capturing != cudaStreamCaptureStatusNone) reject("expired waits are counted when the stream gets there, which a captured one does not");
     *count = uint64_t(step_expired_waits(stream)) + span_expired_waits(stream);
   });
 }

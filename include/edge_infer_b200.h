@@ -185,7 +185,7 @@ ei_status ei_attention_prefill_static_bf16(const ei_context* ctx, ei_view3 q, ei
  * needed it come out as NaN and add nothing to accumulated weights; ei_context_expired_waits counts it. */
 
 /* How many bounded waits of these operators have run out on the context's device since the library was loaded, on any stream. Waits
- * for the context's stream first (so it cannot be captured): when the count has not grown, nothing that this stream has run since
+ * for the context's stream first (and is refused while that is captured): when the count has not grown, nothing that this stream has run since
  * gave up. */
 ei_status ei_context_expired_waits(const ei_context* ctx, uint64_t* count);
 

@@ -664,3 +664,22 @@ def test_offsets_beyond_32_bits(cuda, package, ctx):
         assert kept[-1, h].tolist() == want
         index = torch.tensor(want, device="cuda")
         assert torch.equal(k_out[-1, :, h], k[-1, index, h]) and torch.equal(v_out[-1, :, h], v[-1, index, h])
+
+
+def test_counting_expired_waits_leaves_a_capture_alone(cuda, package):
+    """Refused while the stream is captured, and the capture goes on."""
+    torch, ops, c = cuda, package.operators, context_cases.FEW
+    q, k, v = inputs_of(torch, c)
+    out, want, stream, graph = torch.zeros_like(q), torch.empty_like(q), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    context = ops.prepare_execution_context(stream.cuda_stream)
+    with torch.cuda.stream(stream):
+        window_call(torch, ops, context, c, q, k, v, want)
+    torch.cuda.synchronize()
+    before = ops.expired_waits(context)
+    with torch.cuda.graph(graph, stream=stream):
+        with pytest.raises(ValueError, match="captured"):
+            ops.expired_waits(context)
+        window_call(torch, ops, context, c, q, k, v, out)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and ops.expired_waits(context) == before
